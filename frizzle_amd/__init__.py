@@ -5,7 +5,7 @@ The compute runs in libfrizzle_hip.so, a HIP library with a C ABI
 package does not load the library; the first call that needs it does, and
 raises if it has not been built.
 """
-from ._lib import FrzError, exported_symbols, load
+from ._lib import Adapters, FrzError, Pages, exported_symbols, load
 from .runtime import (CAPTURE_SLOTS, PREFILL_BF16, PREFILL_EXACT, Q4_0, Q4_1, Q8_0,
                       TO_THE_END, Device,
                       DeviceArray, Edit, EditError, EditKind, Model, block_split,
@@ -15,7 +15,7 @@ from .runtime import (CAPTURE_SLOTS, PREFILL_BF16, PREFILL_EXACT, Q4_0, Q4_1, Q8
                       tensor_bytes)
 
 __all__ = [
-    "FrzError", "exported_symbols", "load", "CAPTURE_SLOTS", "PREFILL_BF16", "PREFILL_EXACT",
+    "Adapters", "FrzError", "Pages", "exported_symbols", "load", "CAPTURE_SLOTS", "PREFILL_BF16", "PREFILL_EXACT",
     "Q4_0", "Q4_1", "Q8_0",
     "capture_layout", "capture_words",
     "TO_THE_END", "Device", "block_split",

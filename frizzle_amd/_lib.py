@@ -63,6 +63,21 @@ class LoadPolicy(ctypes.Structure):
     _fields_ = [("memory_budget", c_uint64), ("rollback_reserve", c_uint32)]
 
 
+class Pages(ctypes.Structure):
+    """frz_pages: caches in pages, by their device addresses."""
+    _fields_ = [("keys", c_void_p), ("values", c_void_p), ("format", c_int),
+                ("kv_heads", c_int), ("head_dim", c_int), ("page_slots", c_uint32),
+                ("pages", c_uint32), ("page_stride", c_uint64), ("table", c_void_p),
+                ("sequences", c_uint32), ("width", c_uint32)]
+
+
+class Adapters(ctypes.Structure):
+    """frz_adapters: a projection's low-rank adapters, by their device addresses."""
+    _fields_ = [("format", c_int), ("count", c_uint32), ("rank", c_int), ("cols", c_int),
+                ("rows", c_int), ("down", c_void_p), ("up", c_void_p), ("ranks", c_void_p),
+                ("scales", c_void_p)]
+
+
 class Range(ctypes.Structure):
     _fields_ = [("buffer", c_uint32), ("offset", c_uint64), ("length", c_uint64)]
 
@@ -154,6 +169,12 @@ _SIGS = {
     "frz_op_topk": (c_int, [_P, _P, c_int, _P]),
     "frz_op_draw": (c_int, [_P, _P, POINTER(Sampling), c_uint32, c_uint32,
                             _P]),
+    "frz_op_rope_paged": (c_int, [_P, POINTER(Pages), _P, _P, _P, _P, _P, _P, _P, _P, c_int,
+                                  c_int, _P, c_int, c_int, c_float, c_uint32]),
+    "frz_op_attention_paged": (c_int, [_P, POINTER(Pages), _P, _P, _P, c_int, _P, c_int, c_int,
+                                       c_uint32, c_float, c_uint32]),
+    "frz_op_adapters": (c_int, [_P, POINTER(Adapters), _P, _P, c_int, _P, c_int, _P, c_int,
+                                c_uint32]),
     "frz_op_numerics": (c_int, [_P, c_int, _P, _P, c_int]),
     "frz_bench_launch_floor": (c_int, [_P, c_int, c_int, POINTER(c_double)]),
     "frz_bench_stream": (c_int, [_P, POINTER(c_void_p), c_int, c_uint64, _P, c_int, c_int,

@@ -26,6 +26,9 @@ struct frz_device {
   // 1,048,576 logits; longer calls allocate their own): an allocation and
   // its free, which waits for the device, cost more than the selection.
   uint32_t* topk_scratch = nullptr;
+  // The workspace of the ops over a batch of requests (batch_api.hip), there
+  // from the first of them on; their work, and so its use, is in stream order.
+  void* batch_scratch = nullptr;
   // Held while a one-kernel op enqueues its launches, so that ops of several
   // threads run one after another: they share the stream and what is above.
   std::mutex ops;

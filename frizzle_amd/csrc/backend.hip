@@ -236,6 +236,7 @@ void frz_close(frz_device* dev) {
   if (!dev) return;
   (void)hipSetDevice(dev->ordinal);
   (void)hipStreamSynchronize(dev->stream);
+  if (dev->batch_scratch) (void)hipFree(dev->batch_scratch);
   (void)hipFree(dev->topk_scratch);
   (void)hipFree(dev->step);
   (void)hipStreamDestroy(dev->stream);

@@ -1,0 +1,98 @@
+// Where a batch of requests finds its keys and how its work is cut, from
+// sizes alone (no HIP, so that a test can compile it by itself).
+//
+// A request's keys lie in pages: slot s of its key p / page_slots is
+// p % page_slots, and the page's number stands in the request's row of the
+// table. A row of the batch reads the keys (p - window, p]; those past the
+// table's width, or in a page that the pool does not have, are not there.
+//
+// Attention's work is counted in blocks of 32 keys, which lie by position, a
+// row's keys' blocks taken by each of its head blocks (a key-value head with
+// up to 16 of its query heads). A row of n blocks is cut into ceil(n / chunk)
+// parts, a workgroup each, for one chunk that the whole batch shares: a batch
+// of one long and many short requests then keeps every compute unit at work,
+// where a cut of so many parts a row would leave the long one last. The chunk
+// is a multiple of the workgroup's waves, a block a wave and turn.
+
+#pragma once
+
+#include <stdint.h>
+
+#if defined(__HIPCC__)
+#define FRZ_RULE __host__ __device__ inline
+#else
+#define FRZ_RULE inline
+#endif
+
+namespace frz {
+namespace rules {
+
+constexpr uint32_t kNone = 0xFFFFFFFFu;  // no position, no page, no adapter
+
+// ---- pages -------------------------------------------------------------------
+
+// The page that holds a sequence's `index`-th page of keys, or kNone.
+FRZ_RULE uint32_t page_at(const uint32_t* table, uint32_t sequences, uint32_t width,
+                          uint32_t pages, uint32_t sequence, uint32_t index) {
+  if (sequence >= sequences || index >= width) return kNone;
+  const uint32_t page = table[(uint64_t)sequence * width + index];
+  return page < pages ? page : kNone;
+}
+
+// The most keys of a sequence: positions stay below 2^24, which F32 holds.
+constexpr uint64_t kMostKeys = 1u << 24;
+
+// ---- attention's parts -------------------------------------------------------
+
+constexpr uint32_t kBlockKeys = 32;
+constexpr uint32_t kPartWaves = 4;   // a part's workgroup
+constexpr uint32_t kHeadBlock = 16;  // query heads that share a part at most
+constexpr uint32_t kMostRows = 512;
+
+// The keys [first, end) that a row at `position` reads of a sequence whose
+// table holds `capacity`.
+struct KeyRange {
+  uint32_t first, end;
+};
+FRZ_RULE KeyRange key_range(uint32_t position, uint32_t window, uint32_t capacity) {
+  KeyRange r;
+  const uint32_t after = position + 1;  // position is not kNone
+  r.first = after > window ? after - window : 0;
+  r.end = after < capacity ? after : capacity;
+  if (r.first > r.end) r.first = r.end;
+  return r;
+}
+
+// Blocks of a row's keys; one where it has none, so that its output is written.
+FRZ_RULE uint32_t row_blocks(KeyRange r) {
+  if (r.first >= r.end) return 1;
+  return (r.end + kBlockKeys - 1) / kBlockKeys - r.first / kBlockKeys;
+}
+
+// Parts that a batch aims for: what its `units` (rows times head blocks) leave
+// of the workgroups that run at once, so that all parts of few long rows run
+// together; two for each of those where the rows alone nearly fill them.
+FRZ_RULE uint32_t part_target(uint32_t units, uint32_t at_once) {
+  return units <= at_once / 2 ? at_once - units : 2 * at_once;
+}
+
+// Blocks of a part, for the batch's blocks in all (each row's counted once a
+// head block).
+FRZ_RULE uint32_t part_chunk(uint64_t blocks, uint32_t target) {
+  const uint64_t even = (blocks + target - 1) / target;
+  return (uint32_t)((even + kPartWaves - 1) / kPartWaves * kPartWaves);
+}
+
+// The most parts there can be (a row has less than one part more than its
+// blocks fill), and the most that belong to rows of several parts: such a row
+// has fewer than twice the parts that its blocks fill.
+FRZ_RULE uint32_t most_parts(uint32_t units, uint32_t at_once) {
+  return part_target(units, at_once) + units;
+}
+FRZ_RULE uint32_t most_joined_parts(uint32_t units, uint32_t at_once) {
+  const uint32_t all = most_parts(units, at_once), twice = 2 * part_target(units, at_once);
+  return all < twice ? all : twice;
+}
+
+}  // namespace rules
+}  // namespace frz

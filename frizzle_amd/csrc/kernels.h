@@ -428,6 +428,93 @@ hipError_t launch_edit(hipStream_t s, const DevStep* step,
                        const uint32_t* edits, int layer, float* act,
                        int width, int max_tokens);
 
+// ---- a step of many requests ----------------------------------------------
+// Caches in pages (frz_pages), and where a row's are found (batch_rules.h).
+struct PagedCache {
+  uint16_t* keys;
+  uint16_t* values;
+  bool bf16;  // else F16
+  uint32_t kv_heads;
+  uint32_t head_dim;
+  uint32_t page_slots;
+  uint32_t pages;
+  uint64_t page_stride;  // values
+  const uint32_t* table;
+  uint32_t sequences;
+  uint32_t width;
+};
+
+struct PagedRopeArgs {
+  PagedCache cache;
+  const uint32_t* sequences;  // null: row r's is r
+  const uint32_t* positions;
+  const float* turns;
+  const float* query_gain;
+  const float* key_gain;
+  const float* query;
+  const float* key;
+  const float* value;
+  uint32_t q_stride;
+  uint32_t kv_stride;
+  float* roped;
+  uint32_t roped_stride;
+  uint32_t query_heads;
+  float epsilon;
+  uint32_t rows;
+};
+hipError_t launch_paged_rope(hipStream_t s, const PagedRopeArgs& a);
+
+struct PagedAttentionArgs {
+  PagedCache cache;
+  const uint32_t* sequences;
+  const uint32_t* positions;
+  const float* query;
+  uint32_t q_stride;
+  float* out;
+  uint32_t out_stride;
+  uint32_t query_heads;
+  uint32_t window;
+  float scale_log2e;
+  uint32_t rows;
+  // The states of rows cut into several parts: [kMostJoinedParts][16 heads]
+  // of head_dim outputs, and of (m, l); a record of each such row and head
+  // block, and their number.
+  float* states;
+  float* stats;
+  uint4* records;
+  uint32_t* record_count;
+  uint32_t units = 0, target = 0;  // set by the launcher
+};
+constexpr int kMostComputeUnits = 256;  // gfx950's
+constexpr int kAttentionWorkgroups = 2;  // a compute unit's at once
+constexpr int kMostJoinedParts = 4 * kAttentionWorkgroups * kMostComputeUnits;
+hipError_t launch_paged_attention(hipStream_t s, const PagedAttentionArgs& a, int compute_units);
+
+struct AdapterArgs {
+  const void* down;  // [count][rank][cols]
+  const void* up;    // [count][rows][rank]
+  int format;        // GGUF's: 0 F32, 1 F16, 30 BF16
+  uint32_t count;
+  int rank;
+  int cols;
+  int rows;
+  const uint32_t* ranks;  // null: all rank
+  const float* scales;    // null: all 1
+  const uint32_t* which;
+  const float* x;
+  int x_stride;
+  const float* base;
+  int base_stride;
+  float* y;
+  int y_stride;
+  uint32_t tokens;
+  float* low;        // [splits][tokens][rank]
+  int splits = 0, split_cols = 0;  // set by the launcher
+};
+constexpr int kMostAdapterRank = 128;
+constexpr int kMostAdapterSplits = 32;
+hipError_t launch_adapters(hipStream_t s, const AdapterArgs& a);
+
 // ---- output ------------------------------------------------------------
 // Top-64 of `count` logits into candidates (64 x {bits, token}), sorted;
 // `scratch` holds topk_scratch_words(count) words.

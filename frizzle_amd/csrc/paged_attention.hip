@@ -1,0 +1,658 @@
+// Attention of a batch's rows, one token each, over caches in pages.
+//
+// A row's keys are cut into parts (batch_rules.h), a workgroup each: one
+// key-value head and up to 16 of its query heads. A wave takes every fourth
+// of the part's blocks of 32 keys with a running maximum m, sum l and output
+// O of its own; the part's waves are joined through LDS, the parts of a row
+// that has several by a second launch, in order.
+//
+// What bounds it is the stream of key and value rows, so nothing of it waits:
+// both go from memory to the registers that the matrix instructions read,
+// with no LDS between, a block's values requested before its scores are
+// formed and the next block's keys right after.
+//   S^T = K q^T   16 keys a tile, A = K: lane (n, g) holds 8 of key n's
+//                 values, as they lie in memory. It leaves the lane with the
+//                 scores of head n at keys 4g .. 4g + 3.
+//   O^T += V^T P  B = P: those same keys, of both of a block's tiles, are
+//                 the lane's 8 of the 32 that an instruction sums, so P needs
+//                 no move; A = V: the lane's 8 keys' rows at dimensions 8n ..,
+//                 paired up two keys a register by v_perm. O^T leaves each
+//                 lane one head, so m and l stay a lane's own.
+//
+// The matrix cores take 16-bit operands, the cache's type; the query and the
+// weights are F32. Each is split into parts that add up to it, hi + lo of F16
+// (to 2^-22) or three of BF16 (2^-24), which are further columns of the same
+// instruction where the heads leave some free: columns n and n + W belong to
+// one head, W the next of 4, 8 or 16 above the heads. A head's query is
+// scaled by a power of two to lie below 2^15, weights by 2^14, so that their
+// low parts stay clear of the formats' smallest values; both scales are
+// exact. Products are exact in F32, sums F32.
+//
+// Keys outside the row's range or in no page are never read: a lane's row is
+// clamped to one that the row reads, and its score is -inf.
+
+#include <math.h>
+
+#include "batch_rules.h"
+#include "kernels.h"
+#include "numerics.h"
+
+namespace frz {
+namespace {
+
+using namespace rules;
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 64 * kPartWaves;
+constexpr float kWeightScale = 14.0f;  // weights are 2^14 at the running maximum
+constexpr float kMinusInf = -__builtin_inff();
+
+template <bool kBf16>
+struct Types;
+template <>
+struct Types<false> {
+  typedef half8 vec;
+  typedef _Float16 scalar;
+  static constexpr int kParts = 2;
+  static __device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a),
+                                                  __builtin_bit_cast(half8, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct Types<true> {
+  typedef bf16x8 vec;
+  typedef __bf16 scalar;
+  static constexpr int kParts = 3;
+  static __device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+};
+
+// The shapes a kernel is compiled for.
+template <int kD, bool kBf16, int kW>
+struct Shape {
+  static constexpr int kParts = Types<kBf16>::kParts;
+  static constexpr int kPerTile = 16 / kW;                              // parts a column tile holds
+  static constexpr int kTiles = (kParts + kPerTile - 1) / kPerTile;     // column tiles
+  static constexpr int kChunks = kD / 32;                               // of a key row
+  static constexpr int kVec = kD >= 128 ? 8 : 4;                        // values a lane loads at once
+  static constexpr int kSpans = kD / (16 * kVec);                       // of a value row
+};
+
+// Workgroups a compute unit runs at once: the registers of heads of 256 leave
+// room for one.
+template <int kD>
+constexpr int kWorkgroups = kD == 256 ? 1 : kAttentionWorkgroups;
+
+// Part `part` of x, of which the parts add up: x rounded, what that left
+// rounded, and so on; 0 past the format's parts.
+template <bool kBf16>
+__device__ __forceinline__ typename Types<kBf16>::scalar split_part(float x, int part) {
+  typedef typename Types<kBf16>::scalar T;
+  const T hi = (T)x;
+  float rest = x - (float)hi;
+  const T lo = (T)rest;
+  T r = part == 0 ? hi : lo;
+  if constexpr (kBf16) {
+    rest -= (float)lo;
+    r = part == 2 ? (T)rest : r;
+  }
+  return part < Types<kBf16>::kParts ? r : (T)0.0f;
+}
+
+// x of the lanes 32 and 16 away, reduced with the lane's own: every lane of
+// the four that share n = lane % 16 gets all four's result.
+template <typename Op>
+__device__ __forceinline__ float across_groups(float x, Op op) {
+  float a = x, b = x;
+  asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+  x = op(a, b);
+  a = x;
+  b = x;
+  asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+  return op(a, b);
+}
+
+template <int kShift>
+__device__ __forceinline__ float row_rotated(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x),
+                                                               0x120 + kShift, 0xF, 0xF, true));
+}
+
+// A head's columns summed, into each of them.
+template <int kW>
+__device__ __forceinline__ float across_columns(float x) {
+  if constexpr (kW <= 8) x += row_rotated<8>(x);
+  if constexpr (kW <= 4) x += row_rotated<4>(x);
+  return x;
+}
+
+__device__ __forceinline__ uint32_t wave_sum_before(uint32_t x, int lane, uint32_t* total) {
+  uint32_t sum = x;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t up = __shfl_up(sum, o);
+    if (lane >= o) sum += up;
+  }
+  *total = __shfl(sum, 63);
+  return sum - x;
+}
+
+// What a workgroup works on.
+struct Part {
+  uint32_t row, position, sequence;
+  uint32_t unit;         // the row's head block
+  uint32_t index, parts; // of the unit's parts
+  uint32_t chunk;
+  uint32_t slot;         // the unit's first state, where it has several parts
+  uint32_t record;       // the unit's number among those
+  uint32_t records;      // of them
+};
+
+// The part numbered `want`, found by each wave for itself from the rows'
+// positions: the rows' blocks give the chunk, the chunk each row's parts,
+// and those the row. False past the last part (but for the records' number).
+__device__ __forceinline__ bool find_part(const PagedAttentionArgs& a, uint32_t want, int lane,
+                                          Part* out) {
+  constexpr int kPer = kMostRows / 64;
+  const uint32_t per = (a.rows + 63) / 64, capacity = a.cache.width * a.cache.page_slots;
+  uint32_t position[kPer], sequence[kPer], blocks[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const uint32_t r = lane * per + i;
+    const bool live = (uint32_t)i < per && r < a.rows;
+    position[i] = live ? a.positions[r] : kNone;
+    sequence[i] = live && a.sequences ? a.sequences[r] : r;
+  }
+  uint32_t mine = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const uint32_t held = sequence[i] < a.cache.sequences ? capacity : 0;
+    blocks[i] = position[i] == kNone ? 0 : row_blocks(key_range(position[i], a.window, held));
+    mine += blocks[i];
+  }
+  uint32_t all;
+  wave_sum_before(mine, lane, &all);
+  const uint32_t chunk = part_chunk((uint64_t)all * a.units, a.target);
+  uint32_t parts[kPer], total = 0, joined = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    parts[i] = chunk ? (blocks[i] + chunk - 1) / chunk : 0;
+    total += parts[i];
+    joined += parts[i] > 1 ? parts[i] + (1u << 20) : 0;  // parts, and rows above them
+  }
+  // Sums of rows' parts stay below 2^20, all their parts of one head block.
+  uint32_t count, joins;
+  uint32_t before = wave_sum_before(total, lane, &count);
+  uint32_t joined_before = wave_sum_before(joined, lane, &joins);
+  out->records = (joins >> 20) * a.units;
+  const bool owner = want >= before * a.units && want < (before + total) * a.units;
+  const uint64_t owners = __ballot(owner);
+  if (owners == 0) return false;
+  const int leader = __builtin_ctzll(owners);
+  Part p{};
+  uint32_t rest = want - before * a.units;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (p.parts == 0) {
+      if (rest < parts[i] * a.units) {
+        p.row = lane * per + i;
+        p.position = position[i];
+        p.sequence = sequence[i];
+        p.parts = parts[i];
+      } else {
+        rest -= parts[i] * a.units;
+        joined_before += parts[i] > 1 ? parts[i] + (1u << 20) : 0;
+      }
+    }
+  }
+  auto lead = [&](uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, leader); };
+  out->row = lead(p.row);
+  out->position = lead(p.position);
+  out->sequence = lead(p.sequence);
+  out->parts = lead(p.parts);
+  rest = lead(rest);
+  joined_before = lead(joined_before);
+  out->chunk = chunk;
+  // Neighbouring workgroups take the head blocks of the same keys, whose
+  // rows lie side by side.
+  out->unit = rest % a.units;
+  out->index = rest / a.units;
+  const uint32_t mask = (1u << 20) - 1;
+  out->slot = (joined_before & mask) * a.units + out->unit * out->parts;
+  out->record = (joined_before >> 20) * a.units + out->unit;
+  return true;
+}
+
+template <int kD, bool kBf16, int kW>
+__global__ __launch_bounds__(kThreads, kWorkgroups<kD>) void paged_attention_kernel(
+    PagedAttentionArgs a) {
+  typedef Shape<kD, kBf16, kW> S;
+  typedef Types<kBf16> T;
+  constexpr int kPitch = kD + 8;  // floats a head's outputs take in LDS
+  __shared__ __attribute__((aligned(16))) float joined_out[kPartWaves][kW * kPitch];
+  __shared__ float joined_m[kPartWaves][kW], joined_l[kPartWaves][kW];
+  const int lane = threadIdx.x & 63;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int n = lane & 15, g = lane >> 4;
+
+  Part part;
+  const bool found = find_part(a, blockIdx.x, lane, &part);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.record_count = part.records;
+  if (!found) return;
+  const uint32_t head_blocks = a.units / a.cache.kv_heads;
+  const uint32_t kv = part.unit / head_blocks;
+  const uint32_t group = a.query_heads / a.cache.kv_heads;
+  const uint32_t head0 = kv * group + part.unit % head_blocks * kHeadBlock;
+  const uint32_t heads = min(group - part.unit % head_blocks * kHeadBlock, kHeadBlock);
+
+  // The part's keys and the wave's blocks of them.
+  const uint32_t held = part.sequence < a.cache.sequences
+                            ? a.cache.width * a.cache.page_slots : 0;
+  const KeyRange keys = key_range(part.position, a.window, held);
+  const uint32_t base_block = keys.first / kBlockKeys;
+  const uint32_t last_block = base_block + min((part.index + 1) * part.chunk, row_blocks(keys));
+  const uint32_t first_block = base_block + part.index * part.chunk;
+
+  // The wave's next 32 blocks' pages, a lane a half block of 16 keys: where
+  // that half's first key lies in the pool, in values, or ~0.
+  const uint64_t row_stride = (uint64_t)a.cache.kv_heads * kD;
+  auto find_pages = [&](uint32_t block) {
+    const uint32_t key = (block + kPartWaves * (lane >> 1)) * kBlockKeys + 16 * (lane & 1);
+    uint64_t at = ~0ull;
+    if (key < keys.end && key + 16 > keys.first) {
+      const uint32_t index = key / a.cache.page_slots;
+      const uint32_t page = page_at(a.cache.table, a.cache.sequences, a.cache.width,
+                                    a.cache.pages, part.sequence, index);
+      if (page != kNone)
+        at = page * a.cache.page_stride + (key - index * a.cache.page_slots) * row_stride;
+    }
+    return at;
+  };
+  uint32_t block = first_block + wave;
+  uint64_t pages = find_pages(block);
+
+  // The query's columns: column n of tile t is part t kPerTile + n / W of
+  // head n % W.
+  const uint32_t head = n % kW;
+  float scale;  // what turns the scaled query's products into log2 units
+  uint4 q[S::kTiles][S::kChunks];
+  {
+    const bool live = head < heads;
+    const float* src =
+        a.query + (uint64_t)part.row * a.q_stride + (uint64_t)(head0 + (live ? head : 0)) * kD;
+    float x[S::kChunks][8];
+    float most = 0.0f;
+#pragma unroll
+    for (int c = 0; c < S::kChunks; ++c) {
+      const float4 lo = *reinterpret_cast<const float4*>(src + 32 * c + 8 * g);
+      const float4 hi = *reinterpret_cast<const float4*>(src + 32 * c + 8 * g + 4);
+      const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[c][i] = live ? v[i] : 0.0f;
+        most = __builtin_fmaxf(most, __builtin_fabsf(x[c][i]));
+      }
+    }
+    most = across_groups(most, [](float p, float r) { return __builtin_fmaxf(p, r); });
+    // 2^up takes the largest to [2^14, 2^15); zeros, infinities and the
+    // smallest values as far as both factors stay ordinary numbers.
+    int up = 141 - (int)(float_to_bits(most) >> 23);
+    up = up > 100 ? 100 : up < -100 ? -100 : up;
+    const float factor = bits_to_float((uint32_t)(127 + up) << 23);
+    scale = a.scale_log2e * bits_to_float((uint32_t)(127 - up) << 23);
+#pragma unroll
+    for (int t = 0; t < S::kTiles; ++t)
+#pragma unroll
+      for (int c = 0; c < S::kChunks; ++c) {
+        typename T::vec v;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          v[i] = split_part<kBf16>(x[c][i] * factor, t * S::kPerTile + n / kW);
+        q[t][c] = __builtin_bit_cast(uint4, v);
+      }
+  }
+
+  const uint16_t* key_pool = a.cache.keys + (uint64_t)kv * kD;
+  const uint16_t* value_pool = a.cache.values + (uint64_t)kv * kD;
+
+  // A block: where its halves lie, and which of each half's 16 keys the row
+  // reads. A half without keys takes the other's rows.
+  struct Block {
+    uint64_t at[2];
+    int lo[2], hi[2];    // live keys of each half
+    int from[2], to[2];  // rows that may be read at `at`
+  };
+  auto locate = [&](uint32_t b, uint32_t turn, Block* k) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int from = 2 * turn + h;
+      const uint32_t low = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)pages, from);
+      const uint32_t high = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(pages >> 32), from);
+      k->at[h] = (uint64_t)high << 32 | low;
+      const int key = (int)(b * kBlockKeys + 16 * h);
+      k->lo[h] = max(0, (int)keys.first - key);
+      k->hi[h] = k->at[h] == ~0ull ? 0 : min(16, (int)keys.end - key);
+      k->from[h] = k->lo[h];
+      k->to[h] = k->hi[h];
+    }
+    const bool some[2] = {k->lo[0] < k->hi[0], k->lo[1] < k->hi[1]};
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (!some[h]) {
+        k->at[h] = k->at[1 - h];
+        k->from[h] = k->lo[1 - h];
+        k->to[h] = k->hi[1 - h];
+      }
+    return some[0] || some[1];
+  };
+  uint4 key_rows[2][S::kChunks];
+  auto load_keys = [&](const Block& k) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint16_t* src = key_pool + k.at[h];
+      const uint32_t at = min(max(n, k.from[h]), k.to[h] - 1) * (uint32_t)row_stride + 8 * g;
+#pragma unroll
+      for (int c = 0; c < S::kChunks; ++c)
+        key_rows[h][c] = *reinterpret_cast<const uint4*>(src + at + 32 * c);
+    }
+  };
+  uint4 value_rows[2][4][S::kSpans];
+  auto load_values = [&](const Block& k) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint16_t* src = value_pool + k.at[h];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t at =
+            min(max(4 * g + e, k.from[h]), k.to[h] - 1) * (uint32_t)row_stride + S::kVec * n;
+#pragma unroll
+        for (int s = 0; s < S::kSpans; ++s) {
+          if constexpr (S::kVec == 8) {
+            value_rows[h][e][s] = *reinterpret_cast<const uint4*>(src + at + 128 * s);
+          } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(src + at);
+            value_rows[h][e][s] = make_uint4(v.x, v.y, 0, 0);
+          }
+        }
+      }
+    }
+  };
+
+  f32x4 out[S::kSpans][S::kVec];
+#pragma unroll
+  for (int s = 0; s < S::kSpans; ++s)
+#pragma unroll
+    for (int j = 0; j < S::kVec; ++j) out[s][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  float m = kMinusInf, l = 0.0f;  // m less kWeightScale, once there is a key
+
+  uint32_t turn = 0;
+  Block now, next;
+  // The first block from `block` on that holds a key; `turn` counts the
+  // blocks whose pages are known.
+  auto seek = [&](Block* k) {
+    for (; block < last_block; block += kPartWaves, ++turn) {
+      if (turn == 32) {
+        pages = find_pages(block);
+        turn = 0;
+      }
+      if (locate(block, turn, k)) return true;
+    }
+    return false;
+  };
+  bool more = seek(&now);
+  if (more) load_keys(now);
+  while (more) {
+    load_values(now);
+    f32x4 scores[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      scores[h] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < S::kChunks; ++c)
+#pragma unroll
+        for (int t = 0; t < S::kTiles; ++t)
+          scores[h] = T::mfma(key_rows[h][c], q[t][c], scores[h]);
+    }
+    block += kPartWaves;
+    ++turn;
+    more = seek(&next);
+    if (more) load_keys(next);
+
+    float most = kMinusInf;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float s = across_columns<kW>(scores[h][e]) * scale;
+        const bool live = 4 * g + e >= now.lo[h] && 4 * g + e < now.hi[h];
+        scores[h][e] = live ? s : kMinusInf;
+        most = __builtin_fmaxf(most, scores[h][e]);
+      }
+    most = across_groups(most, [](float p, float r) { return __builtin_fmaxf(p, r); });
+    // A block that is worked on holds a key, so `most` is a number but where
+    // scores are not.
+    const float to = __builtin_fmaxf(m, most - kWeightScale);
+    if (__ballot(to > m)) {
+      const float old = __builtin_amdgcn_exp2f(m - to);
+      l *= old;
+#pragma unroll
+      for (int s = 0; s < S::kSpans; ++s)
+#pragma unroll
+        for (int j = 0; j < S::kVec; ++j) out[s][j] *= old;
+      m = to;
+    }
+    float weight[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      weight[i] = __builtin_amdgcn_exp2f(scores[i >> 2][i & 3] - m);
+      l += weight[i];
+    }
+    uint4 w[S::kTiles];
+#pragma unroll
+    for (int t = 0; t < S::kTiles; ++t) {
+      typename T::vec v;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        v[i] = split_part<kBf16>(weight[i], t * S::kPerTile + n / kW);
+      w[t] = __builtin_bit_cast(uint4, v);
+    }
+#pragma unroll
+    for (int s = 0; s < S::kSpans; ++s)
+#pragma unroll
+      for (int j = 0; j < S::kVec; ++j) {
+        // The lane's 8 keys at dimension j of its span.
+        const uint32_t select = j & 1 ? 0x07060302u : 0x05040100u;
+        auto word = [&](int h, int e) {
+          const uint4& r = value_rows[h][e][s];
+          return (j >> 1) == 0 ? r.x : (j >> 1) == 1 ? r.y : (j >> 1) == 2 ? r.z : r.w;
+        };
+        auto pair = [&](int h, int e) {
+          return __builtin_amdgcn_perm(word(h, e + 1), word(h, e), select);
+        };
+        const uint4 v = make_uint4(pair(0, 0), pair(0, 2), pair(1, 0), pair(1, 2));
+#pragma unroll
+        for (int t = 0; t < S::kTiles; ++t) out[s][j] = T::mfma(v, w[t], out[s][j]);
+      }
+    now = next;
+  }
+
+  // The waves' states joined. Lane (n, g) holds dimensions 16 kVec s +
+  // kVec (4g + e) + j of its column.
+  l = across_groups(l, [](float p, float r) { return p + r; });
+  if (g == 0 && n < kW) {
+    joined_m[wave][n] = m;
+    joined_l[wave][n] = l;
+  }
+#pragma unroll
+  for (int s = 0; s < S::kSpans; ++s)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float v[S::kVec];
+#pragma unroll
+      for (int j = 0; j < S::kVec; ++j) v[j] = across_columns<kW>(out[s][j][e]);
+      if (n < kW) {
+        float* dst = &joined_out[wave][n * kPitch + 16 * S::kVec * s + S::kVec * (4 * g + e)];
+#pragma unroll
+        for (int j = 0; j < S::kVec; j += 4)
+          *reinterpret_cast<float4*>(dst + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+      }
+    }
+  __syncthreads();
+  const bool whole = part.parts == 1;
+  for (uint32_t i = threadIdx.x; i < heads * (kD / 4); i += kThreads) {
+    const uint32_t h = i / (kD / 4), d = i % (kD / 4) * 4;
+    float top = joined_m[0][h];
+#pragma unroll
+    for (uint32_t w = 1; w < kPartWaves; ++w) top = __builtin_fmaxf(top, joined_m[w][h]);
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float weights = 0.0f;
+#pragma unroll
+    for (uint32_t w = 0; w < kPartWaves; ++w) {
+      // A wave without a key holds zeros, and so does a row without one.
+      const float f = top == kMinusInf ? 0.0f : __builtin_amdgcn_exp2f(joined_m[w][h] - top);
+      const float4 o = *reinterpret_cast<const float4*>(&joined_out[w][h * kPitch + d]);
+      weights = fmaf_(joined_l[w][h], f, weights);
+      sum.x = fmaf_(o.x, f, sum.x);
+      sum.y = fmaf_(o.y, f, sum.y);
+      sum.z = fmaf_(o.z, f, sum.z);
+      sum.w = fmaf_(o.w, f, sum.w);
+    }
+    if (whole) {
+      const float f = weights == 0.0f ? 0.0f : 1.0f / weights;
+      sum.x *= f;
+      sum.y *= f;
+      sum.z *= f;
+      sum.w *= f;
+      *reinterpret_cast<float4*>(a.out + (uint64_t)part.row * a.out_stride +
+                                 (uint64_t)(head0 + h) * kD + d) = sum;
+    } else {
+      const uint64_t state = (uint64_t)(part.slot + part.index) * kHeadBlock + h;
+      *reinterpret_cast<float4*>(a.states + state * kD + d) = sum;
+      if (d == 0) *reinterpret_cast<float2*>(a.stats + 2 * state) = make_float2(top, weights);
+    }
+  }
+  if (!whole && part.index == 0 && threadIdx.x == 0) {
+    a.records[part.record] = make_uint4(part.row, head0 | heads << 16, part.parts, part.slot);
+  }
+}
+
+// The parts of the rows that have several, joined in order: a workgroup a
+// (record, head, 64 dimensions), 16 lanes of it the dimensions, four each,
+// and its 16 groups every sixteenth part.
+constexpr uint32_t kJoinGroups = kThreads / 16;
+template <int kD>
+__global__ __launch_bounds__(kThreads) void paged_attention_join_kernel(PagedAttentionArgs a) {
+  __shared__ float wave_top[kPartWaves], wave_sum[kPartWaves];
+  __shared__ float factors[kMostJoinedParts];
+  __shared__ float4 sums[kJoinGroups][16];
+  const uint32_t count = *a.record_count;
+  const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  for (uint32_t i = blockIdx.x; i < count; i += gridDim.x) {
+    const uint4 record = a.records[i];
+    const uint32_t h = blockIdx.y / (kD / 64), d = blockIdx.y % (kD / 64) * 64 + t % 16 * 4;
+    const uint32_t parts = record.z;
+    if (h >= record.y >> 16) continue;
+    const uint64_t first = (uint64_t)record.w * kHeadBlock + h;
+    float top = kMinusInf;
+    for (uint32_t p = t; p < parts; p += kThreads)
+      top = __builtin_fmaxf(top, a.stats[2 * (first + (uint64_t)p * kHeadBlock)]);
+    for (int o = 32; o > 0; o >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, o));
+    __syncthreads();  // the last record's reads are done
+    if (lane == 0) wave_top[wave] = top;
+    __syncthreads();
+    for (uint32_t w = 0; w < kPartWaves; ++w) top = __builtin_fmaxf(top, wave_top[w]);
+    float weights = 0.0f;
+    for (uint32_t p = t; p < parts; p += kThreads) {
+      const float2 s =
+          *reinterpret_cast<const float2*>(a.stats + 2 * (first + (uint64_t)p * kHeadBlock));
+      const float f = top == kMinusInf ? 0.0f : __builtin_amdgcn_exp2f(s.x - top);
+      factors[p] = f;
+      weights = fmaf_(s.y, f, weights);
+    }
+    for (int o = 32; o > 0; o >>= 1) weights += __shfl_xor(weights, o);
+    if (lane == 0) wave_sum[wave] = weights;
+    __syncthreads();
+    const uint32_t group = t / 16;
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (uint32_t p = group; p < parts; p += kJoinGroups) {
+      const float f = factors[p];
+      const float4 o = *reinterpret_cast<const float4*>(
+          a.states + (first + (uint64_t)p * kHeadBlock) * kD + d);
+      sum.x = fmaf_(o.x, f, sum.x);
+      sum.y = fmaf_(o.y, f, sum.y);
+      sum.z = fmaf_(o.z, f, sum.z);
+      sum.w = fmaf_(o.w, f, sum.w);
+    }
+    sums[group][t % 16] = sum;
+    __syncthreads();
+    if (t < 64) {
+      // A lane a dimension.
+      const float* column = reinterpret_cast<const float*>(&sums[0][0]) + t;
+      float x = 0.0f;
+      for (uint32_t k = 0; k < kJoinGroups; ++k) x += column[64 * k];
+      const float l = wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3];
+      a.out[(uint64_t)record.x * a.out_stride + (uint64_t)((record.y & 0xFFFF) + h) * kD +
+            blockIdx.y % (kD / 64) * 64 + t] = l == 0.0f ? 0.0f : x / l;
+    }
+  }
+}
+
+template <int kD, bool kBf16, int kW>
+void launch_parts(hipStream_t s, const PagedAttentionArgs& a, uint32_t grid) {
+  hipLaunchKernelGGL((paged_attention_kernel<kD, kBf16, kW>), dim3(grid), dim3(kThreads), 0, s, a);
+}
+
+template <int kD>
+hipError_t launch_shape(hipStream_t s, PagedAttentionArgs a, int compute_units) {
+  const uint32_t group = a.query_heads / a.cache.kv_heads;
+  const uint32_t heads = group < kHeadBlock ? group : kHeadBlock;
+  a.units = a.cache.kv_heads * ((group + kHeadBlock - 1) / kHeadBlock);
+  const uint32_t units = a.rows * a.units;
+  const uint32_t at_once = kWorkgroups<kD> * (uint32_t)compute_units;
+  a.target = part_target(units, at_once);
+  // No more parts than the rows' blocks fill, at a part's least blocks.
+  const uint64_t capacity = (uint64_t)a.cache.width * a.cache.page_slots;
+  const uint64_t most_keys = a.window < capacity ? a.window : capacity;
+  const uint64_t blocks = most_keys / kBlockKeys + 2;
+  const uint64_t fill = units * ((blocks + kPartWaves - 1) / kPartWaves);
+  const uint64_t bound = most_parts(units, at_once);
+  const uint32_t grid = (uint32_t)(fill < bound ? fill : bound);
+  if (a.cache.bf16) {
+    if (heads <= 4) launch_parts<kD, true, 4>(s, a, grid);
+    else if (heads <= 8) launch_parts<kD, true, 8>(s, a, grid);
+    else launch_parts<kD, true, 16>(s, a, grid);
+  } else {
+    if (heads <= 8) launch_parts<kD, false, 8>(s, a, grid);
+    else launch_parts<kD, false, 16>(s, a, grid);
+  }
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || blocks <= kPartWaves) return e;  // no row has two parts
+  const uint32_t joins = most_joined_parts(units, at_once) / 2;
+  const uint32_t records = units < joins ? units : joins;
+  hipLaunchKernelGGL(paged_attention_join_kernel<kD>,
+                     dim3(records < 256 ? records : 256, heads * (kD / 64)), dim3(kThreads), 0, s,
+                     a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_paged_attention(hipStream_t s, const PagedAttentionArgs& a, int compute_units) {
+  if (a.rows == 0 || a.rows > kMostRows || compute_units <= 0 || compute_units > kMostComputeUnits)
+    return hipErrorInvalidValue;
+  switch (a.cache.head_dim) {
+    case 64: return launch_shape<64>(s, a, compute_units);
+    case 128: return launch_shape<128>(s, a, compute_units);
+    case 256: return launch_shape<256>(s, a, compute_units);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+}  // namespace frz

@@ -211,6 +211,88 @@ int frz_op_draw(frz_device* dev, const uint32_t* candidates_dev,
                 const frz_sampling* sampling, uint32_t position,
                 uint32_t tokens, uint32_t* record_dev);
 
+/* ---- a step of many requests ---------------------------------------------
+ * What differs by request in one step of a batch: the keys and values each
+ * has cached, which lie in pages, and its adapter. (The reference runs one
+ * request, over one cache: no counterparts.) Rows are the step's tokens, at
+ * most 512, row r one token of the request sequences[r] (null: request r) at
+ * positions[r]; a row at FRZ_NO_POSITION is none, and its outputs are left as
+ * they are. These calls enqueue and return, in order on the device's stream;
+ * frz_sync waits. They may be made from several threads, and with any device
+ * current. Pointers to floats or 16-bit values must be multiples of 16 bytes
+ * and strides of 4 floats. */
+#define FRZ_FORMAT_F16 1
+#define FRZ_FORMAT_BF16 30
+#define FRZ_NO_POSITION 0xFFFFFFFFu
+#define FRZ_NO_PAGE 0xFFFFFFFFu
+#define FRZ_NO_ADAPTER 0xFFFFFFFFu
+/* Caches in pages. Page p's slot s holds head h's key at keys + p *
+ * page_stride + (s * kv_heads + h) * head_dim, its value likewise; a
+ * request's key at position j is in slot j % page_slots of the page that
+ * table[request * width + j / page_slots] names. Requests may share pages
+ * that they only read. An entry that names no page of the pool (FRZ_NO_PAGE,
+ * or any number from `pages` on), a position past the table's width and a
+ * request past its last row hold no key: nothing is read or written there. */
+typedef struct frz_pages {
+  void* keys;             /* dev */
+  void* values;           /* dev */
+  int format;             /* FRZ_FORMAT_F16 or FRZ_FORMAT_BF16 */
+  int kv_heads;           /* 1 to 1,024 */
+  int head_dim;           /* 64, 128 or 256 */
+  uint32_t page_slots;    /* a multiple of 16 */
+  uint32_t pages;         /* pages in the pool */
+  uint64_t page_stride;   /* values from a page to the next, a multiple of 8 */
+  const uint32_t* table;  /* dev: sequences rows of width entries */
+  uint32_t sequences;
+  uint32_t width;         /* width * page_slots at most 2^24 */
+} frz_pages;
+/* Each row's QK-norm and rope, its key and value appended to its request's
+ * pages: frz_op_rope's arithmetic, bit for bit, at positions of the rows'
+ * own. query_heads is a multiple of kv_heads, at most 1,024. Rows of query
+ * are q_stride, of key and value kv_stride floats apart; the roped queries go
+ * to roped (roped_stride apart), which may be query itself, with its stride.
+ * Keys and values round to the cache's format, to nearest even (F16
+ * saturates at 65,504). Of rows that name one slot the last one's stay. */
+int frz_op_rope_paged(frz_device* dev, const frz_pages* cache, const uint32_t* sequences,
+                      const uint32_t* positions, const float* turns, const float* query_gain,
+                      const float* key_gain, const float* query, const float* key,
+                      const float* value, int q_stride, int kv_stride, float* roped,
+                      int roped_stride, int query_heads, float epsilon, uint32_t rows);
+/* Each row's attention over the keys of its request at (position - window,
+ * position], its own among them (window at least 1; 0xFFFFFFFF: all): query
+ * head i reads key-value head i / (query_heads / kv_heads). Within about
+ * 1e-6 of the exact sums, not the reference's order. A row with no key gets
+ * zeros. Cached values must be finite where a row reads them, and may be
+ * anything elsewhere. out's rows are out_stride floats apart; out must not
+ * overlap query. */
+int frz_op_attention_paged(frz_device* dev, const frz_pages* cache, const uint32_t* sequences,
+                           const uint32_t* positions, const float* query, int q_stride,
+                           float* out, int out_stride, int query_heads, uint32_t window,
+                           float scale, uint32_t rows);
+/* Low-rank adapters of a projection, in one pool: adapter a's down matrix is
+ * rank rows of cols weights at down + a * rank * cols, its up matrix rows
+ * rows of rank at up + a * rows * rank. Its own rank may be lower: only the
+ * first ranks[a] rows and columns count, the others may hold anything. */
+typedef struct frz_adapters {
+  int format;             /* FRZ_FORMAT_F32, _F16 or _BF16 */
+  uint32_t count;         /* adapters in the pool */
+  int rank;               /* a multiple of 8, at most 128 */
+  int cols;               /* inputs, a multiple of 8 */
+  int rows;               /* outputs */
+  const void* down;       /* dev */
+  const void* up;         /* dev */
+  const uint32_t* ranks;  /* dev: count, or null: all rank */
+  const float* scales;    /* dev: count, or null: all 1 */
+} frz_adapters;
+/* y[t] = base[t] + scale up (down x[t]) with the adapter which[t] of each
+ * token (FRZ_NO_ADAPTER, or any number from `count` on: y[t] = base[t]), at
+ * most 512 tokens: beside a product that all tokens share, whose output is
+ * base. y may be base itself, with its stride; otherwise no two of x, base
+ * and y may overlap. Sums are in F32. */
+int frz_op_adapters(frz_device* dev, const frz_adapters* adapters, const uint32_t* which,
+                    const float* x, int x_stride, const float* base, int base_stride, float* y,
+                    int y_stride, uint32_t tokens);
+
 /* The shared numerics on the device, for their contract tests: which = 0
  * exp2, 1 cos, 2 sin, 3 inverse sqrt, 4 gelu_tanh, 5 exp_nonpositive,
  * 6 f16 pack (out holds the halves' bits as floats' low 16 bits, via
