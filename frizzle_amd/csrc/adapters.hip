@@ -1,18 +1,19 @@
 // Low-rank adapters of a batch's tokens beside a shared projection:
 // y = base + s U (D x), each token with an adapter of its own.
 //
-// Tokens next to each other that share an adapter, up to 16 within 16 aligned
-// ones, are a run: an adapter's weights are read once a run, from HBM once a
-// launch. Two launches: the low-rank rows D x of each run, K cut over
-// workgroups, then U times them, added to base. Work is counted in runs, which
-// each wave finds for itself from the tokens' adapters, so that a batch of
-// one adapter and one of an adapter a token both fill the chip.
+// Tokens next to each other that share an adapter, up to 16 (or 64) within as
+// many aligned ones, are a run: an adapter's weights are read once a run, from
+// HBM once a launch. Work is counted in runs, which each wave finds for itself from the
+// tokens' adapters, so that a batch of one adapter and one of an adapter a
+// token both fill the chip.
 //
 // Both products run on the F32 matrix cores (v_mfma_f32_16x16x4_f32), weights
 // of any format widened exactly on the way: products and sums are F32, and
 // rounded nowhere else. The weights are the instruction's A operand, 16 rows
 // by 4 columns: lane (m, g) holds 8 columns of row m as they lie in memory,
-// and instruction j of 8 takes the j-th of each.
+// and instruction j of 8 takes the j-th of each. Loads are a step ahead of the
+// products, and all of a step's loads are requested at once: a kernel is
+// compiled for 1, 2, 4 or 8 tiles of 16 ranks, so that no branch parts them.
 
 #include "batch_rules.h"
 #include "kernels.h"
@@ -25,49 +26,44 @@ using namespace rules;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / 64;
-constexpr int kRunTokens = 16;
-constexpr int kRankTiles = kMostAdapterRank / 16;
-constexpr int kBlockRows = 256;  // outputs a workgroup
+constexpr int kDownWaves = 8, kUpWaves = 4;  // of a workgroup
+constexpr int kTurnCols = 32 * kDownWaves;   // columns that its waves take a turn
+constexpr int kBlockRows = 32 * kUpWaves;    // outputs of a workgroup
+constexpr uint32_t kMostWorkgroups = 1024;   // that a launch has; about what runs at once
+constexpr int kRunTokens = 64;               // of a run of the up product
+constexpr int kTokenWaves = 8;
+constexpr uint32_t kTokenWorkgroups = 256;
+constexpr uint32_t kTokens = 64;
+constexpr uint64_t kTokenBytes = 192 << 10;
 
-struct Weights {
-  float v[8];
-};
-
-// Eight weights from element `at` (a multiple of 8).
+// Eight weights as they lie in memory, from element `at` (a multiple of 8).
 template <int kFormat>
-__device__ __forceinline__ Weights load8(const void* pool, uint64_t at) {
-  Weights w;
-  if constexpr (kFormat == 0) {
-    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(pool) + at);
-    const float4 a = p[0], b = p[1];
-    w = Weights{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
-  } else {
-    const uint4 r = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(pool) + at);
-    const uint32_t word[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (kFormat == 1) {
-        w.v[2 * i] = (float)__builtin_bit_cast(_Float16, (uint16_t)(word[i] & 0xFFFF));
-        w.v[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(word[i] >> 16));
-      } else {
-        w.v[2 * i] = bits_to_float(word[i] << 16);
-        w.v[2 * i + 1] = bits_to_float(word[i] & 0xFFFF0000u);
-      }
-    }
+struct Raw {
+  uint4 r[kFormat == 0 ? 2 : 1];
+  __device__ __forceinline__ void load(const void* pool, uint64_t at) {
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(pool) +
+                                                    at * (kFormat == 0 ? 4 : 2));
+    r[0] = p[0];
+    if constexpr (kFormat == 0) r[1] = p[1];
   }
-  return w;
-}
+  __device__ __forceinline__ float at(int i) const {
+    const uint4& q = r[kFormat == 0 ? i >> 2 : 0];
+    const int word = kFormat == 0 ? i & 3 : i >> 1;
+    const uint32_t w = word == 0 ? q.x : word == 1 ? q.y : word == 2 ? q.z : q.w;
+    if constexpr (kFormat == 0) return bits_to_float(w);
+    if constexpr (kFormat == 1)
+      return (float)__builtin_bit_cast(_Float16, (uint16_t)(i & 1 ? w >> 16 : w & 0xFFFF));
+    return bits_to_float(i & 1 ? w & 0xFFFF0000u : w << 16);
+  }
+};
 
 struct Run {
   uint32_t first, tokens;
   uint32_t adapter;  // kNone: none
-  int rank;          // its own
 };
 
 // The tokens' adapters as a wave holds them, eight tokens a lane, and the
-// runs that start among them.
+// runs of up to kRun tokens, in kRun aligned ones, that start among them.
 struct Runs {
   uint32_t id[8];
   uint32_t starts;  // bit i: a run starts at token 8 lane + i
@@ -75,26 +71,23 @@ struct Runs {
   uint32_t count;
 };
 
-__device__ __forceinline__ uint32_t adapter_of(const AdapterArgs& a, uint32_t token) {
-  const uint32_t id = a.which[token];
-  return id < a.count ? id : kNone;
-}
-
+template <int kRun>
 __device__ __forceinline__ Runs find_runs(const AdapterArgs& a, int lane) {
+  static_assert(kRun % 8 == 0, "a lane's tokens lie in one run's room");
   Runs r;
-  r.starts = 0;
-  uint32_t last = kNone;
-  if (lane > 0 && 8 * lane <= (int)a.tokens) last = adapter_of(a, 8 * lane - 1);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const uint32_t t = 8 * lane + i;
-    r.id[i] = t < a.tokens ? adapter_of(a, t) : kNone;
+    const uint32_t id = t < a.tokens ? a.which[t] : kNone;
+    r.id[i] = id < a.count ? id : kNone;
   }
+  const uint32_t last = __shfl_up(r.id[7], 1);
+  r.starts = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const uint32_t t = 8 * lane + i;
-    const uint32_t prev = i == 0 ? last : r.id[i > 0 ? i - 1 : 0];
-    if (t < a.tokens && (t % kRunTokens == 0 || r.id[i] != prev)) r.starts |= 1u << i;
+    if (t < a.tokens && (t % kRun == 0 || r.id[i] != (i == 0 ? last : r.id[i == 0 ? 0 : i - 1])))
+      r.starts |= 1u << i;
   }
   uint32_t sum = __popc(r.starts);
 #pragma unroll
@@ -102,193 +95,403 @@ __device__ __forceinline__ Runs find_runs(const AdapterArgs& a, int lane) {
     const uint32_t up = __shfl_up(sum, o);
     if (lane >= o) sum += up;
   }
-  r.count = __builtin_amdgcn_readfirstlane((int)__shfl(sum, 63));
+  r.count = (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
   r.before = sum - __popc(r.starts);
   return r;
 }
 
-// Run `want` (below r.count).
-__device__ __forceinline__ Run run_at(const AdapterArgs& a, const Runs& r, uint32_t want,
-                                      int lane) {
+// Run `want` (below r.count): it ends where the next one starts.
+__device__ __forceinline__ Run run_at(const AdapterArgs& a, const Runs& r, uint32_t want) {
   const uint32_t mine = __popc(r.starts);
-  const uint64_t owners = __ballot(want >= r.before && want < r.before + mine);
-  const int leader = __builtin_ctzll(owners);
+  const int leader = __builtin_ctzll(__ballot(want >= r.before && want < r.before + mine));
   uint32_t starts = r.starts;
   for (uint32_t i = r.before; i < want && starts; ++i) starts &= starts - 1;
   const int at = starts ? __builtin_ctz(starts) : 0;
   uint32_t id = kNone;
 #pragma unroll
   for (int i = 0; i < 8; ++i) id = i == at ? r.id[i] : id;
+  starts &= starts - 1;
+  auto lead = [](uint32_t x, int lane) {
+    return (uint32_t)__builtin_amdgcn_readlane((int)x, lane);
+  };
   Run run;
-  run.first = 8 * leader + (uint32_t)__builtin_amdgcn_readlane(at, leader);
-  run.adapter = (uint32_t)__builtin_amdgcn_readlane((int)id, leader);
-  // The tokens of its 16 that go on with the same adapter.
-  const uint32_t room = min(kRunTokens - run.first % kRunTokens, a.tokens - run.first);
-  const bool same = (uint32_t)lane < room && adapter_of(a, run.first + lane) == run.adapter;
-  run.tokens = (uint32_t)__builtin_ctzll(~__ballot(same));
-  run.rank = a.rank;
-  if (run.adapter != kNone && a.ranks) {
-    const uint32_t own = a.ranks[run.adapter];
-    run.rank = own < (uint32_t)a.rank ? (int)own : a.rank;
+  run.first = 8 * leader + lead(at, leader);
+  run.adapter = lead(id, leader);
+  uint32_t rest = lead(starts, leader), lane = leader;
+  if (rest == 0) {
+    const uint64_t after = leader == 63 ? 0 : __ballot(r.starts != 0) >> (leader + 1);
+    if (after) {
+      lane = leader + 1 + __builtin_ctzll(after);
+      rest = lead(r.starts, lane);
+    }
   }
-  run.rank = __builtin_amdgcn_readfirstlane(run.rank);
+  run.tokens = (rest ? 8 * lane + __builtin_ctz(rest) : a.tokens) - run.first;
   return run;
 }
 
-// The low-rank rows of each run over one of K's splits: a workgroup an item
-// (run, split), its waves every fourth 32 columns of the split.
+// An adapter's own rank. What a pool holds past it is loaded (it lies in the
+// pool) but goes into no sum that is kept.
+__device__ __forceinline__ int own_rank(const AdapterArgs& a, const Run& run) {
+  const uint32_t own = a.ranks ? a.ranks[run.adapter] : (uint32_t)a.rank;
+  return (int)min(own, (uint32_t)a.rank);
+}
+
+// Four values of a row of `rows`, from element `at`; one past the row's end
+// repeats the last.
+__device__ __forceinline__ f32x4 load4(const float* row, int at, int rows) {
+  if (at + 4 <= rows) return *reinterpret_cast<const f32x4*>(row + at);
+  f32x4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = row[min(at + e, rows - 1)];
+  return v;
+}
+__device__ __forceinline__ void store4(float* row, int at, int rows, f32x4 v) {
+  if (at + 4 <= rows) {
+    *reinterpret_cast<f32x4*>(row + at) = v;
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (at + e < rows) row[at + e] = v[e];
+}
+
+// Outputs [from, to) of tokens without an adapter: base, where y is not base.
+__device__ __forceinline__ void copy_base(const AdapterArgs& a, uint32_t first, uint32_t tokens,
+                                          int from, int to, int wave, int waves, int lane) {
+  if (a.base == a.y) return;
+  const int pieces = (to - from + 255) / 256;  // of a token, a wave each
+  for (uint32_t i = wave; i < tokens * pieces; i += waves) {
+    const uint32_t t = first + i / pieces;
+    const int o = from + (int)(i % pieces) * 256 + 4 * lane;
+    if (o < to)
+      store4(a.y + (uint64_t)t * a.y_stride, o, to,
+             load4(a.base + (uint64_t)t * a.base_stride, o, to));
+  }
+}
+
+// A wave's share of D x for a run of up to 16 tokens, over the columns
+// [from, to) and 16 ranks from `rank0` on: every kWaves-th 32 of the columns.
+// Lane (n, g) gets token n's ranks rank0 + 4 g .. + 3.
+template <int kFormat, int kWaves>
+__device__ __forceinline__ f32x4 low_rank(const AdapterArgs& a, const Run& run, int rank0, int from,
+                                          int to, int wave, int n, int g) {
+  constexpr int kDepth = 5;  // steps whose loads are in flight at once
+  constexpr int kTurn = 32 * kWaves;
+  Raw<0> x[kDepth];
+  Raw<kFormat> w[kDepth];
+  const float* row =
+      a.x + (uint64_t)(run.first + ((uint32_t)n < run.tokens ? n : 0)) * a.x_stride;
+  const uint64_t pool =
+      ((uint64_t)run.adapter * a.rank + min(rank0 + n, a.rank - 1)) * (uint64_t)a.cols;
+  f32x4 acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int k0 = from + 32 * wave; k0 < to; k0 += kDepth * kTurn) {
+#pragma unroll
+    for (int i = 0; i < kDepth; ++i) {
+      if (k0 + i * kTurn >= to) continue;
+      // Columns are multiples of 8, and so are splits.
+      const int at = k0 + i * kTurn + 8 * g, k = at < to ? at : from;
+      x[i].load(row, k);
+      w[i].load(a.down, pool + k);
+    }
+#pragma unroll
+    for (int i = 0; i < kDepth; ++i) {
+      if (k0 + i * kTurn >= to) continue;
+      const bool in = k0 + i * kTurn + 8 * g < to;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(in ? w[i].at(j) : 0.0f,
+                                                   in ? x[i].at(j) : 0.0f, acc, 0, 0, 0);
+    }
+  }
+  return acc;
+}
+
+// The low-rank rows of each run: a workgroup an item (run, 16 ranks, split of
+// K). Workgroups go round the eight dies: numbered by eights of runs, a run's
+// meet on one die, whose L2 then holds its rows of x alone.
 template <int kFormat>
-__global__ __launch_bounds__(kThreads) void adapter_down_kernel(AdapterArgs a) {
-  __shared__ f32x4 sums[kWaves][kRankTiles][64];
+__global__ __launch_bounds__(64 * kDownWaves, 4) void adapter_down_kernel(AdapterArgs a) {
+  __shared__ f32x4 sums[kDownWaves][64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int n = lane & 15, g = lane >> 4;
-  const Runs runs = find_runs(a, lane);
-  const uint32_t items = runs.count * a.splits;
+  const Runs runs = find_runs<16>(a, lane);
+  const uint32_t places = runs.count < 8 ? runs.count : (runs.count + 7) / 8 * 8;
+  const uint32_t groups = (a.rank + 15) / 16;
+  const uint32_t items = places * groups * a.splits;
   for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const Run run = run_at(a, runs, item / a.splits, lane);
-    if (run.adapter == kNone || run.rank == 0) continue;
-    const uint32_t split = item % a.splits;
+    if (item % places >= runs.count) continue;
+    const Run run = run_at(a, runs, item % places);
+    if (run.adapter == kNone) continue;
+    const uint32_t piece = item / places, split = piece / groups;
+    const int rank0 = piece % groups * 16;
     const int from = split * a.split_cols, to = min(from + a.split_cols, a.cols);
-    const int tiles = (run.rank + 15) / 16;
-    f32x4 acc[kRankTiles];
-#pragma unroll
-    for (int t = 0; t < kRankTiles; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const bool live = (uint32_t)n < run.tokens;
-    const float* x = a.x + (uint64_t)(run.first + (live ? n : 0)) * a.x_stride;
-    const uint64_t pool = (uint64_t)run.adapter * a.rank * a.cols;
-    for (int k0 = from + 32 * wave; k0 < to; k0 += 32 * kWaves) {
-      const int k = k0 + 8 * g;
-      const bool in = k < to;  // columns are multiples of 8, and so are splits
-      const int kc = in ? k : from;
-      const Weights xs = load8<0>(x, kc);
-#pragma unroll
-      for (int t = 0; t < kRankTiles; ++t) {
-        if (t >= tiles) break;
-        const int r = 16 * t + n;
-        const bool held = in && r < run.rank;
-        const Weights w = load8<kFormat>(a.down, pool + (uint64_t)min(r, run.rank - 1) * a.cols + kc);
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(held ? w.v[j] : 0.0f,
-                                                        in && live ? xs.v[j] : 0.0f, acc[t], 0, 0, 0);
-      }
-    }
+    const f32x4 acc = low_rank<kFormat, kDownWaves>(a, run, rank0, from, to, wave, n, g);
     __syncthreads();  // the last item's sums are read
-#pragma unroll
-    for (int t = 0; t < kRankTiles; ++t)
-      if (t < tiles) sums[wave][t][lane] = acc[t];
+    sums[wave][lane] = acc;
     __syncthreads();
-    // Lane (n, g) of tile t: token n, ranks 16 t + 4 g .. + 3.
-    for (int i = threadIdx.x; i < tiles * 64; i += kThreads) {
-      const int t = i >> 6, ln = i & 63, token = ln & 15, r = 16 * t + 4 * (ln >> 4);
-      if ((uint32_t)token >= run.tokens || r >= run.rank) continue;
-      f32x4 sum = sums[0][t][ln];
+    const int r = rank0 + 4 * g;
+    if (wave == 0 && (uint32_t)n < run.tokens && r < a.rank) {
+      f32x4 sum = sums[0][lane];
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) sum += sums[w][t][ln];
-      *reinterpret_cast<f32x4*>(a.low + ((uint64_t)split * a.tokens + run.first + token) * a.rank + r) =
+      for (int w = 1; w < kDownWaves; ++w) sum += sums[w][lane];
+      *reinterpret_cast<f32x4*>(a.low + ((uint64_t)split * a.tokens + run.first + n) * a.rank + r) =
           sum;
     }
   }
 }
 
-// base + s U times the low-rank rows: a workgroup an item (run, 256 outputs),
-// a wave 64 of them.
-template <int kFormat>
-__global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterArgs a) {
-  constexpr int kPitch = kMostAdapterRank + 4;
+// base + s U times the low-rank rows, as the splits left them: a workgroup an
+// item (run of up to 64 tokens, 128 outputs), a wave two tiles of 16 outputs
+// by the run's four of 16 tokens. U is read once a run.
+template <int kFormat, int kTiles>
+__global__ __launch_bounds__(64 * kUpWaves, 3) void adapter_up_kernel(AdapterArgs a) {
+  constexpr int kChunks = (kTiles + 1) / 2;
+  constexpr int kPitch = 32 * kChunks + 4;  // floats a token's row takes in LDS
+  constexpr int kRunTiles = kRunTokens / 16;
   __shared__ __attribute__((aligned(16))) float low[kRunTokens][kPitch];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int n = lane & 15, g = lane >> 4;
-  const Runs runs = find_runs(a, lane);
+  const Runs runs = find_runs<kRunTokens>(a, lane);
+  // As above, by eights of blocks: a block's runs meet on one die.
   const uint32_t blocks = (a.rows + kBlockRows - 1) / kBlockRows;
-  const uint32_t items = runs.count * blocks;
+  const uint32_t places = blocks < 8 ? blocks : (blocks + 7) / 8 * 8;
+  const uint32_t items = runs.count * places;
   for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const Run run = run_at(a, runs, item / blocks, lane);
-    const int out0 = item % blocks * kBlockRows + 64 * wave;
-    const bool none = run.adapter == kNone || run.rank == 0;
-    if (none && a.base == a.y) continue;
-    const int chunks = none ? 0 : (run.rank + 31) / 32;
+    if (item % places >= blocks) continue;
+    const Run run = run_at(a, runs, item / places);
+    const int from = item % places * kBlockRows;
+    if (run.adapter == kNone) {
+      copy_base(a, run.first, run.tokens, from, min(from + kBlockRows, a.rows), wave, kUpWaves,
+                lane);
+      continue;
+    }
+    const int o = from + 32 * wave;  // the wave's outputs: o .. o + 31
+    Raw<kFormat> w[2][2];            // of a chunk of 32 ranks and of the next, by turns
+    auto load = [&](int c, Raw<kFormat> (&to)[2]) {
+      const int r = 32 * c + 8 * g;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        to[i].load(a.up, ((uint64_t)run.adapter * a.rows + min(o + 16 * i + n, a.rows - 1)) *
+                                 (uint64_t)a.rank + (r < a.rank ? r : 0));
+    };
+    load(0, w[0]);
+    const int rank = __builtin_amdgcn_readfirstlane(own_rank(a, run));
+    const float scale = a.scales ? a.scales[run.adapter] : 1.0f;
+    const int run_tiles = (int)((run.tokens + 15) / 16);
     __syncthreads();  // the last item's rows are read
-    if (!none) {
-      const float scale = a.scales ? a.scales[run.adapter] : 1.0f;
-      const int width = 32 * chunks;
-      for (int i = threadIdx.x; i < kRunTokens * width; i += kThreads) {
-        const int t = i / width, r = i % width;
-        float sum = 0.0f;
-        if ((uint32_t)t < run.tokens && r < run.rank) {
-          const float* src = a.low + (uint64_t)(run.first + t) * a.rank + r;
-          for (int s = 0; s < a.splits; ++s) sum += src[(uint64_t)s * a.tokens * a.rank];
-        }
-        low[t][r] = sum * scale;
+    // Four ranks a thread and turn; those past the adapter's own, and tokens
+    // past the run, are zero.
+    for (int i = threadIdx.x; i < run_tiles * 16 * 8 * kChunks; i += 64 * kUpWaves) {
+      const int t = i / (8 * kChunks), r = i % (8 * kChunks) * 4;
+      f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if ((uint32_t)t < run.tokens && r < a.rank) {
+        const float* src = a.low + (uint64_t)(run.first + t) * a.rank + r;
+#pragma unroll 4
+        for (int s = 0; s < a.splits; ++s)
+          sum += *reinterpret_cast<const f32x4*>(src + (uint64_t)s * a.tokens * a.rank);
       }
+      f32x4 row;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) row[e] = r + e < rank ? sum[e] * scale : 0.0f;
+      *reinterpret_cast<f32x4*>(&low[t][r]) = row;
     }
     __syncthreads();
-    const uint64_t pool = (uint64_t)run.adapter * a.rows * a.rank;
-#pragma unroll 1
-    for (int tile = 0; tile < 4; ++tile) {
-      const int o = out0 + 16 * tile;
-      if (o >= a.rows) break;
-      f32x4 acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      const uint64_t at = pool + (uint64_t)min(o + n, a.rows - 1) * a.rank;
-      for (int c = 0; c < chunks; ++c) {
-        const int r = 32 * c + 8 * g;
-        const Weights w = load8<kFormat>(a.up, at + (r < a.rank ? r : 0));
-        const Weights h = load8<0>(&low[n][0], r);
+    f32x4 acc[2][kRunTiles];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int t = 0; t < kRunTiles; ++t) acc[i][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      if (c + 1 < kChunks) load(c + 1, w[(c + 1) & 1]);
+#pragma unroll
+      for (int t = 0; t < kRunTiles; ++t) {
+        if (t >= run_tiles) break;
+        const f32x4 h0 = *reinterpret_cast<const f32x4*>(&low[16 * t + n][32 * c + 8 * g]);
+        const f32x4 h1 = *reinterpret_cast<const f32x4*>(&low[16 * t + n][32 * c + 8 * g + 4]);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          acc = __builtin_amdgcn_mfma_f32_16x16x4f32(r + j < run.rank ? w.v[j] : 0.0f, h.v[j], acc,
-                                                     0, 0, 0);
-      }
-      // Lane (n, g): token n, outputs o + 4 g .. + 3.
-      const int first = o + 4 * g;
-      if ((uint32_t)n >= run.tokens || first >= a.rows) continue;
-      const float* base = a.base + (uint64_t)(run.first + n) * a.base_stride + first;
-      float* y = a.y + (uint64_t)(run.first + n) * a.y_stride + first;
-      if (first + 4 <= a.rows) {
-        *reinterpret_cast<f32x4*>(y) = *reinterpret_cast<const f32x4*>(base) + acc;
-      } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (first + e < a.rows) y[e] = base[e] + acc[e];
+          for (int i = 0; i < 2; ++i)
+            acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                32 * c + 8 * g + j < rank ? w[c & 1][i].at(j) : 0.0f, j < 4 ? h0[j & 3] : h1[j & 3],
+                acc[i][t], 0, 0, 0);
       }
+    }
+    // Lane (n, g): outputs 4 g .. + 3 of each tile, of token n of each 16.
+    f32x4 base[2][kRunTiles];
+#pragma unroll
+    for (int t = 0; t < kRunTiles; ++t) {
+      if (t >= run_tiles) break;
+      const float* src =
+          a.base + (uint64_t)(run.first + min(16u * t + n, run.tokens - 1)) * a.base_stride;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) base[i][t] = load4(src, o + 16 * i + 4 * g, a.rows);
+    }
+#pragma unroll
+    for (int t = 0; t < kRunTiles; ++t) {
+      if (16u * t + n >= run.tokens) break;
+      float* dst = a.y + (uint64_t)(run.first + 16 * t + n) * a.y_stride;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        store4(dst, o + 16 * i + 4 * g, a.rows, base[i][t] + acc[i][t]);
     }
   }
 }
 
+// Both products of one token: a workgroup a (token, block of outputs), on the
+// vector units. All that it reads is asked for at once: a wave's rows of D,
+// a lane 8 columns of each 512, and a thread's outputs' rows of U. Each of a
+// token's workgroups forms all of D x for itself, from L2; numbered by eights
+// of tokens, they are on one die.
 template <int kFormat>
-hipError_t launch_format(hipStream_t s, const AdapterArgs& a, uint32_t down, uint32_t up) {
-  hipLaunchKernelGGL(adapter_down_kernel<kFormat>, dim3(down), dim3(kThreads), 0, s, a);
+__global__ __launch_bounds__(64 * kTokenWaves, 2) void adapter_token_kernel(AdapterArgs a) {
+  constexpr int kThreads = 64 * kTokenWaves;
+  __shared__ float low[kMostAdapterRank];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint32_t places = a.tokens < 8 ? a.tokens : (a.tokens + 7) / 8 * 8;
+  const uint32_t token = blockIdx.x % places;
+  if (token >= a.tokens) return;
+  const int from = blockIdx.x / places * a.block_rows, to = min(from + a.block_rows, a.rows);
+  if (from >= a.rows) return;
+  uint32_t adapter = a.which[token];
+  if (adapter >= a.count) {
+    copy_base(a, token, 1, from, to, wave, kTokenWaves, lane);
+    return;
+  }
+  Run run{token, 1, adapter};
+  // The first 32 ranks of a thread's first outputs, which wait for nothing.
+  constexpr int kAhead = kFormat == 0 ? 1 : 2;
+  Raw<kFormat> u[kAhead][4];
+  auto load_up = [&](int o, int c, Raw<kFormat> (&to4)[4]) {
+    const uint64_t at =
+        ((uint64_t)adapter * a.rows + min(o, a.rows - 1)) * (uint64_t)a.rank + 32 * c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (32 * c + 8 * i < a.rank) to4[i].load(a.up, at + 8 * i);
+  };
+  const float* x = a.x + (uint64_t)token * a.x_stride;
+  const uint64_t pool = (uint64_t)adapter * a.rank * (uint64_t)a.cols;
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) load_up(from + (int)threadIdx.x + i * kThreads, 0, u[i]);
+  const int rank = __builtin_amdgcn_readfirstlane(own_rank(a, run));
+  const float scale = a.scales ? a.scales[adapter] : 1.0f;
+  // Four ranks a wave and turn, 1,024 columns at a time.
+  for (int r0 = 4 * wave; r0 < a.rank; r0 += 4 * kTokenWaves) {
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k0 = 0; k0 < a.cols; k0 += 1536) {
+      Raw<0> xs[3];
+      Raw<kFormat> d[3][4];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        const int at = k0 + 512 * i + 8 * lane, k = at < a.cols ? at : 0;
+        if (k0 + 512 * i >= a.cols) continue;
+        xs[i].load(x, k);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)  // ranks come in eights
+          d[i][r].load(a.down, pool + (uint64_t)(r0 + r) * a.cols + k);
+      }
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        if (k0 + 512 * i + 8 * lane >= a.cols) continue;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) sum[r] = fmaf_(d[i][r].at(j), xs[i].at(j), sum[r]);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      sum[r] = wave_tree(sum[r]);
+      if (lane == 0) low[r0 + r] = r0 + r < rank ? sum[r] * scale : 0.0f;
+    }
+  }
+  __syncthreads();
+  const float* base = a.base + (uint64_t)token * a.base_stride;
+  float* y = a.y + (uint64_t)token * a.y_stride;
+  for (int o = from + (int)threadIdx.x, turn = 0; o < to; o += kThreads, ++turn) {
+    float sum = 0.0f;
+    const float add = base[o];
+    for (int c = 0; 32 * c < rank; ++c) {
+      Raw<kFormat> v[4];
+      if (c == 0 && turn < kAhead) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = kAhead == 2 && turn ? u[kAhead - 1][i] : u[0][i];
+      } else {
+        load_up(o, c, v);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int r = 32 * c + 8 * i + j;
+          if (r < rank) sum = fmaf_(v[i].at(j), low[r], sum);
+        }
+    }
+    y[o] = add + sum;
+  }
+}
+
+template <int kFormat, int kTiles>
+hipError_t launch_up(hipStream_t s, const AdapterArgs& a) {
+  // As many workgroups as items where every token is a run; past a bound each
+  // takes every so many.
+  const uint32_t blocks = (a.rows + kBlockRows - 1) / kBlockRows;
+  const uint64_t items = (uint64_t)a.tokens * (blocks < 8 ? blocks : (blocks + 7) / 8 * 8);
+  hipLaunchKernelGGL((adapter_up_kernel<kFormat, kTiles>),
+                     dim3((uint32_t)(items < kMostWorkgroups ? items : kMostWorkgroups)),
+                     dim3(64 * kUpWaves), 0, s, a);
+  return hipGetLastError();
+}
+
+template <int kFormat>
+hipError_t launch_format(hipStream_t s, AdapterArgs a) {
+  const uint64_t weights = (uint64_t)a.rank * a.cols * (kFormat == 0 ? 4 : 2);
+  if (a.tokens <= kTokens && weights <= kTokenBytes) {
+    // Blocks of whole turns of a workgroup's threads, so many that the tokens'
+    // workgroups fill the chip.
+    const uint32_t turn = 64 * kTokenWaves;
+    const uint32_t turns = (a.rows + turn - 1) / turn;
+    const uint32_t wanted = (kTokenWorkgroups + a.tokens - 1) / a.tokens;
+    const uint32_t each = wanted < turns ? (turns + wanted - 1) / wanted : 1;
+    a.block_rows = (int)(each * turn);
+    const uint32_t places = a.tokens < 8 ? a.tokens : (a.tokens + 7) / 8 * 8;
+    hipLaunchKernelGGL(adapter_token_kernel<kFormat>, dim3(places * ((turns + each - 1) / each)),
+                       dim3(turn), 0, s, a);
+    return hipGetLastError();
+  }
+  // Splits of whole turns of a workgroup's waves, so many that the runs'
+  // workgroups fill the chip.
+  const uint32_t items = (a.tokens + 15) / 16 * ((a.rank + 15) / 16);
+  uint32_t splits = 512 / items;
+  splits = splits < 1 ? 1 : splits > kMostAdapterSplits ? kMostAdapterSplits : splits;
+  const int turns = (a.cols + kTurnCols - 1) / kTurnCols;
+  a.split_cols = kTurnCols * ((turns + (int)splits - 1) / (int)splits);
+  a.splits = (a.cols + a.split_cols - 1) / a.split_cols;
+  const uint64_t down = (uint64_t)((a.tokens + 7) / 8 * 8) * ((a.rank + 15) / 16) * a.splits;
+  hipLaunchKernelGGL(adapter_down_kernel<kFormat>,
+                     dim3((uint32_t)(down < kMostWorkgroups ? down : kMostWorkgroups)),
+                     dim3(64 * kDownWaves), 0, s, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(adapter_up_kernel<kFormat>, dim3(up), dim3(kThreads), 0, s, a);
-  return hipGetLastError();
+  if (a.rank <= 32) return launch_up<kFormat, 2>(s, a);
+  if (a.rank <= 64) return launch_up<kFormat, 4>(s, a);
+  return launch_up<kFormat, 8>(s, a);
 }
 
 }  // namespace
 
-hipError_t launch_adapters(hipStream_t s, const AdapterArgs& args) {
-  AdapterArgs a = args;
+hipError_t launch_adapters(hipStream_t s, const AdapterArgs& a) {
   if (a.tokens == 0 || a.tokens > kMostRows || a.rank <= 0 || a.rank > kMostAdapterRank ||
       a.rank % 8 || a.cols <= 0 || a.cols % 8 || a.rows <= 0)
     return hipErrorInvalidValue;
-  // Splits of 256 columns, two turns of a workgroup's waves; longer ones past
-  // kMostAdapterSplits.
-  const int turn = 32 * kWaves;
-  const int turns = (a.cols + turn - 1) / turn;
-  a.split_cols = turn * (turns <= 2 * kMostAdapterSplits
-                             ? 2 : (turns + kMostAdapterSplits - 1) / kMostAdapterSplits);
-  a.splits = (a.cols + a.split_cols - 1) / a.split_cols;
-  const uint32_t blocks = (a.rows + kBlockRows - 1) / kBlockRows;
-  const uint64_t most = 2048;  // workgroups; each takes every so many items
-  const uint64_t down = (uint64_t)a.tokens * a.splits, up = (uint64_t)a.tokens * blocks;
-  const uint32_t grid_down = (uint32_t)(down < most ? down : most);
-  const uint32_t grid_up = (uint32_t)(up < most ? up : most);
   switch (a.format) {
-    case 0: return launch_format<0>(s, a, grid_down, grid_up);
-    case 1: return launch_format<1>(s, a, grid_down, grid_up);
-    case 30: return launch_format<30>(s, a, grid_down, grid_up);
+    case 0: return launch_format<0>(s, a);
+    case 1: return launch_format<1>(s, a);
+    case 30: return launch_format<30>(s, a);
     default: return hipErrorInvalidValue;
   }
 }

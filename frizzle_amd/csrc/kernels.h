@@ -509,7 +509,7 @@ struct AdapterArgs {
   int y_stride;
   uint32_t tokens;
   float* low;        // [splits][tokens][rank]
-  int splits = 0, split_cols = 0;  // set by the launcher
+  int splits = 0, split_cols = 0, block_rows = 0;  // set by the launcher
 };
 constexpr int kMostAdapterRank = 128;
 constexpr int kMostAdapterSplits = 32;
