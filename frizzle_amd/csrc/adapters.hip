@@ -29,7 +29,10 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int kDownWaves = 8, kUpWaves = 4;  // of a workgroup
 constexpr int kTurnCols = 32 * kDownWaves;   // columns that its waves take a turn
 constexpr int kBlockRows = 32 * kUpWaves;    // outputs of a workgroup
-constexpr uint32_t kMostWorkgroups = 1024;   // that a launch has; about what runs at once
+// Workgroups that run at once; a launch has no more, and each takes every so
+// many items: ones without an item would wait for a place, then for the tokens'
+// adapters, after all others.
+constexpr uint32_t kMostDown = 512, kMostUp = 768;
 constexpr int kRunTokens = 64;               // of a run of the up product
 constexpr int kTokenWaves = 8;
 constexpr uint32_t kTokenWorkgroups = 256;
@@ -62,70 +65,67 @@ struct Run {
   uint32_t adapter;  // kNone: none
 };
 
-// The tokens' adapters as a wave holds them, eight tokens a lane, and the
+// The tokens' adapters as a wave holds them, token 64 i + lane a lane, and the
 // runs of up to kRun tokens, in kRun aligned ones, that start among them.
+constexpr int kTokenGroups = kMostRows / 64;
 struct Runs {
-  uint32_t id[8];
-  uint32_t starts;  // bit i: a run starts at token 8 lane + i
-  uint32_t before;  // runs before the lane's
+  uint32_t id[kTokenGroups];
+  uint64_t starts[kTokenGroups];  // a bit a token
   uint32_t count;
 };
 
 template <int kRun>
 __device__ __forceinline__ Runs find_runs(const AdapterArgs& a, int lane) {
-  static_assert(kRun % 8 == 0, "a lane's tokens lie in one run's room");
+  static_assert(64 % kRun == 0, "a run lies in one group");
   Runs r;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t t = 8 * lane + i;
-    const uint32_t id = t < a.tokens ? a.which[t] : kNone;
-    r.id[i] = id < a.count ? id : kNone;
+  for (int i = 0; i < kTokenGroups; ++i) {
+    r.id[i] = a.which[min(64u * i + lane, a.tokens - 1)];
   }
-  const uint32_t last = __shfl_up(r.id[7], 1);
-  r.starts = 0;
+  r.count = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t t = 8 * lane + i;
-    if (t < a.tokens && (t % kRun == 0 || r.id[i] != (i == 0 ? last : r.id[i == 0 ? 0 : i - 1])))
-      r.starts |= 1u << i;
+  for (int i = 0; i < kTokenGroups; ++i) {
+    if (r.id[i] >= a.count) r.id[i] = kNone;
+    // The token before, of lane - 1 (DPP wave_shr:1); a group's first starts a
+    // run whatever it is.
+    const uint32_t last = (uint32_t)__builtin_amdgcn_update_dpp((int)r.id[i], (int)r.id[i], 0x138,
+                                                                0xF, 0xF, false);
+    r.starts[i] =
+        __ballot(64u * i + lane < a.tokens && (lane % kRun == 0 || r.id[i] != last));
+    r.count += __popcll(r.starts[i]);
   }
-  uint32_t sum = __popc(r.starts);
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t up = __shfl_up(sum, o);
-    if (lane >= o) sum += up;
-  }
-  r.count = (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
-  r.before = sum - __popc(r.starts);
   return r;
 }
 
 // Run `want` (below r.count): it ends where the next one starts.
 __device__ __forceinline__ Run run_at(const AdapterArgs& a, const Runs& r, uint32_t want) {
-  const uint32_t mine = __popc(r.starts);
-  const int leader = __builtin_ctzll(__ballot(want >= r.before && want < r.before + mine));
-  uint32_t starts = r.starts;
-  for (uint32_t i = r.before; i < want && starts; ++i) starts &= starts - 1;
-  const int at = starts ? __builtin_ctz(starts) : 0;
-  uint32_t id = kNone;
+  uint32_t group = 0;
+  uint64_t starts = r.starts[0];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) id = i == at ? r.id[i] : id;
-  starts &= starts - 1;
-  auto lead = [](uint32_t x, int lane) {
-    return (uint32_t)__builtin_amdgcn_readlane((int)x, lane);
-  };
-  Run run;
-  run.first = 8 * leader + lead(at, leader);
-  run.adapter = lead(id, leader);
-  uint32_t rest = lead(starts, leader), lane = leader;
-  if (rest == 0) {
-    const uint64_t after = leader == 63 ? 0 : __ballot(r.starts != 0) >> (leader + 1);
-    if (after) {
-      lane = leader + 1 + __builtin_ctzll(after);
-      rest = lead(r.starts, lane);
+  for (int i = 1; i < kTokenGroups; ++i) {
+    const uint32_t before = __popcll(starts);
+    if (group == (uint32_t)i - 1 && want >= before) {
+      want -= before;
+      group = i;
+      starts = r.starts[i];
     }
   }
-  run.tokens = (rest ? 8 * lane + __builtin_ctz(rest) : a.tokens) - run.first;
+  // The lane whose start has `want` others before it.
+  const uint32_t before =
+      __builtin_amdgcn_mbcnt_hi((uint32_t)(starts >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)starts, 0));
+  const uint64_t at = __ballot(before == want) & starts;
+  const int lane = __builtin_ctzll(at);
+  Run run;
+  run.first = 64 * group + lane;
+  run.adapter = kNone;
+#pragma unroll
+  for (int i = 0; i < kTokenGroups; ++i) {
+    // Every group's, then the one: an index that varies would put them in memory.
+    const uint32_t id = (uint32_t)__builtin_amdgcn_readlane((int)r.id[i], lane);
+    run.adapter = group == (uint32_t)i ? id : run.adapter;
+  }
+  const uint64_t rest = lane == 63 ? 0 : starts >> (lane + 1);
+  run.tokens = rest ? 1 + __builtin_ctzll(rest) : min(64 * (group + 1), a.tokens) - run.first;
   return run;
 }
 
@@ -281,23 +281,43 @@ __global__ __launch_bounds__(64 * kUpWaves, 3) void adapter_up_kernel(AdapterArg
     const float scale = a.scales ? a.scales[run.adapter] : 1.0f;
     const int run_tiles = (int)((run.tokens + 15) / 16);
     __syncthreads();  // the last item's rows are read
-    // Four ranks a thread and turn; those past the adapter's own, and tokens
-    // past the run, are zero.
-    for (int i = threadIdx.x; i < run_tiles * 16 * 8 * kChunks; i += 64 * kUpWaves) {
-      const int t = i / (8 * kChunks), r = i % (8 * kChunks) * 4;
-      f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      if ((uint32_t)t < run.tokens && r < a.rank) {
-        const float* src = a.low + (uint64_t)(run.first + t) * a.rank + r;
-#pragma unroll 4
-        for (int s = 0; s < a.splits; ++s)
-          sum += *reinterpret_cast<const f32x4*>(src + (uint64_t)s * a.tokens * a.rank);
-      }
+    // Four ranks a thread and piece, the splits of all its pieces asked for
+    // together; ranks past the adapter's own, and tokens past the run, are zero.
+    constexpr int kPieces = kRunTokens * 8 * kChunks / (64 * kUpWaves);
+    f32x4 piece[kPieces];
+    const float* src[kPieces];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      // A piece past the run or the pool's rank reads another's place.
+      const uint32_t at = threadIdx.x + i * 64 * kUpWaves;
+      const uint32_t t = min(at / (8 * kChunks), run.tokens - 1);
+      const int r = min((int)(at % (8 * kChunks) * 4), a.rank - 4);
+      src[i] = a.low + (uint64_t)(run.first + t) * a.rank + r;
+      piece[i] = *reinterpret_cast<const f32x4*>(src[i]);
+    }
+    for (int s = 1; s < a.splits; ++s)
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i)
+        piece[i] += *reinterpret_cast<const f32x4*>(src[i] + (uint64_t)s * a.tokens * a.rank);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int at = threadIdx.x + i * 64 * kUpWaves;
+      const int t = at / (8 * kChunks), r = at % (8 * kChunks) * 4;
       f32x4 row;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) row[e] = r + e < rank ? sum[e] * scale : 0.0f;
+      for (int e = 0; e < 4; ++e) row[e] = r + e < rank ? piece[i][e] * scale : 0.0f;
       *reinterpret_cast<f32x4*>(&low[t][r]) = row;
     }
     __syncthreads();
+    // Lane (n, g): outputs 4 g .. + 3 of each tile, of token n of each 16.
+    f32x4 base[2][kRunTiles];
+#pragma unroll
+    for (int t = 0; t < kRunTiles; ++t) {
+      const float* row =
+          a.base + (uint64_t)(run.first + min(16u * t + n, run.tokens - 1)) * a.base_stride;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) base[i][t] = load4(row, o + 16 * i + 4 * g, a.rows);
+    }
     f32x4 acc[2][kRunTiles];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -319,16 +339,6 @@ __global__ __launch_bounds__(64 * kUpWaves, 3) void adapter_up_kernel(AdapterArg
                 32 * c + 8 * g + j < rank ? w[c & 1][i].at(j) : 0.0f, j < 4 ? h0[j & 3] : h1[j & 3],
                 acc[i][t], 0, 0, 0);
       }
-    }
-    // Lane (n, g): outputs 4 g .. + 3 of each tile, of token n of each 16.
-    f32x4 base[2][kRunTiles];
-#pragma unroll
-    for (int t = 0; t < kRunTiles; ++t) {
-      if (t >= run_tiles) break;
-      const float* src =
-          a.base + (uint64_t)(run.first + min(16u * t + n, run.tokens - 1)) * a.base_stride;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) base[i][t] = load4(src, o + 16 * i + 4 * g, a.rows);
     }
 #pragma unroll
     for (int t = 0; t < kRunTiles; ++t) {
@@ -437,12 +447,11 @@ __global__ __launch_bounds__(64 * kTokenWaves, 2) void adapter_token_kernel(Adap
 
 template <int kFormat, int kTiles>
 hipError_t launch_up(hipStream_t s, const AdapterArgs& a) {
-  // As many workgroups as items where every token is a run; past a bound each
-  // takes every so many.
+  // As many workgroups as items where every token is a run.
   const uint32_t blocks = (a.rows + kBlockRows - 1) / kBlockRows;
   const uint64_t items = (uint64_t)a.tokens * (blocks < 8 ? blocks : (blocks + 7) / 8 * 8);
   hipLaunchKernelGGL((adapter_up_kernel<kFormat, kTiles>),
-                     dim3((uint32_t)(items < kMostWorkgroups ? items : kMostWorkgroups)),
+                     dim3((uint32_t)(items < kMostUp ? items : kMostUp)),
                      dim3(64 * kUpWaves), 0, s, a);
   return hipGetLastError();
 }
@@ -466,14 +475,14 @@ hipError_t launch_format(hipStream_t s, AdapterArgs a) {
   // Splits of whole turns of a workgroup's waves, so many that the runs'
   // workgroups fill the chip.
   const uint32_t items = (a.tokens + 15) / 16 * ((a.rank + 15) / 16);
-  uint32_t splits = 512 / items;
+  uint32_t splits = 384 / items;
   splits = splits < 1 ? 1 : splits > kMostAdapterSplits ? kMostAdapterSplits : splits;
   const int turns = (a.cols + kTurnCols - 1) / kTurnCols;
   a.split_cols = kTurnCols * ((turns + (int)splits - 1) / (int)splits);
   a.splits = (a.cols + a.split_cols - 1) / a.split_cols;
   const uint64_t down = (uint64_t)((a.tokens + 7) / 8 * 8) * ((a.rank + 15) / 16) * a.splits;
   hipLaunchKernelGGL(adapter_down_kernel<kFormat>,
-                     dim3((uint32_t)(down < kMostWorkgroups ? down : kMostWorkgroups)),
+                     dim3((uint32_t)(down < kMostDown ? down : kMostDown)),
                      dim3(64 * kDownWaves), 0, s, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
