@@ -170,71 +170,80 @@ __device__ __forceinline__ void copy_base(const AdapterArgs& a, uint32_t first, 
 }
 
 // A wave's share of D x for a run of up to 16 tokens, over the columns
-// [from, to) and 16 ranks from `rank0` on: every kWaves-th 32 of the columns.
-// Lane (n, g) gets token n's ranks rank0 + 4 g .. + 3.
-template <int kFormat, int kWaves>
-__device__ __forceinline__ f32x4 low_rank(const AdapterArgs& a, const Run& run, int rank0, int from,
-                                          int to, int wave, int n, int g) {
-  constexpr int kDepth = 5;  // steps whose loads are in flight at once
-  constexpr int kTurn = 32 * kWaves;
+// [from, to) and kTiles tiles of 16 ranks from `rank0` on: every eighth 32 of
+// the columns. acc[t] has, in lane (n, g), token n's ranks rank0 + 16 t + 4 g
+// .. + 3.
+template <int kFormat, int kTiles>
+__device__ __forceinline__ void low_rank(const AdapterArgs& a, const Run& run, int rank0, int from,
+                                         int to, int wave, int n, int g, f32x4 (&acc)[kTiles]) {
+  // Steps whose loads are in flight at once.
+  constexpr int kDepth = kTiles == 1 ? 5 : kFormat == 0 ? 3 : 4;
   Raw<0> x[kDepth];
-  Raw<kFormat> w[kDepth];
+  Raw<kFormat> w[kDepth][kTiles];
   const float* row =
       a.x + (uint64_t)(run.first + ((uint32_t)n < run.tokens ? n : 0)) * a.x_stride;
-  const uint64_t pool =
-      ((uint64_t)run.adapter * a.rank + min(rank0 + n, a.rank - 1)) * (uint64_t)a.cols;
-  f32x4 acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int k0 = from + 32 * wave; k0 < to; k0 += kDepth * kTurn) {
+  const uint64_t pool = (uint64_t)run.adapter * a.rank * (uint64_t)a.cols;
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int k0 = from + 32 * wave; k0 < to; k0 += kDepth * kTurnCols) {
 #pragma unroll
     for (int i = 0; i < kDepth; ++i) {
-      if (k0 + i * kTurn >= to) continue;
+      if (k0 + i * kTurnCols >= to) continue;
       // Columns are multiples of 8, and so are splits.
-      const int at = k0 + i * kTurn + 8 * g, k = at < to ? at : from;
+      const int at = k0 + i * kTurnCols + 8 * g, k = at < to ? at : from;
       x[i].load(row, k);
-      w[i].load(a.down, pool + k);
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+        w[i][t].load(a.down,
+                     pool + (uint64_t)min(rank0 + 16 * t + n, a.rank - 1) * (uint64_t)a.cols + k);
     }
 #pragma unroll
     for (int i = 0; i < kDepth; ++i) {
-      if (k0 + i * kTurn >= to) continue;
-      const bool in = k0 + i * kTurn + 8 * g < to;
+      if (k0 + i * kTurnCols >= to) continue;
+      const bool in = k0 + i * kTurnCols + 8 * g < to;
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(in ? w[i].at(j) : 0.0f,
-                                                   in ? x[i].at(j) : 0.0f, acc, 0, 0, 0);
+      for (int j = 0; j < 8; ++j) {
+        const float xj = in ? x[i].at(j) : 0.0f;
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+          acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(in ? w[i][t].at(j) : 0.0f, xj, acc[t], 0,
+                                                        0, 0);
+      }
     }
   }
-  return acc;
 }
 
-// The low-rank rows of each run: a workgroup an item (run, 16 ranks, split of
-// K). Workgroups go round the eight dies: numbered by eights of runs, a run's
-// meet on one die, whose L2 then holds its rows of x alone.
-template <int kFormat>
+// The low-rank rows of each run: a workgroup an item (run, ranks of kTiles
+// tiles, split of K). Workgroups go round the eight dies: numbered by eights
+// of runs, a run's meet on one die, whose L2 then holds its rows of x alone.
+template <int kFormat, int kTiles>
 __global__ __launch_bounds__(64 * kDownWaves, 4) void adapter_down_kernel(AdapterArgs a) {
-  __shared__ f32x4 sums[kDownWaves][64];
+  __shared__ f32x4 sums[kDownWaves][kTiles][64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int n = lane & 15, g = lane >> 4;
   const Runs runs = find_runs<16>(a, lane);
   const uint32_t places = runs.count < 8 ? runs.count : (runs.count + 7) / 8 * 8;
-  const uint32_t groups = (a.rank + 15) / 16;
+  const uint32_t groups = (a.rank + 16 * kTiles - 1) / (16 * kTiles);
   const uint32_t items = places * groups * a.splits;
   for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
     if (item % places >= runs.count) continue;
     const Run run = run_at(a, runs, item % places);
     if (run.adapter == kNone) continue;
     const uint32_t piece = item / places, split = piece / groups;
-    const int rank0 = piece % groups * 16;
+    const int rank0 = piece % groups * 16 * kTiles;
     const int from = split * a.split_cols, to = min(from + a.split_cols, a.cols);
-    const f32x4 acc = low_rank<kFormat, kDownWaves>(a, run, rank0, from, to, wave, n, g);
+    f32x4 acc[kTiles];
+    low_rank<kFormat, kTiles>(a, run, rank0, from, to, wave, n, g, acc);
     __syncthreads();  // the last item's sums are read
-    sums[wave][lane] = acc;
-    __syncthreads();
-    const int r = rank0 + 4 * g;
-    if (wave == 0 && (uint32_t)n < run.tokens && r < a.rank) {
-      f32x4 sum = sums[0][lane];
 #pragma unroll
-      for (int w = 1; w < kDownWaves; ++w) sum += sums[w][lane];
+    for (int t = 0; t < kTiles; ++t) sums[wave][t][lane] = acc[t];
+    __syncthreads();
+    const int r = rank0 + 16 * wave + 4 * g;
+    if (wave < kTiles && (uint32_t)n < run.tokens && r < a.rank) {
+      f32x4 sum = sums[0][wave][lane];
+#pragma unroll
+      for (int w = 1; w < kDownWaves; ++w) sum += sums[w][wave][lane];
       *reinterpret_cast<f32x4*>(a.low + ((uint64_t)split * a.tokens + run.first + n) * a.rank + r) =
           sum;
     }
@@ -456,6 +465,24 @@ hipError_t launch_up(hipStream_t s, const AdapterArgs& a) {
   return hipGetLastError();
 }
 
+// Sets the splits.
+template <int kFormat, int kTiles>
+hipError_t launch_down(hipStream_t s, AdapterArgs& a) {
+  // Splits of whole turns of a workgroup's waves, so many that the runs'
+  // workgroups fill the chip.
+  const uint32_t groups = (a.rank + 16 * kTiles - 1) / (16 * kTiles);
+  uint32_t splits = 256 / ((a.tokens + 15) / 16 * groups);
+  splits = splits < 1 ? 1 : splits > kMostAdapterSplits ? kMostAdapterSplits : splits;
+  const int turns = (a.cols + kTurnCols - 1) / kTurnCols;
+  a.split_cols = kTurnCols * ((turns + (int)splits - 1) / (int)splits);
+  a.splits = (a.cols + a.split_cols - 1) / a.split_cols;
+  const uint64_t items = (uint64_t)((a.tokens + 7) / 8 * 8) * groups * a.splits;
+  hipLaunchKernelGGL((adapter_down_kernel<kFormat, kTiles>),
+                     dim3((uint32_t)(items < kMostDown ? items : kMostDown)),
+                     dim3(64 * kDownWaves), 0, s, a);
+  return hipGetLastError();
+}
+
 template <int kFormat>
 hipError_t launch_format(hipStream_t s, AdapterArgs a) {
   const uint64_t weights = (uint64_t)a.rank * a.cols * (kFormat == 0 ? 4 : 2);
@@ -472,19 +499,7 @@ hipError_t launch_format(hipStream_t s, AdapterArgs a) {
                        dim3(turn), 0, s, a);
     return hipGetLastError();
   }
-  // Splits of whole turns of a workgroup's waves, so many that the runs'
-  // workgroups fill the chip.
-  const uint32_t items = (a.tokens + 15) / 16 * ((a.rank + 15) / 16);
-  uint32_t splits = 384 / items;
-  splits = splits < 1 ? 1 : splits > kMostAdapterSplits ? kMostAdapterSplits : splits;
-  const int turns = (a.cols + kTurnCols - 1) / kTurnCols;
-  a.split_cols = kTurnCols * ((turns + (int)splits - 1) / (int)splits);
-  a.splits = (a.cols + a.split_cols - 1) / a.split_cols;
-  const uint64_t down = (uint64_t)((a.tokens + 7) / 8 * 8) * ((a.rank + 15) / 16) * a.splits;
-  hipLaunchKernelGGL(adapter_down_kernel<kFormat>,
-                     dim3((uint32_t)(down < kMostDown ? down : kMostDown)),
-                     dim3(64 * kDownWaves), 0, s, a);
-  hipError_t e = hipGetLastError();
+  const hipError_t e = a.rank <= 16 ? launch_down<kFormat, 1>(s, a) : launch_down<kFormat, 2>(s, a);
   if (e != hipSuccess) return e;
   if (a.rank <= 32) return launch_up<kFormat, 2>(s, a);
   if (a.rank <= 64) return launch_up<kFormat, 4>(s, a);

@@ -132,92 +132,101 @@ __device__ __forceinline__ float across_columns(float x) {
   return x;
 }
 
-__device__ __forceinline__ uint32_t wave_sum_before(uint32_t x, int lane, uint32_t* total) {
-  uint32_t sum = x;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t up = __shfl_up(sum, o);
-    if (lane >= o) sum += up;
-  }
-  *total = __shfl(sum, 63);
-  return sum - x;
+// x of the lanes up to this one, summed (DPP: row_shr 1, 2, 4, 8, then the
+// rows' last lanes broadcast to the rows after).
+template <int kCtrl, int kRows>
+__device__ __forceinline__ uint32_t add_dpp(uint32_t x) {
+  return x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, kCtrl, kRows, 0xF, false);
+}
+__device__ __forceinline__ uint32_t wave_sum_to(uint32_t x) {
+  x = add_dpp<0x111, 0xF>(x);
+  x = add_dpp<0x112, 0xF>(x);
+  x = add_dpp<0x114, 0xF>(x);
+  x = add_dpp<0x118, 0xF>(x);
+  x = add_dpp<0x142, 0xA>(x);
+  return add_dpp<0x143, 0xC>(x);
+}
+
+__device__ __forceinline__ uint32_t lane_of(uint32_t x, int lane) {
+  return (uint32_t)__builtin_amdgcn_readlane((int)x, lane);
 }
 
 // What a workgroup works on.
 struct Part {
   uint32_t row, position, sequence;
-  uint32_t unit;         // the row's head block
-  uint32_t index, parts; // of the unit's parts
+  uint32_t unit;          // the row's head block
+  uint32_t index, parts;  // of the unit's parts
   uint32_t chunk;
-  uint32_t slot;         // the unit's first state, where it has several parts
-  uint32_t record;       // the unit's number among those
-  uint32_t records;      // of them
+  uint32_t slot;          // the unit's first state, where it has several parts
+  uint32_t record;        // the unit's number among those
+  uint32_t records;       // of them
 };
 
 // The part numbered `want`, found by each wave for itself from the rows'
-// positions: the rows' blocks give the chunk, the chunk each row's parts,
-// and those the row. False past the last part (but for the records' number).
+// positions, kPer rows a lane: the rows' blocks give the chunk, the chunk each
+// row's parts, and those the row. False past the last part (but for the
+// records' number).
+template <int kPer>
 __device__ __forceinline__ bool find_part(const PagedAttentionArgs& a, uint32_t want, int lane,
                                           Part* out) {
-  constexpr int kPer = kMostRows / 64;
-  const uint32_t per = (a.rows + 63) / 64, capacity = a.cache.width * a.cache.page_slots;
+  const uint32_t capacity = a.cache.width * a.cache.page_slots;
   uint32_t position[kPer], sequence[kPer], blocks[kPer];
 #pragma unroll
+  for (int i = 0; i < kPer; ++i) position[i] = a.positions[min((uint32_t)lane * kPer + i, a.rows - 1)];
+#pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const uint32_t r = lane * per + i;
-    const bool live = (uint32_t)i < per && r < a.rows;
-    position[i] = live ? a.positions[r] : kNone;
-    sequence[i] = live && a.sequences ? a.sequences[r] : r;
+    const uint32_t r = min((uint32_t)lane * kPer + i, a.rows - 1);
+    sequence[i] = a.sequences ? a.sequences[r] : r;
   }
   uint32_t mine = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
+    if ((uint32_t)lane * kPer + i >= a.rows) position[i] = kNone;
     const uint32_t held = sequence[i] < a.cache.sequences ? capacity : 0;
     blocks[i] = position[i] == kNone ? 0 : row_blocks(key_range(position[i], a.window, held));
     mine += blocks[i];
   }
-  uint32_t all;
-  wave_sum_before(mine, lane, &all);
+  const uint32_t all = lane_of(wave_sum_to(mine), 63);
   const uint32_t chunk = part_chunk((uint64_t)all * a.units, a.target);
+  // A row's blocks are below 2^20, so that their quotient is right within one
+  // from F32.
+  const float each = 1.0f / (float)(chunk ? chunk : 1);
   uint32_t parts[kPer], total = 0, joined = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    parts[i] = chunk ? (blocks[i] + chunk - 1) / chunk : 0;
-    total += parts[i];
-    joined += parts[i] > 1 ? parts[i] + (1u << 20) : 0;  // parts, and rows above them
+    uint32_t n = (uint32_t)((float)blocks[i] * each);
+    n += n * chunk < blocks[i];
+    n += n * chunk < blocks[i];
+    n -= n > 0 && (n - 1) * chunk >= blocks[i];
+    parts[i] = n;
+    total += n;
+    joined += n > 1 ? n + (1u << 20) : 0;  // parts, and rows above them
   }
   // Sums of rows' parts stay below 2^20, all their parts of one head block.
-  uint32_t count, joins;
-  uint32_t before = wave_sum_before(total, lane, &count);
-  uint32_t joined_before = wave_sum_before(joined, lane, &joins);
-  out->records = (joins >> 20) * a.units;
-  const bool owner = want >= before * a.units && want < (before + total) * a.units;
-  const uint64_t owners = __ballot(owner);
+  const uint32_t to = wave_sum_to(total), joined_to = wave_sum_to(joined);
+  out->records = (lane_of(joined_to, 63) >> 20) * a.units;
+  const uint64_t owners = __ballot(want < to * a.units);
   if (owners == 0) return false;
-  const int leader = __builtin_ctzll(owners);
-  Part p{};
-  uint32_t rest = want - before * a.units;
+  const int leader = __builtin_ctzll(owners);  // the first lane whose parts reach past `want`
+  uint32_t rest = want - (to - total) * a.units, joined_before = joined_to - joined;
+  uint32_t row = 0, position_ = 0, sequence_ = 0, parts_ = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    if (p.parts == 0) {
-      if (rest < parts[i] * a.units) {
-        p.row = lane * per + i;
-        p.position = position[i];
-        p.sequence = sequence[i];
-        p.parts = parts[i];
-      } else {
-        rest -= parts[i] * a.units;
-        joined_before += parts[i] > 1 ? parts[i] + (1u << 20) : 0;
-      }
-    }
+    const bool here = parts_ == 0 && rest < parts[i] * a.units;
+    row = here ? lane * kPer + i : row;
+    position_ = here ? position[i] : position_;
+    sequence_ = here ? sequence[i] : sequence_;
+    parts_ = here ? parts[i] : parts_;
+    const bool past = parts_ == 0;
+    rest -= past ? parts[i] * a.units : 0;
+    joined_before += past && parts[i] > 1 ? parts[i] + (1u << 20) : 0;
   }
-  auto lead = [&](uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, leader); };
-  out->row = lead(p.row);
-  out->position = lead(p.position);
-  out->sequence = lead(p.sequence);
-  out->parts = lead(p.parts);
-  rest = lead(rest);
-  joined_before = lead(joined_before);
+  out->row = lane_of(row, leader);
+  out->position = lane_of(position_, leader);
+  out->sequence = lane_of(sequence_, leader);
+  out->parts = lane_of(parts_, leader);
+  rest = lane_of(rest, leader);
+  joined_before = lane_of(joined_before, leader);
   out->chunk = chunk;
   // Neighbouring workgroups take the head blocks of the same keys, whose
   // rows lie side by side.
@@ -242,7 +251,8 @@ __global__ __launch_bounds__(kThreads, kWorkgroups<kD>) void paged_attention_ker
   const int n = lane & 15, g = lane >> 4;
 
   Part part;
-  const bool found = find_part(a, blockIdx.x, lane, &part);
+  const bool found = a.rows <= 64 ? find_part<1>(a, blockIdx.x, lane, &part)
+                                  : find_part<kMostRows / 64>(a, blockIdx.x, lane, &part);
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.record_count = part.records;
   if (!found) return;
   const uint32_t head_blocks = a.units / a.cache.kv_heads;
