@@ -69,29 +69,38 @@ FRZ_RULE uint32_t row_blocks(KeyRange r) {
   return (r.end + kBlockKeys - 1) / kBlockKeys - r.first / kBlockKeys;
 }
 
-// Parts that a batch aims for: what its `units` (rows times head blocks) leave
-// of the workgroups that run at once, so that all parts of few long rows run
-// together; two for each of those where the rows alone nearly fill them.
-FRZ_RULE uint32_t part_target(uint32_t units, uint32_t at_once) {
-  return units <= at_once / 2 ? at_once - units : 2 * at_once;
-}
-
-// Blocks of a part, for the batch's blocks in all (each row's counted once a
-// head block).
-FRZ_RULE uint32_t part_chunk(uint64_t blocks, uint32_t target) {
-  const uint64_t even = (blocks + target - 1) / target;
+// Blocks of a part: as few as leave no more parts than workgroups run at once,
+// in fours. A part's time is mostly the same whatever its length (its rows'
+// positions, then its pages, then its first keys come one after another), so a
+// second round of parts would cost more than longer ones do. The fewest are
+// between the batch's blocks shared out evenly and those shared over what the
+// `units` (rows times head blocks) leave, as each has at most one part that is
+// not full; `parts` counts a chunk's parts, and six halvings come near enough.
+// Where the units alone are more than run at once, an even share.
+FRZ_RULE uint32_t even_chunk(uint64_t blocks, uint32_t share) {
+  const uint64_t even = (blocks + share - 1) / share;
   return (uint32_t)((even + kPartWaves - 1) / kPartWaves * kPartWaves);
 }
+template <typename Count>
+FRZ_RULE uint32_t part_chunk(uint64_t blocks, uint32_t units, uint32_t at_once, Count parts) {
+  uint32_t low = even_chunk(blocks, at_once);
+  if (units >= at_once || parts(low) <= at_once) return low;
+  uint32_t high = even_chunk(blocks, at_once - units);
+  for (int i = 0; i < 6 && high - low > kPartWaves; ++i) {
+    const uint32_t mid = low + (high - low) / (2 * kPartWaves) * kPartWaves;
+    if (parts(mid) <= at_once) high = mid;
+    else low = mid;
+  }
+  return high;
+}
 
-// The most parts there can be (a row has less than one part more than its
-// blocks fill), and the most that belong to rows of several parts: such a row
-// has fewer than twice the parts that its blocks fill.
+// The most parts there can be, and the most that belong to rows of several
+// parts: such a row has fewer than twice the parts that its blocks fill.
 FRZ_RULE uint32_t most_parts(uint32_t units, uint32_t at_once) {
-  return part_target(units, at_once) + units;
+  return units < at_once ? at_once : at_once + units;
 }
 FRZ_RULE uint32_t most_joined_parts(uint32_t units, uint32_t at_once) {
-  const uint32_t all = most_parts(units, at_once), twice = 2 * part_target(units, at_once);
-  return all < twice ? all : twice;
+  return units < at_once ? at_once : 2 * at_once;
 }
 
 }  // namespace rules

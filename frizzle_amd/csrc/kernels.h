@@ -483,11 +483,11 @@ struct PagedAttentionArgs {
   float* stats;
   uint4* records;
   uint32_t* record_count;
-  uint32_t units = 0, target = 0;  // set by the launcher
+  uint32_t units = 0, at_once = 0;  // set by the launcher
 };
 constexpr int kMostComputeUnits = 256;  // gfx950's
-constexpr int kAttentionWorkgroups = 2;  // a compute unit's at once
-constexpr int kMostJoinedParts = 4 * kAttentionWorkgroups * kMostComputeUnits;
+constexpr int kAttentionWorkgroups = 4;  // a compute unit's at once, at most
+constexpr int kMostJoinedParts = 2 * kAttentionWorkgroups * kMostComputeUnits;
 hipError_t launch_paged_attention(hipStream_t s, const PagedAttentionArgs& a, int compute_units);
 
 struct AdapterArgs {

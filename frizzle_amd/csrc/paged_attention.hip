@@ -31,8 +31,6 @@
 // Keys outside the row's range or in no page are never read: a lane's row is
 // clamped to one that the row reads, and its score is -inf.
 
-#include <math.h>
-
 #include "batch_rules.h"
 #include "kernels.h"
 #include "numerics.h"
@@ -79,31 +77,38 @@ struct Shape {
   static constexpr int kParts = Types<kBf16>::kParts;
   static constexpr int kPerTile = 16 / kW;                              // parts a column tile holds
   static constexpr int kTiles = (kParts + kPerTile - 1) / kPerTile;     // column tiles
+  static constexpr bool kSpare = kTiles * kPerTile > kParts;            // columns of no part
   static constexpr int kChunks = kD / 32;                               // of a key row
   static constexpr int kVec = kD >= 128 ? 8 : 4;                        // values a lane loads at once
   static constexpr int kSpans = kD / (16 * kVec);                       // of a value row
 };
 
-// Workgroups a compute unit runs at once: the registers of heads of 256 leave
-// room for one.
-template <int kD>
-constexpr int kWorkgroups = kD == 256 ? 1 : kAttentionWorkgroups;
+// Workgroups a compute unit runs at once, by the registers that a shape takes.
+template <int kD, bool kBf16, int kW>
+constexpr int kWorkgroups = kD == 256   ? 1
+                            : kD == 128 ? (Shape<kD, kBf16, kW>::kTiles == 1 ? 3 : 2)
+                                        : (Shape<kD, kBf16, kW>::kTiles <= 2 ? 4 : 3);
+static_assert(kWorkgroups<64, false, 8> <= kAttentionWorkgroups, "the workspace holds their parts");
 
-// Part `part` of x, of which the parts add up: x rounded, what that left
-// rounded, and so on; 0 past the format's parts.
+// A column's part of a value: what rounding it left to the parts before, taken
+// off (`less` holds -1 for each of those, 0 for the others), rounded in its turn.
 template <bool kBf16>
-__device__ __forceinline__ typename Types<kBf16>::scalar split_part(float x, int part) {
-  typedef typename Types<kBf16>::scalar T;
-  const T hi = (T)x;
-  float rest = x - (float)hi;
-  const T lo = (T)rest;
-  T r = part == 0 ? hi : lo;
-  if constexpr (kBf16) {
-    rest -= (float)lo;
-    r = part == 2 ? (T)rest : r;
+struct Column {
+  float keep;     // 1; 0 for a column past the format's parts
+  float less[2];
+  Column() = default;
+  __device__ __forceinline__ explicit Column(int part) {
+    keep = part < Types<kBf16>::kParts ? 1.0f : 0.0f;
+    less[0] = part >= 1 ? -1.0f : 0.0f;
+    less[1] = part >= 2 ? -1.0f : 0.0f;
   }
-  return part < Types<kBf16>::kParts ? r : (T)0.0f;
-}
+  __device__ __forceinline__ typename Types<kBf16>::scalar part_of(float x) const {
+    typedef typename Types<kBf16>::scalar T;
+    x = fmaf_(less[0], (float)(T)x, x);
+    if constexpr (kBf16) x = fmaf_(less[1], (float)(T)x, x);
+    return (T)x;
+  }
+};
 
 // x of the lanes 32 and 16 away, reduced with the lane's own: every lane of
 // the four that share n = lane % 16 gets all four's result.
@@ -147,6 +152,9 @@ __device__ __forceinline__ uint32_t wave_sum_to(uint32_t x) {
   return add_dpp<0x143, 0xC>(x);
 }
 
+// Nothing is moved past here: registers hold one block's rows, not two.
+__device__ __forceinline__ void hold() { __builtin_amdgcn_sched_barrier(0); }
+
 __device__ __forceinline__ uint32_t lane_of(uint32_t x, int lane) {
   return (uint32_t)__builtin_amdgcn_readlane((int)x, lane);
 }
@@ -187,21 +195,29 @@ __device__ __forceinline__ bool find_part(const PagedAttentionArgs& a, uint32_t 
     mine += blocks[i];
   }
   const uint32_t all = lane_of(wave_sum_to(mine), 63);
-  const uint32_t chunk = part_chunk((uint64_t)all * a.units, a.target);
-  // A row's blocks are below 2^20, so that their quotient is right within one
-  // from F32.
-  const float each = 1.0f / (float)(chunk ? chunk : 1);
-  uint32_t parts[kPer], total = 0, joined = 0;
+  uint32_t parts[kPer], total, joined;
+  auto cut = [&](uint32_t chunk) {
+    // A row's blocks are below 2^20, so that their quotient is right within one
+    // from F32.
+    const float each = 1.0f / (float)(chunk ? chunk : 1);
+    total = joined = 0;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    uint32_t n = (uint32_t)((float)blocks[i] * each);
-    n += n * chunk < blocks[i];
-    n += n * chunk < blocks[i];
-    n -= n > 0 && (n - 1) * chunk >= blocks[i];
-    parts[i] = n;
-    total += n;
-    joined += n > 1 ? n + (1u << 20) : 0;  // parts, and rows above them
-  }
+    for (int i = 0; i < kPer; ++i) {
+      uint32_t n = (uint32_t)((float)blocks[i] * each);
+      n += n * chunk < blocks[i];
+      n += n * chunk < blocks[i];
+      n -= n > 0 && (n - 1) * chunk >= blocks[i];
+      parts[i] = n;
+      total += n;
+      joined += n > 1 ? n + (1u << 20) : 0;  // parts, and rows above them
+    }
+  };
+  const uint32_t chunk =
+      part_chunk((uint64_t)all * a.units, a.rows * a.units, a.at_once, [&](uint32_t c) {
+        cut(c);
+        return lane_of(wave_sum_to(total), 63) * a.units;
+      });
+  cut(chunk);
   // Sums of rows' parts stay below 2^20, all their parts of one head block.
   const uint32_t to = wave_sum_to(total), joined_to = wave_sum_to(joined);
   out->records = (lane_of(joined_to, 63) >> 20) * a.units;
@@ -239,7 +255,7 @@ __device__ __forceinline__ bool find_part(const PagedAttentionArgs& a, uint32_t 
 }
 
 template <int kD, bool kBf16, int kW>
-__global__ __launch_bounds__(kThreads, kWorkgroups<kD>) void paged_attention_kernel(
+__global__ __launch_bounds__(kThreads, (kWorkgroups<kD, kBf16, kW>)) void paged_attention_kernel(
     PagedAttentionArgs a) {
   typedef Shape<kD, kBf16, kW> S;
   typedef Types<kBf16> T;
@@ -271,7 +287,7 @@ __global__ __launch_bounds__(kThreads, kWorkgroups<kD>) void paged_attention_ker
 
   // The wave's next 32 blocks' pages, a lane a half block of 16 keys: where
   // that half's first key lies in the pool, in values, or ~0.
-  const uint64_t row_stride = (uint64_t)a.cache.kv_heads * kD;
+  const uint32_t row_values = a.cache.kv_heads * kD, row_bytes = 2 * row_values;
   auto find_pages = [&](uint32_t block) {
     const uint32_t key = (block + kPartWaves * (lane >> 1)) * kBlockKeys + 16 * (lane & 1);
     uint64_t at = ~0ull;
@@ -280,7 +296,7 @@ __global__ __launch_bounds__(kThreads, kWorkgroups<kD>) void paged_attention_ker
       const uint32_t page = page_at(a.cache.table, a.cache.sequences, a.cache.width,
                                     a.cache.pages, part.sequence, index);
       if (page != kNone)
-        at = page * a.cache.page_stride + (key - index * a.cache.page_slots) * row_stride;
+        at = page * a.cache.page_stride + (uint64_t)(key - index * a.cache.page_slots) * row_values;
     }
     return at;
   };
@@ -288,44 +304,23 @@ __global__ __launch_bounds__(kThreads, kWorkgroups<kD>) void paged_attention_ker
   uint64_t pages = find_pages(block);
 
   // The query's columns: column n of tile t is part t kPerTile + n / W of
-  // head n % W.
+  // head n % W; a column past the heads takes the first one's query.
   const uint32_t head = n % kW;
-  float scale;  // what turns the scaled query's products into log2 units
-  uint4 q[S::kTiles][S::kChunks];
+  Column<kBf16> columns[S::kTiles];
+#pragma unroll
+  for (int t = 0; t < S::kTiles; ++t) columns[t] = Column<kBf16>(t * S::kPerTile + n / kW);
+  float x[S::kChunks][8];
   {
-    const bool live = head < heads;
     const float* src =
-        a.query + (uint64_t)part.row * a.q_stride + (uint64_t)(head0 + (live ? head : 0)) * kD;
-    float x[S::kChunks][8];
-    float most = 0.0f;
+        a.query + (uint64_t)part.row * a.q_stride + (uint64_t)(head0 + (head < heads ? head : 0)) * kD;
 #pragma unroll
     for (int c = 0; c < S::kChunks; ++c) {
       const float4 lo = *reinterpret_cast<const float4*>(src + 32 * c + 8 * g);
       const float4 hi = *reinterpret_cast<const float4*>(src + 32 * c + 8 * g + 4);
       const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[c][i] = live ? v[i] : 0.0f;
-        most = __builtin_fmaxf(most, __builtin_fabsf(x[c][i]));
-      }
+      for (int i = 0; i < 8; ++i) x[c][i] = v[i];
     }
-    most = across_groups(most, [](float p, float r) { return __builtin_fmaxf(p, r); });
-    // 2^up takes the largest to [2^14, 2^15); zeros, infinities and the
-    // smallest values as far as both factors stay ordinary numbers.
-    int up = 141 - (int)(float_to_bits(most) >> 23);
-    up = up > 100 ? 100 : up < -100 ? -100 : up;
-    const float factor = bits_to_float((uint32_t)(127 + up) << 23);
-    scale = a.scale_log2e * bits_to_float((uint32_t)(127 - up) << 23);
-#pragma unroll
-    for (int t = 0; t < S::kTiles; ++t)
-#pragma unroll
-      for (int c = 0; c < S::kChunks; ++c) {
-        typename T::vec v;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          v[i] = split_part<kBf16>(x[c][i] * factor, t * S::kPerTile + n / kW);
-        q[t][c] = __builtin_bit_cast(uint4, v);
-      }
   }
 
   const uint16_t* key_pool = a.cache.keys + (uint64_t)kv * kD;
@@ -365,26 +360,27 @@ __global__ __launch_bounds__(kThreads, kWorkgroups<kD>) void paged_attention_ker
   auto load_keys = [&](const Block& k) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint16_t* src = key_pool + k.at[h];
-      const uint32_t at = min(max(n, k.from[h]), k.to[h] - 1) * (uint32_t)row_stride + 8 * g;
+      // Bytes from a uniform address, in 32 bits: at most 15 rows.
+      const char* src = reinterpret_cast<const char*>(key_pool + k.at[h]);
+      const uint32_t at = min(max(n, k.from[h]), k.to[h] - 1) * row_bytes + 16 * g;
 #pragma unroll
       for (int c = 0; c < S::kChunks; ++c)
-        key_rows[h][c] = *reinterpret_cast<const uint4*>(src + at + 32 * c);
+        key_rows[h][c] = *reinterpret_cast<const uint4*>(src + (at + 64 * c));
     }
   };
   uint4 value_rows[2][4][S::kSpans];
   auto load_values = [&](const Block& k) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint16_t* src = value_pool + k.at[h];
+      const char* src = reinterpret_cast<const char*>(value_pool + k.at[h]);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint32_t at =
-            min(max(4 * g + e, k.from[h]), k.to[h] - 1) * (uint32_t)row_stride + S::kVec * n;
+            min(max(4 * g + e, k.from[h]), k.to[h] - 1) * row_bytes + 2 * S::kVec * n;
 #pragma unroll
         for (int s = 0; s < S::kSpans; ++s) {
           if constexpr (S::kVec == 8) {
-            value_rows[h][e][s] = *reinterpret_cast<const uint4*>(src + at + 128 * s);
+            value_rows[h][e][s] = *reinterpret_cast<const uint4*>(src + (at + 256 * s));
           } else {
             const uint2 v = *reinterpret_cast<const uint2*>(src + at);
             value_rows[h][e][s] = make_uint4(v.x, v.y, 0, 0);
@@ -415,81 +411,117 @@ __global__ __launch_bounds__(kThreads, kWorkgroups<kD>) void paged_attention_ker
     }
     return false;
   };
-  bool more = seek(&now);
-  if (more) load_keys(now);
-  while (more) {
-    load_values(now);
-    f32x4 scores[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      scores[h] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  if (seek(&now)) {
+    load_keys(now);
+    hold();
+    float scale;  // what turns the scaled query's products into log2 units
+    uint4 q[S::kTiles][S::kChunks];
+    {
+      float most = 0.0f;
 #pragma unroll
       for (int c = 0; c < S::kChunks; ++c)
 #pragma unroll
-        for (int t = 0; t < S::kTiles; ++t)
-          scores[h] = T::mfma(key_rows[h][c], q[t][c], scores[h]);
-    }
-    block += kPartWaves;
-    ++turn;
-    more = seek(&next);
-    if (more) load_keys(next);
-
-    float most = kMinusInf;
+        for (int i = 0; i < 8; ++i) most = __builtin_fmaxf(most, __builtin_fabsf(x[c][i]));
+      most = across_groups(most, [](float p, float r) { return __builtin_fmaxf(p, r); });
+      // 2^up takes the largest to [2^14, 2^15); zeros, infinities and the
+      // smallest values as far as both factors stay ordinary numbers.
+      int up = 141 - (int)(float_to_bits(most) >> 23);
+      up = up > 100 ? 100 : up < -100 ? -100 : up;
+      const float factor = bits_to_float((uint32_t)(127 + up) << 23);
+      scale = a.scale_log2e * bits_to_float((uint32_t)(127 - up) << 23);
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+      for (int t = 0; t < S::kTiles; ++t) {
+        const float kept = factor * columns[t].keep;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float s = across_columns<kW>(scores[h][e]) * scale;
-        const bool live = 4 * g + e >= now.lo[h] && 4 * g + e < now.hi[h];
-        scores[h][e] = live ? s : kMinusInf;
-        most = __builtin_fmaxf(most, scores[h][e]);
+        for (int c = 0; c < S::kChunks; ++c) {
+          typename T::vec v;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = columns[t].part_of(x[c][i] * kept);
+          q[t][c] = __builtin_bit_cast(uint4, v);
+        }
       }
-    most = across_groups(most, [](float p, float r) { return __builtin_fmaxf(p, r); });
-    // A block that is worked on holds a key, so `most` is a number but where
-    // scores are not.
-    const float to = __builtin_fmaxf(m, most - kWeightScale);
-    if (__ballot(to > m)) {
-      const float old = __builtin_amdgcn_exp2f(m - to);
-      l *= old;
+    }
+    for (bool more = true; more;) {
+      load_values(now);
+      hold();
+      f32x4 scores[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        scores[h] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < S::kChunks; ++c)
+#pragma unroll
+          for (int t = 0; t < S::kTiles; ++t)
+            scores[h] = T::mfma(key_rows[h][c], q[t][c], scores[h]);
+      }
+      hold();
+      // The last block's keys once more where there is no next one: a branch
+      // around the loads would make the wait for the values one for these too.
+      block += kPartWaves;
+      ++turn;
+      more = seek(&next);
+      if (!more) next = now;
+      load_keys(next);
+      hold();
+      float most = kMinusInf;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float s = across_columns<kW>(scores[h][e]) * scale;
+          const bool live = 4 * g + e >= now.lo[h] && 4 * g + e < now.hi[h];
+          scores[h][e] = live ? s : kMinusInf;
+          most = __builtin_fmaxf(most, scores[h][e]);
+        }
+      most = across_groups(most, [](float p, float r) { return __builtin_fmaxf(p, r); });
+      // A block that is worked on holds a key, so `most` is a number but where
+      // scores are not.
+      const float to = __builtin_fmaxf(m, most - kWeightScale);
+      if (__ballot(to > m)) {
+        const float old = __builtin_amdgcn_exp2f(m - to);
+        l *= old;
+#pragma unroll
+        for (int s = 0; s < S::kSpans; ++s)
+#pragma unroll
+          for (int j = 0; j < S::kVec; ++j) out[s][j] *= old;
+        m = to;
+      }
+      float weight[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        weight[i] = __builtin_amdgcn_exp2f(scores[i >> 2][i & 3] - m);
+        l += weight[i];
+      }
+      uint4 w[S::kTiles];
+#pragma unroll
+      for (int t = 0; t < S::kTiles; ++t) {
+        typename T::vec v;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          v[i] = columns[t].part_of(S::kSpare ? weight[i] * columns[t].keep : weight[i]);
+        w[t] = __builtin_bit_cast(uint4, v);
+      }
+      hold();
 #pragma unroll
       for (int s = 0; s < S::kSpans; ++s)
 #pragma unroll
-        for (int j = 0; j < S::kVec; ++j) out[s][j] *= old;
-      m = to;
+        for (int j = 0; j < S::kVec; ++j) {
+          // The lane's 8 keys at dimension j of its span.
+          const uint32_t select = j & 1 ? 0x07060302u : 0x05040100u;
+          auto word = [&](int h, int e) {
+            const uint4& r = value_rows[h][e][s];
+            return (j >> 1) == 0 ? r.x : (j >> 1) == 1 ? r.y : (j >> 1) == 2 ? r.z : r.w;
+          };
+          auto pair = [&](int h, int e) {
+            return __builtin_amdgcn_perm(word(h, e + 1), word(h, e), select);
+          };
+          const uint4 v = make_uint4(pair(0, 0), pair(0, 2), pair(1, 0), pair(1, 2));
+#pragma unroll
+          for (int t = 0; t < S::kTiles; ++t) out[s][j] = T::mfma(v, w[t], out[s][j]);
+          if (j & 1) hold();
+        }
+      now = next;
     }
-    float weight[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      weight[i] = __builtin_amdgcn_exp2f(scores[i >> 2][i & 3] - m);
-      l += weight[i];
-    }
-    uint4 w[S::kTiles];
-#pragma unroll
-    for (int t = 0; t < S::kTiles; ++t) {
-      typename T::vec v;
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        v[i] = split_part<kBf16>(weight[i], t * S::kPerTile + n / kW);
-      w[t] = __builtin_bit_cast(uint4, v);
-    }
-#pragma unroll
-    for (int s = 0; s < S::kSpans; ++s)
-#pragma unroll
-      for (int j = 0; j < S::kVec; ++j) {
-        // The lane's 8 keys at dimension j of its span.
-        const uint32_t select = j & 1 ? 0x07060302u : 0x05040100u;
-        auto word = [&](int h, int e) {
-          const uint4& r = value_rows[h][e][s];
-          return (j >> 1) == 0 ? r.x : (j >> 1) == 1 ? r.y : (j >> 1) == 2 ? r.z : r.w;
-        };
-        auto pair = [&](int h, int e) {
-          return __builtin_amdgcn_perm(word(h, e + 1), word(h, e), select);
-        };
-        const uint4 v = make_uint4(pair(0, 0), pair(0, 2), pair(1, 0), pair(1, 2));
-#pragma unroll
-        for (int t = 0; t < S::kTiles; ++t) out[s][j] = T::mfma(v, w[t], out[s][j]);
-      }
-    now = next;
   }
 
   // The waves' states joined. Lane (n, g) holds dimensions 16 kVec s +
@@ -615,41 +647,39 @@ __global__ __launch_bounds__(kThreads) void paged_attention_join_kernel(PagedAtt
 }
 
 template <int kD, bool kBf16, int kW>
-void launch_parts(hipStream_t s, const PagedAttentionArgs& a, uint32_t grid) {
-  hipLaunchKernelGGL((paged_attention_kernel<kD, kBf16, kW>), dim3(grid), dim3(kThreads), 0, s, a);
-}
-
-template <int kD>
-hipError_t launch_shape(hipStream_t s, PagedAttentionArgs a, int compute_units) {
-  const uint32_t group = a.query_heads / a.cache.kv_heads;
-  const uint32_t heads = group < kHeadBlock ? group : kHeadBlock;
-  a.units = a.cache.kv_heads * ((group + kHeadBlock - 1) / kHeadBlock);
+hipError_t launch_shape(hipStream_t s, PagedAttentionArgs a, uint32_t heads, int compute_units) {
   const uint32_t units = a.rows * a.units;
-  const uint32_t at_once = kWorkgroups<kD> * (uint32_t)compute_units;
-  a.target = part_target(units, at_once);
+  a.at_once = kWorkgroups<kD, kBf16, kW> * (uint32_t)compute_units;
   // No more parts than the rows' blocks fill, at a part's least blocks.
   const uint64_t capacity = (uint64_t)a.cache.width * a.cache.page_slots;
   const uint64_t most_keys = a.window < capacity ? a.window : capacity;
   const uint64_t blocks = most_keys / kBlockKeys + 2;
   const uint64_t fill = units * ((blocks + kPartWaves - 1) / kPartWaves);
-  const uint64_t bound = most_parts(units, at_once);
-  const uint32_t grid = (uint32_t)(fill < bound ? fill : bound);
-  if (a.cache.bf16) {
-    if (heads <= 4) launch_parts<kD, true, 4>(s, a, grid);
-    else if (heads <= 8) launch_parts<kD, true, 8>(s, a, grid);
-    else launch_parts<kD, true, 16>(s, a, grid);
-  } else {
-    if (heads <= 8) launch_parts<kD, false, 8>(s, a, grid);
-    else launch_parts<kD, false, 16>(s, a, grid);
-  }
-  hipError_t e = hipGetLastError();
+  const uint64_t bound = most_parts(units, a.at_once);
+  hipLaunchKernelGGL((paged_attention_kernel<kD, kBf16, kW>),
+                     dim3((uint32_t)(fill < bound ? fill : bound)), dim3(kThreads), 0, s, a);
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess || blocks <= kPartWaves) return e;  // no row has two parts
-  const uint32_t joins = most_joined_parts(units, at_once) / 2;
+  const uint32_t joins = most_joined_parts(units, a.at_once) / 2;
   const uint32_t records = units < joins ? units : joins;
   hipLaunchKernelGGL(paged_attention_join_kernel<kD>,
                      dim3(records < 256 ? records : 256, heads * (kD / 64)), dim3(kThreads), 0, s,
                      a);
   return hipGetLastError();
+}
+
+template <int kD>
+hipError_t launch_heads(hipStream_t s, PagedAttentionArgs a, int compute_units) {
+  const uint32_t group = a.query_heads / a.cache.kv_heads;
+  const uint32_t heads = group < kHeadBlock ? group : kHeadBlock;
+  a.units = a.cache.kv_heads * ((group + kHeadBlock - 1) / kHeadBlock);
+  if (a.cache.bf16) {
+    if (heads <= 4) return launch_shape<kD, true, 4>(s, a, heads, compute_units);
+    if (heads <= 8) return launch_shape<kD, true, 8>(s, a, heads, compute_units);
+    return launch_shape<kD, true, 16>(s, a, heads, compute_units);
+  }
+  if (heads <= 8) return launch_shape<kD, false, 8>(s, a, heads, compute_units);
+  return launch_shape<kD, false, 16>(s, a, heads, compute_units);
 }
 
 }  // namespace
@@ -658,9 +688,9 @@ hipError_t launch_paged_attention(hipStream_t s, const PagedAttentionArgs& a, in
   if (a.rows == 0 || a.rows > kMostRows || compute_units <= 0 || compute_units > kMostComputeUnits)
     return hipErrorInvalidValue;
   switch (a.cache.head_dim) {
-    case 64: return launch_shape<64>(s, a, compute_units);
-    case 128: return launch_shape<128>(s, a, compute_units);
-    case 256: return launch_shape<256>(s, a, compute_units);
+    case 64: return launch_heads<64>(s, a, compute_units);
+    case 128: return launch_heads<128>(s, a, compute_units);
+    case 256: return launch_heads<256>(s, a, compute_units);
     default: return hipErrorInvalidValue;
   }
 }

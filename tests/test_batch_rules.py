@@ -20,7 +20,6 @@ using namespace frz::rules;
 static void cut(const std::vector<uint32_t>& lengths, uint32_t window, uint32_t capacity,
                 uint32_t head_blocks, uint32_t at_once) {
   const uint32_t units = lengths.size() * head_blocks;
-  const uint32_t target = part_target(units, at_once);
   std::vector<uint32_t> blocks;
   uint64_t all = 0;
   for (uint32_t n : lengths) {
@@ -28,7 +27,11 @@ static void cut(const std::vector<uint32_t>& lengths, uint32_t window, uint32_t 
     blocks.push_back(b);
     all += b;
   }
-  const uint32_t chunk = part_chunk(all * head_blocks, target);
+  const uint32_t chunk = part_chunk(all * head_blocks, units, at_once, [&](uint32_t c) {
+    uint32_t n = 0;
+    for (uint32_t b : blocks) n += c ? (b + c - 1) / c : 0;
+    return n * head_blocks;
+  });
   uint64_t parts = 0, joined = 0;
   bool covered = true;
   for (uint32_t b : blocks) {
@@ -127,6 +130,6 @@ def test_every_block_in_one_part_within_the_grid(rules, lengths, window, capacit
     assert chunk % 4 == 0
     assert parts <= most
     # The workspace holds the parts of rows that have several.
-    assert joined <= most_joined <= 4 * at_once
+    assert joined <= most_joined <= 2 * at_once
     if any(lengths):
         assert chunk >= 4
