@@ -53,8 +53,10 @@ __global__ __launch_bounds__(256) void paged_rope_kernel(PagedRopeArgs a) {
     ga = ld4f(gain + 4 * l);
     gb = ld4f(gain + kHalf + 4 * l);
   }
-  // Where the row's keys and values go. Of rows that name one slot the last
-  // is kept: a row looks whether one of those after it does.
+  // Where the row's keys and values go. Of rows at one request's position the
+  // last is kept: a row looks whether one after it is there too, at all of
+  // them at once (each of few loads that wait for one another had taken twice
+  // the rest of a full step's kernel).
   uint64_t at = 0;
   bool kept = false;
   if (first + kWaveHeads > a.query_heads) {
@@ -64,17 +66,24 @@ __global__ __launch_bounds__(256) void paged_rope_kernel(PagedRopeArgs a) {
                                   sequence, index);
     kept = page != kNone;
     at = page * a.cache.page_stride + (uint64_t)slot * a.cache.kv_heads * kD;
-    bool again = false;
-#pragma unroll 2
-    for (uint32_t r = row + 1 + lane; r < a.rows; r += 64) {
-      const uint32_t other = a.positions[r];
-      const uint32_t s = a.sequences ? a.sequences[r] : r;
-      const uint32_t i = other / a.cache.page_slots;
-      if (other != kNone && other - i * a.cache.page_slots == slot)
-        again |= page_at(a.cache.table, a.cache.sequences, a.cache.width, a.cache.pages, s, i) ==
-                 page;
+    if (a.sequences) {  // without, each row is its own request
+      constexpr int kGroups = kMostRows / 64;
+      uint32_t other[kGroups], of[kGroups];
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) {
+        if (row + 1 + 64 * i >= a.rows) continue;
+        const uint32_t r = min(row + 1 + 64 * i + lane, a.rows - 1);
+        other[i] = a.positions[r];
+        of[i] = a.sequences[r];
+      }
+      bool again = false;
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) {
+        if (row + 1 + 64 * i >= a.rows) continue;
+        again |= row + 1 + 64 * i + lane < a.rows && other[i] == p && of[i] == sequence;
+      }
+      kept = kept && __ballot(again) == 0;
     }
-    kept = kept && __ballot(again) == 0;
   }
   const float4 turns = ld4f(a.turns + 4 * l);
   float cosine[4], sine[4];

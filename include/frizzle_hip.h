@@ -252,7 +252,8 @@ typedef struct frz_pages {
  * are q_stride, of key and value kv_stride floats apart; the roped queries go
  * to roped (roped_stride apart), which may be query itself, with its stride.
  * Keys and values round to the cache's format, to nearest even (F16
- * saturates at 65,504). Of rows that name one slot the last one's stay. */
+ * saturates at 65,504). Of rows at one request's position the last one's
+ * stay; two requests must not append to a page that they share. */
 int frz_op_rope_paged(frz_device* dev, const frz_pages* cache, const uint32_t* sequences,
                       const uint32_t* positions, const float* turns, const float* query_gain,
                       const float* key_gain, const float* query, const float* key,

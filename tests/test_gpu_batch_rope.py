@@ -109,26 +109,26 @@ def test_in_place_and_requests_in_any_order(device):
         assert np.array_equal(got.ravel(), to_format(value[row], F16))
 
 
-def test_the_last_of_rows_that_name_one_slot_stays(device):
+@pytest.mark.parametrize("rows", [2, 65, 150, 512])
+def test_the_last_of_rows_at_one_position_stays(device, rows):
     rng = np.random.default_rng(5)
     paged = Paged(device, rng, [64, 64, 64], 2, 64, 16, F16)
-    paged.table[2, 1] = paged.table[0, 3]  # two requests' page, at other positions
-    paged.upload()
-    rows = 150  # rows of one slot in other waves' reach too
+    # All at one request's position but a few, which come to be alone or last.
     requests, positions = np.zeros(rows, np.uint32), np.full(rows, 50, np.uint32)
-    requests[1::2], positions[1::2] = 2, 18
-    requests[2], positions[2] = 1, 50
-    positions[3] = NONE
-    requests[5], positions[5] = 0, 51
+    last = {(0, 50): rows - 1}
+    if rows > 2:
+        requests[2], last[1, 50] = 1, 2
+        positions[3] = NONE
+        positions[5] = positions[rows - 2] = 51
+        last[0, 51] = rows - 2
     query, key, value, gains = inputs(rng, rows, 4, 2, 64)
     rope(device, paged, positions, fz.rope_turns(1e4, 64), gains, query, key, value, 4, requests)
     keys, values, _ = paged.read()
-    at = paged.page(0, 50)
-    for page, slot, row in ((at, 2, rows - 1), (paged.page(1, 50), 2, 2), (at, 3, 5)):
-        assert np.array_equal(values[page, slot].ravel(), to_format(value[row], F16)), row
-        want, size = rope_exact(key[row].reshape(2, 64), gains[1], fz.rope_turns(1e4, 64),
-                                positions[row])
-        k = of_format(keys[page, slot], F16)
+    for (request, p), row in last.items():
+        at = paged.page(request, p), p % 16
+        assert np.array_equal(values[at].ravel(), to_format(value[row], F16)), row
+        want, size = rope_exact(key[row].reshape(2, 64), gains[1], fz.rope_turns(1e4, 64), p)
+        k = of_format(keys[at], F16)
         assert (abs(k - want) <= 2.0 ** -11 * abs(want) + 2 * near(size) + 2.0 ** -25).all()
 
 
