@@ -33,9 +33,10 @@ FLAGS = [
 ]
 
 
-# The prefill products keep their matrix accumulators in ordinary vector
-# registers, which the totals are added from.
-FILE_FLAGS = {"gemv.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form"]}
+# Matrix accumulators kept in ordinary vector registers: the prefill products'
+# totals are added from them, and the paged attention's outputs rescaled there.
+FILE_FLAGS = {f: ["-mllvm", "--amdgpu-mfma-vgpr-form"]
+              for f in ("gemv.hip", "paged_attention.hip")}
 
 
 def _compile(src: Path) -> Path:

@@ -8,8 +8,8 @@
 //
 // What bounds it is the stream of key and value rows, so nothing of it waits:
 // both go from memory to the registers that the matrix instructions read,
-// with no LDS between, a block's values requested before its scores are
-// formed and the next block's keys right after.
+// with no LDS between, the next block's keys requested as soon as a block's
+// scores are formed, its values as soon as the block's are used.
 //   S^T = K q^T   16 keys a tile, A = K: lane (n, g) holds 8 of key n's
 //                 values, as they lie in memory. It leaves the lane with the
 //                 scores of head n at keys 4g .. 4g + 3.
@@ -28,8 +28,8 @@
 // low parts stay clear of the formats' smallest values; both scales are
 // exact. Products are exact in F32, sums F32.
 //
-// Keys outside the row's range or in no page are never read: a lane's row is
-// clamped to one that the row reads, and its score is -inf.
+// Keys outside the row's range or in no page are never read: their rows are
+// zeros, and their scores -inf.
 
 #include "batch_rules.h"
 #include "kernels.h"
@@ -47,6 +47,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int kThreads = 64 * kPartWaves;
 constexpr float kWeightScale = 14.0f;  // weights are 2^14 at the running maximum
 constexpr float kMinusInf = -__builtin_inff();
+constexpr int kBufferWord3 = 0x00020000;  // raw 32-bit data
 
 template <bool kBf16>
 struct Types;
@@ -326,63 +327,60 @@ __global__ __launch_bounds__(kThreads, (kWorkgroups<kD, kBf16, kW>)) void paged_
   const uint16_t* key_pool = a.cache.keys + (uint64_t)kv * kD;
   const uint16_t* value_pool = a.cache.values + (uint64_t)kv * kD;
 
-  // A block: where its halves lie, and which of each half's 16 keys the row
-  // reads. A half without keys takes the other's rows.
+  // A block: where the rows that are read of each of its halves begin, and
+  // which of its 16 keys these are, [lo, hi).
   struct Block {
     uint64_t at[2];
-    int lo[2], hi[2];    // live keys of each half
-    int from[2], to[2];  // rows that may be read at `at`
+    int lo[2], hi[2];
   };
   auto locate = [&](uint32_t b, uint32_t turn, Block* k) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int from = 2 * turn + h;
-      const uint32_t low = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)pages, from);
-      const uint32_t high = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(pages >> 32), from);
-      k->at[h] = (uint64_t)high << 32 | low;
+      const uint64_t page = (uint64_t)lane_of((uint32_t)(pages >> 32), 2 * turn + h) << 32 |
+                            lane_of((uint32_t)pages, 2 * turn + h);
       const int key = (int)(b * kBlockKeys + 16 * h);
       k->lo[h] = max(0, (int)keys.first - key);
-      k->hi[h] = k->at[h] == ~0ull ? 0 : min(16, (int)keys.end - key);
-      k->from[h] = k->lo[h];
-      k->to[h] = k->hi[h];
+      k->hi[h] = page == ~0ull ? 0 : min(16, (int)keys.end - key);
+      const bool some = k->lo[h] < k->hi[h];
+      k->at[h] = some ? page + (uint64_t)k->lo[h] * row_values : 0;
+      k->hi[h] = some ? k->hi[h] : k->lo[h];
     }
-    const bool some[2] = {k->lo[0] < k->hi[0], k->lo[1] < k->hi[1]};
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (!some[h]) {
-        k->at[h] = k->at[1 - h];
-        k->from[h] = k->lo[1 - h];
-        k->to[h] = k->hi[1 - h];
-      }
-    return some[0] || some[1];
+    return k->lo[0] < k->hi[0] || k->lo[1] < k->hi[1];
+  };
+  // Rows come through a buffer of just those that are read: a lane whose row is
+  // before its start or past its end gets zeros, and no memory is touched.
+  auto rows_of = [&](const uint16_t* pool, const Block& k, int h) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(pool + k.at[h]), 0,
+                                             (k.hi[h] - k.lo[h]) * (int)row_bytes, kBufferWord3);
   };
   uint4 key_rows[2][S::kChunks];
   auto load_keys = [&](const Block& k) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      // Bytes from a uniform address, in 32 bits: at most 15 rows.
-      const char* src = reinterpret_cast<const char*>(key_pool + k.at[h]);
-      const uint32_t at = min(max(n, k.from[h]), k.to[h] - 1) * row_bytes + 16 * g;
+      const __amdgpu_buffer_rsrc_t rows = rows_of(key_pool, k, h);
+      const int at = (n - k.lo[h]) * (int)row_bytes + 16 * g;
 #pragma unroll
       for (int c = 0; c < S::kChunks; ++c)
-        key_rows[h][c] = *reinterpret_cast<const uint4*>(src + (at + 64 * c));
+        key_rows[h][c] = __builtin_bit_cast(
+            uint4, __builtin_amdgcn_raw_buffer_load_b128(rows, at + 64 * c, 0, 0));
     }
   };
   uint4 value_rows[2][4][S::kSpans];
   auto load_values = [&](const Block& k) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const char* src = reinterpret_cast<const char*>(value_pool + k.at[h]);
+      const __amdgpu_buffer_rsrc_t rows = rows_of(value_pool, k, h);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const uint32_t at =
-            min(max(4 * g + e, k.from[h]), k.to[h] - 1) * row_bytes + 2 * S::kVec * n;
+        const int at = (4 * g + e - k.lo[h]) * (int)row_bytes + 2 * S::kVec * n;
 #pragma unroll
         for (int s = 0; s < S::kSpans; ++s) {
           if constexpr (S::kVec == 8) {
-            value_rows[h][e][s] = *reinterpret_cast<const uint4*>(src + (at + 256 * s));
+            value_rows[h][e][s] = __builtin_bit_cast(
+                uint4, __builtin_amdgcn_raw_buffer_load_b128(rows, at + 256 * s, 0, 0));
           } else {
-            const uint2 v = *reinterpret_cast<const uint2*>(src + at);
+            const uint2 v = __builtin_bit_cast(
+                uint2, __builtin_amdgcn_raw_buffer_load_b64(rows, at, 0, 0));
             value_rows[h][e][s] = make_uint4(v.x, v.y, 0, 0);
           }
         }
@@ -409,10 +407,13 @@ __global__ __launch_bounds__(kThreads, (kWorkgroups<kD, kBf16, kW>)) void paged_
       }
       if (locate(block, turn, k)) return true;
     }
+    k->at[0] = k->at[1] = 0;
+    k->lo[0] = k->lo[1] = k->hi[0] = k->hi[1] = 0;  // no row
     return false;
   };
   if (seek(&now)) {
     load_keys(now);
+    load_values(now);
     hold();
     float scale;  // what turns the scaled query's products into log2 units
     uint4 q[S::kTiles][S::kChunks];
@@ -442,8 +443,6 @@ __global__ __launch_bounds__(kThreads, (kWorkgroups<kD, kBf16, kW>)) void paged_
       }
     }
     for (bool more = true; more;) {
-      load_values(now);
-      hold();
       f32x4 scores[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -455,14 +454,14 @@ __global__ __launch_bounds__(kThreads, (kWorkgroups<kD, kBf16, kW>)) void paged_
             scores[h] = T::mfma(key_rows[h][c], q[t][c], scores[h]);
       }
       hold();
-      // The last block's keys once more where there is no next one: a branch
-      // around the loads would make the wait for the values one for these too.
+      // After the last block, of no rows: a branch around the loads would make
+      // each wait one for all that are under way.
       block += kPartWaves;
       ++turn;
       more = seek(&next);
-      if (!more) next = now;
       load_keys(next);
       hold();
+
       float most = kMinusInf;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -520,6 +519,9 @@ __global__ __launch_bounds__(kThreads, (kWorkgroups<kD, kBf16, kW>)) void paged_
           for (int t = 0; t < S::kTiles; ++t) out[s][j] = T::mfma(v, w[t], out[s][j]);
           if (j & 1) hold();
         }
+      hold();
+      load_values(next);
+      hold();
       now = next;
     }
   }
