@@ -11,8 +11,8 @@
 // up to 16 of its query heads). A row of n blocks is cut into ceil(n / chunk)
 // parts, a workgroup each, for one chunk that the whole batch shares: a batch
 // of one long and many short requests then keeps every compute unit at work,
-// where a cut of so many parts a row would leave the long one last. The chunk
-// is a multiple of the workgroup's waves, a block a wave and turn.
+// where a cut of so many parts a row would leave the long one last. A part's
+// waves take its blocks in turn.
 
 #pragma once
 
@@ -69,22 +69,27 @@ FRZ_RULE uint32_t row_blocks(KeyRange r) {
   return (r.end + kBlockKeys - 1) / kBlockKeys - r.first / kBlockKeys;
 }
 
-// Blocks of a part: as few as leave no more parts than workgroups run at once,
-// in fours. A part's time is mostly the same whatever its length (its rows'
-// positions, then its pages, then its first keys come one after another), so a
-// second round of parts would cost more than longer ones do. The fewest are
-// between the batch's blocks shared out evenly and those shared over what the
-// `units` (rows times head blocks) leave, as each has at most one part that is
-// not full; `parts` counts a chunk's parts, and six halvings come near enough.
-// Where the units alone are more than run at once, an even share.
+// Blocks of a part: as few as leave no more parts than workgroups run at once.
+// A part's time is mostly the same whatever its length (its rows' positions,
+// then its pages, then its first keys come one after another), so a second
+// round of parts would cost more than longer ones do; and a compute unit takes
+// in about 40 GB/s, so few blocks are best spread over as many as there are,
+// though three of a workgroup's waves then idle (one request's 5,004 keys: 40
+// parts of four blocks 9.6 us, 157 of one 7.6). From four on, in fours. The
+// fewest are between the batch's blocks shared out evenly and those shared
+// over what the `units` (rows times head blocks) leave, as each has at most one
+// part that is not full; `parts` counts a chunk's parts, and six halvings come
+// near enough. Where the units alone are more than run at once, an even share.
 FRZ_RULE uint32_t even_chunk(uint64_t blocks, uint32_t share) {
   const uint64_t even = (blocks + share - 1) / share;
-  return (uint32_t)((even + kPartWaves - 1) / kPartWaves * kPartWaves);
+  return (uint32_t)(even <= 2 ? even : (even + kPartWaves - 1) / kPartWaves * kPartWaves);
 }
 template <typename Count>
 FRZ_RULE uint32_t part_chunk(uint64_t blocks, uint32_t units, uint32_t at_once, Count parts) {
   uint32_t low = even_chunk(blocks, at_once);
-  if (units >= at_once || parts(low) <= at_once) return low;
+  if (units >= at_once) return low;
+  while (low < kPartWaves && parts(low) > at_once) low = low < 2 ? 2 : kPartWaves;
+  if (parts(low) <= at_once) return low;
   uint32_t high = even_chunk(blocks, at_once - units);
   for (int i = 0; i < 6 && high - low > kPartWaves; ++i) {
     const uint32_t mid = low + (high - low) / (2 * kPartWaves) * kPartWaves;

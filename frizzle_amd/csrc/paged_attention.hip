@@ -624,7 +624,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_join_kernel(PagedAtt
     __syncthreads();
     const uint32_t group = t / 16;
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
+#pragma unroll 8
     for (uint32_t p = group; p < parts; p += kJoinGroups) {
       const float f = factors[p];
       const float4 o = *reinterpret_cast<const float4*>(
@@ -652,16 +652,17 @@ template <int kD, bool kBf16, int kW>
 hipError_t launch_shape(hipStream_t s, PagedAttentionArgs a, uint32_t heads, int compute_units) {
   const uint32_t units = a.rows * a.units;
   a.at_once = kWorkgroups<kD, kBf16, kW> * (uint32_t)compute_units;
-  // No more parts than the rows' blocks fill, at a part's least blocks.
+  // No more parts than the rows have blocks.
   const uint64_t capacity = (uint64_t)a.cache.width * a.cache.page_slots;
-  const uint64_t most_keys = a.window < capacity ? a.window : capacity;
-  const uint64_t blocks = most_keys / kBlockKeys + 2;
-  const uint64_t fill = units * ((blocks + kPartWaves - 1) / kPartWaves);
+  const uint64_t held = (capacity + kBlockKeys - 1) / kBlockKeys;
+  const uint64_t seen = (uint64_t)a.window / kBlockKeys + 2;
+  const uint64_t blocks = held < seen ? held : seen;
+  const uint64_t fill = units * blocks;
   const uint64_t bound = most_parts(units, a.at_once);
   hipLaunchKernelGGL((paged_attention_kernel<kD, kBf16, kW>),
                      dim3((uint32_t)(fill < bound ? fill : bound)), dim3(kThreads), 0, s, a);
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || blocks <= kPartWaves) return e;  // no row has two parts
+  if (e != hipSuccess || blocks == 1) return e;  // no row has two parts
   const uint32_t joins = most_joined_parts(units, a.at_once) / 2;
   const uint32_t records = units < joins ? units : joins;
   hipLaunchKernelGGL(paged_attention_join_kernel<kD>,

@@ -127,9 +127,9 @@ def test_every_block_in_one_part_within_the_grid(rules, lengths, window, capacit
     chunk, parts, most, joined, most_joined, covered = map(
         int, rules(window, capacity, head_blocks, at_once, *lengths))
     assert covered == 1
-    assert chunk % 4 == 0
+    assert chunk % 4 == 0 or chunk <= 2
     assert parts <= most
     # The workspace holds the parts of rows that have several.
     assert joined <= most_joined <= 2 * at_once
     if any(lengths):
-        assert chunk >= 4
+        assert chunk >= 1
