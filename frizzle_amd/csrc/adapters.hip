@@ -33,7 +33,6 @@ constexpr int kBlockRows = 32 * kUpWaves;    // outputs of a workgroup
 // many items: ones without an item would wait for a place, then for the tokens'
 // adapters, after all others.
 constexpr uint32_t kMostDown = 512, kMostUp = 768;
-constexpr int kRunTokens = 64;               // of a run of the up product
 constexpr int kTokenWaves = 8;
 constexpr uint32_t kTokenWorkgroups = 256;
 constexpr uint32_t kTokens = 64;
@@ -251,18 +250,18 @@ __global__ __launch_bounds__(64 * kDownWaves, 4) void adapter_down_kernel(Adapte
 }
 
 // base + s U times the low-rank rows, as the splits left them: a workgroup an
-// item (run of up to 64 tokens, 128 outputs), a wave two tiles of 16 outputs
-// by the run's four of 16 tokens. U is read once a run.
-template <int kFormat, int kTiles>
+// item (run of up to kRun tokens, 128 outputs), a wave two tiles of 16 outputs
+// by the run's tiles of 16 tokens. U is read once a run.
+template <int kFormat, int kTiles, int kRun>
 __global__ __launch_bounds__(64 * kUpWaves, 3) void adapter_up_kernel(AdapterArgs a) {
   constexpr int kChunks = (kTiles + 1) / 2;
   constexpr int kPitch = 32 * kChunks + 4;  // floats a token's row takes in LDS
-  constexpr int kRunTiles = kRunTokens / 16;
-  __shared__ __attribute__((aligned(16))) float low[kRunTokens][kPitch];
+  constexpr int kRunTiles = kRun / 16;
+  __shared__ __attribute__((aligned(16))) float low[kRun][kPitch];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int n = lane & 15, g = lane >> 4;
-  const Runs runs = find_runs<kRunTokens>(a, lane);
+  const Runs runs = find_runs<kRun>(a, lane);
   // As above, by eights of blocks: a block's runs meet on one die.
   const uint32_t blocks = (a.rows + kBlockRows - 1) / kBlockRows;
   const uint32_t places = blocks < 8 ? blocks : (blocks + 7) / 8 * 8;
@@ -292,7 +291,7 @@ __global__ __launch_bounds__(64 * kUpWaves, 3) void adapter_up_kernel(AdapterArg
     __syncthreads();  // the last item's rows are read
     // Four ranks a thread and piece, the splits of all its pieces asked for
     // together; ranks past the adapter's own, and tokens past the run, are zero.
-    constexpr int kPieces = kRunTokens * 8 * kChunks / (64 * kUpWaves);
+    constexpr int kPieces = kRun * 8 * kChunks / (64 * kUpWaves);
     f32x4 piece[kPieces];
     const float* src[kPieces];
 #pragma unroll
@@ -454,15 +453,24 @@ __global__ __launch_bounds__(64 * kTokenWaves, 2) void adapter_token_kernel(Adap
   }
 }
 
+template <int kFormat, int kTiles, int kRun>
+hipError_t launch_runs(hipStream_t s, const AdapterArgs& a, uint32_t blocks) {
+  // As many workgroups as items where every token is a run.
+  const uint64_t items = (uint64_t)a.tokens * (blocks < 8 ? blocks : (blocks + 7) / 8 * 8);
+  hipLaunchKernelGGL((adapter_up_kernel<kFormat, kTiles, kRun>),
+                     dim3((uint32_t)(items < kMostUp ? items : kMostUp)), dim3(64 * kUpWaves), 0, s,
+                     a);
+  return hipGetLastError();
+}
+
 template <int kFormat, int kTiles>
 hipError_t launch_up(hipStream_t s, const AdapterArgs& a) {
-  // As many workgroups as items where every token is a run.
+  // Runs of 64 tokens read U half as often as runs of 32; but a compute unit
+  // takes in about 40 GB/s, so shorter ones where the long ones' workgroups
+  // leave compute units idle.
   const uint32_t blocks = (a.rows + kBlockRows - 1) / kBlockRows;
-  const uint64_t items = (uint64_t)a.tokens * (blocks < 8 ? blocks : (blocks + 7) / 8 * 8);
-  hipLaunchKernelGGL((adapter_up_kernel<kFormat, kTiles>),
-                     dim3((uint32_t)(items < kMostUp ? items : kMostUp)),
-                     dim3(64 * kUpWaves), 0, s, a);
-  return hipGetLastError();
+  return (a.tokens + 63) / 64 * blocks < 256 ? launch_runs<kFormat, kTiles, 32>(s, a, blocks)
+                                             : launch_runs<kFormat, kTiles, 64>(s, a, blocks);
 }
 
 // Sets the splits.
