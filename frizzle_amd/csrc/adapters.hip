@@ -1,19 +1,22 @@
 // Low-rank adapters of a batch's tokens beside a shared projection:
 // y = base + s U (D x), each token with an adapter of its own.
 //
-// Tokens next to each other that share an adapter, up to 16 (or 64) within as
-// many aligned ones, are a run: an adapter's weights are read once a run, from
-// HBM once a launch. Work is counted in runs, which each wave finds for itself from the
-// tokens' adapters, so that a batch of one adapter and one of an adapter a
-// token both fill the chip.
+// A call that reads little goes by tokens: one launch on the vector units, each
+// token's workgroups forming D x for themselves. A large one goes by runs, in
+// two launches: tokens next to each other that share an adapter, up to 16, 32
+// or 64 within as many aligned ones, are a run, and an adapter's weights are
+// read once a run, from HBM once a launch. Work is counted in runs, which each
+// wave finds for itself from the tokens' adapters, so that a batch of one
+// adapter and one of an adapter a token both fill the chip.
 //
-// Both products run on the F32 matrix cores (v_mfma_f32_16x16x4_f32), weights
-// of any format widened exactly on the way: products and sums are F32, and
-// rounded nowhere else. The weights are the instruction's A operand, 16 rows
-// by 4 columns: lane (m, g) holds 8 columns of row m as they lie in memory,
-// and instruction j of 8 takes the j-th of each. Loads are a step ahead of the
-// products, and all of a step's loads are requested at once: a kernel is
-// compiled for 1, 2, 4 or 8 tiles of 16 ranks, so that no branch parts them.
+// The products of runs are on the F32 matrix cores (v_mfma_f32_16x16x4_f32),
+// weights of any format widened exactly on the way: products and sums are F32
+// in both forms, and rounded nowhere else. The weights are the instruction's A
+// operand, 16 rows by 4 columns: lane (m, g) holds 8 columns of row m as they
+// lie in memory, and instruction j of 8 takes the j-th of each. Loads are a
+// step ahead of the products, and all of a step's loads are requested at once:
+// the kernels are compiled for 1 or 2 (D) and 2, 4 or 8 (U) tiles of 16 ranks,
+// so that no branch parts them.
 
 #include "batch_rules.h"
 #include "kernels.h"
@@ -34,9 +37,8 @@ constexpr int kBlockRows = 32 * kUpWaves;    // outputs of a workgroup
 // adapters, after all others.
 constexpr uint32_t kMostDown = 512, kMostUp = 768;
 constexpr int kTokenWaves = 8;
-constexpr uint32_t kTokenWorkgroups = 256;
-constexpr uint32_t kTokens = 64;
-constexpr uint64_t kTokenBytes = 192 << 10;
+constexpr uint32_t kTokenWorkgroups = 256;    // that one launch by tokens is cut into, about
+constexpr uint64_t kTokenBytes = 128u << 20;  // the most that it reads: takes_tokens
 
 // Eight weights as they lie in memory, from element `at` (a multiple of 8).
 template <int kFormat>
@@ -360,47 +362,57 @@ __global__ __launch_bounds__(64 * kUpWaves, 3) void adapter_up_kernel(AdapterArg
 }
 
 // Both products of one token: a workgroup a (token, block of outputs), on the
-// vector units. All that it reads is asked for at once: a wave's rows of D,
-// a lane 8 columns of each 512, and a thread's outputs' rows of U. Each of a
+// vector units. All that it reads first is asked for at once: a wave's rows of
+// D, a lane 8 columns of each 512, and rows of U, kLanes lanes a row and 8
+// ranks a lane, so that a load is one contiguous piece (a row a lane had been
+// 64 lines a load: 20 to 23 us where this takes 13 to 18, rank 64, 1,152 to
+// 6,912, 64 tokens). Bound by latency at few tokens (two chains of loads and a
+// launch: 3 us of the call's 6) and by what a compute unit takes in, about
+// 40 GB/s, at more: 48 tokens of 41 adapters, BF16, rank 32, 1,152 to 6,912
+// (18.5 MB), 9.2 us a call. Each of a
 // token's workgroups forms all of D x for itself, from L2; numbered by eights
 // of tokens, they are on one die.
-template <int kFormat>
-__global__ __launch_bounds__(64 * kTokenWaves, 2) void adapter_token_kernel(AdapterArgs a) {
-  constexpr int kThreads = 64 * kTokenWaves;
-  __shared__ float low[kMostAdapterRank];
+template <int kFormat, int kLanes>
+__global__ __launch_bounds__(64 * kTokenWaves, kFormat == 0 ? 2 : 4)
+void adapter_token_kernel(AdapterArgs a) {
+  constexpr int kTurn = 64 * kTokenWaves / kLanes;  // outputs of a turn
+  constexpr int kDepth = kFormat == 0 ? 4 : 8;      // turns whose rows are under way at once
+  __shared__ __attribute__((aligned(16))) float low[8 * kLanes];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t places = a.tokens < 8 ? a.tokens : (a.tokens + 7) / 8 * 8;
   const uint32_t token = blockIdx.x % places;
   if (token >= a.tokens) return;
   const int from = blockIdx.x / places * a.block_rows, to = min(from + a.block_rows, a.rows);
-  if (from >= a.rows) return;
-  uint32_t adapter = a.which[token];
+  const uint32_t adapter = a.which[token];
   if (adapter >= a.count) {
     copy_base(a, token, 1, from, to, wave, kTokenWaves, lane);
     return;
   }
-  Run run{token, 1, adapter};
-  // The first 32 ranks of a thread's first outputs, which wait for nothing.
-  constexpr int kAhead = kFormat == 0 ? 1 : 2;
-  Raw<kFormat> u[kAhead][4];
-  auto load_up = [&](int o, int c, Raw<kFormat> (&to4)[4]) {
-    const uint64_t at =
-        ((uint64_t)adapter * a.rows + min(o, a.rows - 1)) * (uint64_t)a.rank + 32 * c;
+  const int o0 = from + (int)threadIdx.x / kLanes, slice = 8 * ((int)threadIdx.x % kLanes);
+  const int held = slice < a.rank ? slice : 0;  // a lane past the pool's rank repeats another
+  Raw<kFormat> u[kDepth];
+  float add[kDepth];
+  const float* base = a.base + (uint64_t)token * a.base_stride;
+  auto load_up = [&](int first) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (32 * c + 8 * i < a.rank) to4[i].load(a.up, at + 8 * i);
+    for (int i = 0; i < kDepth; ++i) {
+      if (first + i * kTurn >= to) continue;
+      const int o = min(o0 - from + first + i * kTurn, a.rows - 1);
+      u[i].load(a.up, ((uint64_t)adapter * a.rows + o) * (uint64_t)a.rank + held);
+      add[i] = base[o];
+    }
   };
-  const float* x = a.x + (uint64_t)token * a.x_stride;
-  const uint64_t pool = (uint64_t)adapter * a.rank * (uint64_t)a.cols;
-#pragma unroll
-  for (int i = 0; i < kAhead; ++i) load_up(from + (int)threadIdx.x + i * kThreads, 0, u[i]);
+  load_up(from);
+  const Run run{token, 1, adapter};
   const int rank = __builtin_amdgcn_readfirstlane(own_rank(a, run));
   const float scale = a.scales ? a.scales[adapter] : 1.0f;
-  // Four ranks a wave and turn, 1,024 columns at a time.
-  for (int r0 = 4 * wave; r0 < a.rank; r0 += 4 * kTokenWaves) {
+  const float* x = a.x + (uint64_t)token * a.x_stride;
+  const uint64_t pool = (uint64_t)adapter * a.rank * (uint64_t)a.cols;
+  // Four ranks a wave and turn, 1,536 columns at a time.
+  for (int r0 = 4 * wave; r0 < 8 * kLanes; r0 += 4 * kTokenWaves) {
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int k0 = 0; k0 < a.cols; k0 += 1536) {
+    for (int k0 = 0; r0 < a.rank && k0 < a.cols; k0 += 1536) {
       Raw<0> xs[3];
       Raw<kFormat> d[3][4];
 #pragma unroll
@@ -428,28 +440,26 @@ __global__ __launch_bounds__(64 * kTokenWaves, 2) void adapter_token_kernel(Adap
     }
   }
   __syncthreads();
-  const float* base = a.base + (uint64_t)token * a.base_stride;
+  float h[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) h[j] = low[slice + j];
   float* y = a.y + (uint64_t)token * a.y_stride;
-  for (int o = from + (int)threadIdx.x, turn = 0; o < to; o += kThreads, ++turn) {
-    float sum = 0.0f;
-    const float add = base[o];
-    for (int c = 0; 32 * c < rank; ++c) {
-      Raw<kFormat> v[4];
-      if (c == 0 && turn < kAhead) {
+  for (int first = from; first < to; first += kDepth * kTurn) {
+    if (first > from) load_up(first);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = kAhead == 2 && turn ? u[kAhead - 1][i] : u[0][i];
-      } else {
-        load_up(o, c, v);
-      }
+    for (int i = 0; i < kDepth; ++i) {
+      if (first + i * kTurn >= to) continue;
+      float sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int r = 32 * c + 8 * i + j;
-          if (r < rank) sum = fmaf_(v[i].at(j), low[r], sum);
-        }
+      for (int j = 0; j < 8; ++j)
+        sum = fmaf_(slice + j < rank ? u[i].at(j) : 0.0f, h[j], sum);
+      if constexpr (kLanes > 1) sum += __shfl_xor(sum, 1);
+      if constexpr (kLanes > 2) sum += __shfl_xor(sum, 2);
+      if constexpr (kLanes > 4) sum += __shfl_xor(sum, 4);
+      if constexpr (kLanes > 8) sum += __shfl_xor(sum, 8);
+      const int o = o0 - from + first + i * kTurn;
+      if (slice == 0 && o < to) y[o] = add[i] + sum;
     }
-    y[o] = add + sum;
   }
 }
 
@@ -491,21 +501,53 @@ hipError_t launch_down(hipStream_t s, AdapterArgs& a) {
   return hipGetLastError();
 }
 
+// A token's workgroups in adapter_token_kernel, each of so many whole turns of
+// outputs that all tokens' workgroups are there at once.
+struct TokenBlocks {
+  uint32_t rows, count;
+};
+TokenBlocks token_blocks(const AdapterArgs& a, uint32_t turn) {
+  const uint32_t turns = (a.rows + turn - 1) / turn;
+  const uint32_t wanted = a.tokens < kTokenWorkgroups ? kTokenWorkgroups / a.tokens : 1;
+  const uint32_t each = wanted < turns ? (turns + wanted - 1) / wanted : 1;
+  return {each * turn, (turns + each - 1) / each};
+}
+
+// Whether it takes a call: where what its workgroups read, each D whole and its
+// part of U, stays below kTokenBytes. Against two launches over runs, 16-bit
+// weights, tokens of one adapter and of an adapter each: rank 64, 1,152 to
+// 6,912, 32 tokens (61 MB) 9.8 and 12.4 us against 10.5 and 14.3, 64 (94 MB) 13.1
+// and 18.2 against 11.4 and 31.1, 128 (151 MB) 20.9 and 28.2 against 11.7 and 31.6;
+// rank 32, 6,912 to 1,152, 128 tokens (122 MB) 9.7 and 14.4 against 17.4 and
+// 33.5, 512 (264 MB) 21.3 and 44.1 against 16.0 and 22.2; rank 16, 1,152 to
+// 1,536, 1 to 256 tokens 7 to 8 against 10 to 12.
+template <int kFormat, int kLanes>
+bool takes_tokens(const AdapterArgs& a) {
+  const TokenBlocks b = token_blocks(a, 64 * kTokenWaves / kLanes);
+  const uint64_t weights = (uint64_t)a.rank * ((uint64_t)b.count * a.cols + a.rows);
+  return a.tokens * weights * (kFormat == 0 ? 4 : 2) <= kTokenBytes;
+}
+
+template <int kFormat, int kLanes>
+hipError_t launch_token(hipStream_t s, AdapterArgs a) {
+  const TokenBlocks b = token_blocks(a, 64 * kTokenWaves / kLanes);
+  a.block_rows = (int)b.rows;
+  const uint32_t places = a.tokens < 8 ? a.tokens : (a.tokens + 7) / 8 * 8;
+  hipLaunchKernelGGL((adapter_token_kernel<kFormat, kLanes>), dim3(places * b.count),
+                     dim3(64 * kTokenWaves), 0, s, a);
+  return hipGetLastError();
+}
+
 template <int kFormat>
 hipError_t launch_format(hipStream_t s, AdapterArgs a) {
-  const uint64_t weights = (uint64_t)a.rank * a.cols * (kFormat == 0 ? 4 : 2);
-  if (a.tokens <= kTokens && weights <= kTokenBytes) {
-    // Blocks of whole turns of a workgroup's threads, so many that the tokens'
-    // workgroups fill the chip.
-    const uint32_t turn = 64 * kTokenWaves;
-    const uint32_t turns = (a.rows + turn - 1) / turn;
-    const uint32_t wanted = (kTokenWorkgroups + a.tokens - 1) / a.tokens;
-    const uint32_t each = wanted < turns ? (turns + wanted - 1) / wanted : 1;
-    a.block_rows = (int)(each * turn);
-    const uint32_t places = a.tokens < 8 ? a.tokens : (a.tokens + 7) / 8 * 8;
-    hipLaunchKernelGGL(adapter_token_kernel<kFormat>, dim3(places * ((turns + each - 1) / each)),
-                       dim3(turn), 0, s, a);
-    return hipGetLastError();
+  if (a.rank <= 16) {
+    if (takes_tokens<kFormat, 2>(a)) return launch_token<kFormat, 2>(s, a);
+  } else if (a.rank <= 32) {
+    if (takes_tokens<kFormat, 4>(a)) return launch_token<kFormat, 4>(s, a);
+  } else if (a.rank <= 64) {
+    if (takes_tokens<kFormat, 8>(a)) return launch_token<kFormat, 8>(s, a);
+  } else if (takes_tokens<kFormat, 16>(a)) {
+    return launch_token<kFormat, 16>(s, a);
   }
   const hipError_t e = a.rank <= 16 ? launch_down<kFormat, 1>(s, a) : launch_down<kFormat, 2>(s, a);
   if (e != hipSuccess) return e;

@@ -273,17 +273,19 @@ def adapters_exact(pool, which, x, base):
     at most one 2^-24 an addition of its terms' absolute sum."""
     y = base.astype(np.float64)
     far = 2.0 ** -23 * abs(y)
-    for t, a in enumerate(which):
+    which = np.asarray(which)
+    for a in sorted(set(which.tolist())):
         r = pool.own(a) if a < pool.count else 0
         if r == 0:
             continue
+        rows = np.flatnonzero(which == a)
         d = of_format(pool.down[a, :r], pool.fmt)
         u = of_format(pool.up[a, :, :r], pool.fmt)
         s = 1.0 if pool.scales is None else float(pool.scales[a])
-        row = x[t].astype(np.float64)
-        y[t] += s * (u @ (d @ row))
-        size = abs(s) * (abs(u) @ (abs(d) @ abs(row)))
-        far[t] += size * (pool.cols + r + 8) * 2.0 ** -24 + 2.0 ** -23 * abs(y[t])
+        x64 = x[rows].astype(np.float64)
+        y[rows] += s * (x64 @ d.T @ u.T)
+        size = abs(s) * (abs(x64) @ abs(d).T @ abs(u).T)
+        far[rows] += size * (pool.cols + r + 8) * 2.0 ** -24 + 2.0 ** -23 * abs(y[rows])
     return y, far
 
 

@@ -7,8 +7,8 @@ import numpy as np
 import pytest
 
 import frizzle_amd as fz
-from _batch import (BF16, F16, F32, NONE, Paged, Pool, adapters, attention, attention_exact,
-                    check_adapters, of_format, rope, rope_exact)
+from _batch import (BF16, F16, F32, NONE, Paged, Pool, adapters, adapters_exact, attention_exact,
+                    check_adapters, of_format, rope_exact)
 from frizzle_amd import _lib
 from helpers import q4_blocks
 
@@ -55,6 +55,44 @@ def test_columns_at_the_splits(device, cols):
     check_adapters(device, pool, which, x, base)
 
 
+# Calls that read over 128 MB a token at a time go by runs of tokens with one
+# adapter, in two launches: each compiled number of ranks, both run lengths
+# (over 255 blocks of 128 outputs for 64 tokens at a time: 64), K in one split
+# and in many, the last of them short.
+@pytest.mark.parametrize("fmt,tokens,rank,cols,rows", [
+    (F16, 512, 16, 264, 8100), (BF16, 450, 24, 6912, 300), (F32, 512, 40, 264, 4300),
+    (BF16, 333, 64, 8200, 101), (F16, 512, 64, 40, 4500), (F16, 300, 128, 1152, 1901),
+    (F32, 200, 128, 8, 2600), (BF16, 512, 128, 1000, 5002)])
+@pytest.mark.parametrize("pattern", ["one", "requests", "mixed"])
+def test_runs_of_large_calls(device, fmt, tokens, rank, cols, rows, pattern):
+    size = 4 if fmt == F32 else 2
+    assert tokens * rank * (cols + rows) * size > 128 << 20
+    rng = np.random.default_rng(rank + cols)
+    pool = Pool(device, rng, 5, rank, cols, rows, fmt, ranks=[rank, 1, rank - 3, 0, 7],
+                scales=[1.0, -0.5, 2.0, 3.0, 0.25])
+    if pattern == "one":
+        which = [2] * tokens
+    elif pattern == "requests":
+        which = [(NONE, 0, 1, 2, 3, 4, 0)[i * 7 // tokens] for i in range(tokens)]
+    else:
+        which = [int(i) for i in rng.choice([0, 0, 1, 2, 4, 9], tokens)]
+    x, base = inputs(rng, tokens, pool)
+    check_adapters(device, pool, which, x, base)
+
+
+def test_runs_in_place_and_strided(device):
+    rng = np.random.default_rng(8)
+    pool = Pool(device, rng, 2, 64, 1152, 1538, F16, ranks=[64, 33])
+    assert 512 * 64 * (1152 + 1538) * 2 > 128 << 20
+    which = [0] * 100 + [1] * 200 + [NONE] * 70 + [0] * 142
+    x, base = inputs(rng, 512, pool)
+    plain = check_adapters(device, pool, which, x, base)[:, :1538]
+    wide = check_adapters(device, pool, which, x, base, x_width=1160, base_width=1544, y_width=1600)
+    assert np.array_equal(wide[:, :1538], plain)
+    there = check_adapters(device, pool, which, x, base, in_place=True)
+    assert np.array_equal(there[:, :1538], plain)
+
+
 def test_strides_in_place_and_rows_behind(device):
     rng = np.random.default_rng(3)
     pool = Pool(device, rng, 3, 16, 128, 98, F16, scales=[0.5, 1, 2])
@@ -83,25 +121,28 @@ def test_ranks_past_the_pool_and_an_empty_pool_entry(device):
     assert np.array_equal(got[1], base[1]) and np.array_equal(got[3], base[3])
 
 
-def test_a_token_that_is_no_number_stays_in_its_row(device):
+@pytest.mark.parametrize("tokens,rank,cols,rows", [(4, 16, 96, 50), (500, 64, 96, 2100)])
+def test_a_token_that_is_no_number_stays_in_its_row(device, tokens, rank, cols, rows):
     rng = np.random.default_rng(5)
-    pool = Pool(device, rng, 2, 16, 96, 50, F16, ranks=[13, 16])
-    which = [0, 0, 0, 1]
-    x, base = inputs(rng, 4, pool)
-    want, far = __import__("_batch").adapters_exact(pool, which, x, base)
-    x[1, 3], x[3, 95] = np.nan, np.inf
-    got = adapters(device, pool, which, x, base)[:, :50]
-    assert (abs(got[[0, 2]] - want[[0, 2]]) <= far[[0, 2]]).all()
-    assert np.isnan(got[1]).all() and not np.isfinite(got[3]).any()
+    pool = Pool(device, rng, 2, rank, cols, rows, F16, ranks=[13, rank])
+    which = [0] * (tokens - 1) + [1]
+    x, base = inputs(rng, tokens, pool)
+    want, far = adapters_exact(pool, which, x, base)
+    x[1, 3], x[-1, 95] = np.nan, np.inf
+    got = adapters(device, pool, which, x, base)[:, :rows]
+    sound = [0] + list(range(2, tokens - 1))
+    assert (abs(got[sound] - want[sound]) <= far[sound]).all()
+    assert np.isnan(got[1]).all() and not np.isfinite(got[-1]).any()
 
 
 def test_the_same_bits_every_time_and_from_threads(device):
     rng = np.random.default_rng(6)
     sets = []
-    for rank, cols, rows, fmt in ((16, 1152, 1536, F16), (64, 512, 96, BF16)):
+    # One launch, and two over runs.
+    for rank, cols, rows, fmt, tokens in ((16, 1152, 1536, F16, 70), (128, 2504, 1500, BF16, 200)):
         pool = Pool(device, rng, 4, rank, cols, rows, fmt)
-        which = [int(i) for i in rng.integers(0, 5, 70)]
-        x, base = inputs(rng, 70, pool)
+        which = [int(i) for i in rng.integers(0, 5, tokens)]
+        x, base = inputs(rng, tokens, pool)
         sets.append((pool, which, x, base))
     want = [adapters(device, *s) for s in sets]
     bad = []
@@ -179,7 +220,6 @@ def test_a_batch_of_requests_steps_through_a_layer(device):
                                        n, done.ptr, n, rows))
         device.sync()
         # Q/K/V from the shared product on, each op from what the one before left.
-        from _batch import adapters_exact
         full, _ = adapters_exact(pools["qkv"], which, x, product.numpy())
         got = qkv.numpy()
         keys, values, _ = paged.read()
