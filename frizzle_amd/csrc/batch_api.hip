@@ -23,6 +23,7 @@ constexpr size_t kAdapterBytes =
 constexpr size_t kScratchBytes = kAttentionBytes > kAdapterBytes ? kAttentionBytes : kAdapterBytes;
 
 constexpr int kMostHeads = 1024;
+constexpr float kMostScale = 4096.0f;  // 2^13 in log2 units, as the kernel takes
 
 bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 bool aligned_word(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
@@ -142,6 +143,7 @@ int frz_op_rope_paged(frz_device* dev, const frz_pages* cache, const uint32_t* s
   const int64_t kv = (int64_t)cache->kv_heads * cache->head_dim;
   if (!stride_ok(q_stride, q) || !stride_ok(kv_stride, kv) || !stride_ok(roped_stride, q))
     return refuse(what, "strides (multiples of 4, at least a row)");
+  if (roped == key || roped == value) return refuse(what, "roped is key or value");
   if (roped == query && roped_stride != q_stride)
     return refuse(what, "roped in place with another stride");
   PagedRopeArgs a;
@@ -179,7 +181,7 @@ int frz_op_attention_paged(frz_device* dev, const frz_pages* cache, const uint32
     return refuse(what, "strides (multiples of 4, at least a row)");
   if (out == query) return refuse(what, "out is query");
   if (window == 0) return refuse(what, "window 0");
-  if (!std::isfinite(scale)) return refuse(what, "scale is no number");
+  if (!(std::fabs(scale) <= kMostScale)) return refuse(what, "scale (a number of at most 4,096)");
   PagedAttentionArgs a;
   a.cache = cache_of(cache);
   a.sequences = sequences;
@@ -224,6 +226,7 @@ int frz_op_adapters(frz_device* dev, const frz_adapters* adapters, const uint32_
   if (!stride_ok(x_stride, p.cols) || !stride_ok(base_stride, p.rows) ||
       !stride_ok(y_stride, p.rows))
     return refuse(what, "strides (multiples of 4, at least a row)");
+  if (x == y) return refuse(what, "y is x");
   if (base == y && base_stride != y_stride)
     return refuse(what, "y is base with another stride");
   AdapterArgs a;

@@ -24,9 +24,11 @@
 // (to 2^-22) or three of BF16 (2^-24), which are further columns of the same
 // instruction where the heads leave some free: columns n and n + W belong to
 // one head, W the next of 4, 8 or 16 above the heads. A head's query is
-// scaled by a power of two to lie below 2^15, weights by 2^14, so that their
-// low parts stay clear of the formats' smallest values; both scales are
-// exact. Products are exact in F32, sums F32.
+// scaled by a power of two, for F16 to lie below 2^15, and weights by 2^14, so
+// that their low parts stay clear of the format's smallest values; for BF16,
+// whose range is F32's, the query lies below 2 and weights are at most 1, so
+// that large keys' and values' products stay in range. Both scales are exact,
+// products are exact in F32, sums F32.
 //
 // Keys outside the row's range or in no page are never read: their rows are
 // zeros, and their scores -inf.
@@ -45,7 +47,6 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 64 * kPartWaves;
-constexpr float kWeightScale = 14.0f;  // weights are 2^14 at the running maximum
 constexpr float kMinusInf = -__builtin_inff();
 constexpr int kBufferWord3 = 0x00020000;  // raw 32-bit data
 
@@ -56,6 +57,8 @@ struct Types<false> {
   typedef half8 vec;
   typedef _Float16 scalar;
   static constexpr int kParts = 2;
+  static constexpr int kQueryTop = 14;          // the query's largest lies in [2^14, 2^15)
+  static constexpr float kWeightScale = 14.0f;  // weights are 2^14 at the running maximum
   static __device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a),
                                                   __builtin_bit_cast(half8, b), c, 0, 0, 0);
@@ -66,6 +69,8 @@ struct Types<true> {
   typedef bf16x8 vec;
   typedef __bf16 scalar;
   static constexpr int kParts = 3;
+  static constexpr int kQueryTop = 0;
+  static constexpr float kWeightScale = 0.0f;
   static __device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -393,7 +398,7 @@ __global__ __launch_bounds__(kThreads, (kWorkgroups<kD, kBf16, kW>)) void paged_
   for (int s = 0; s < S::kSpans; ++s)
 #pragma unroll
     for (int j = 0; j < S::kVec; ++j) out[s][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  float m = kMinusInf, l = 0.0f;  // m less kWeightScale, once there is a key
+  float m = kMinusInf, l = 0.0f;  // m less T::kWeightScale, once there is a key
 
   uint32_t turn = 0;
   Block now, next;
@@ -424,10 +429,11 @@ __global__ __launch_bounds__(kThreads, (kWorkgroups<kD, kBf16, kW>)) void paged_
 #pragma unroll
         for (int i = 0; i < 8; ++i) most = __builtin_fmaxf(most, __builtin_fabsf(x[c][i]));
       most = across_groups(most, [](float p, float r) { return __builtin_fmaxf(p, r); });
-      // 2^up takes the largest to [2^14, 2^15); zeros, infinities and the
-      // smallest values as far as both factors stay ordinary numbers.
-      int up = 141 - (int)(float_to_bits(most) >> 23);
-      up = up > 100 ? 100 : up < -100 ? -100 : up;
+      // 2^up takes the largest to its place; zeros and the smallest (and for
+      // BF16 the largest) values as far as both factors, and the scale with its
+      // own (at most 2^13), stay ordinary numbers.
+      int up = 127 + T::kQueryTop - (int)(float_to_bits(most) >> 23);
+      up = up > 100 ? 100 : up < -113 ? -113 : up;
       const float factor = bits_to_float((uint32_t)(127 + up) << 23);
       scale = a.scale_log2e * bits_to_float((uint32_t)(127 - up) << 23);
 #pragma unroll
@@ -475,7 +481,7 @@ __global__ __launch_bounds__(kThreads, (kWorkgroups<kD, kBf16, kW>)) void paged_
       most = across_groups(most, [](float p, float r) { return __builtin_fmaxf(p, r); });
       // A block that is worked on holds a key, so `most` is a number but where
       // scores are not.
-      const float to = __builtin_fmaxf(m, most - kWeightScale);
+      const float to = __builtin_fmaxf(m, most - T::kWeightScale);
       if (__ballot(to > m)) {
         const float old = __builtin_amdgcn_exp2f(m - to);
         l *= old;

@@ -250,7 +250,8 @@ typedef struct frz_pages {
  * pages: frz_op_rope's arithmetic, bit for bit, at positions of the rows'
  * own. query_heads is a multiple of kv_heads, at most 1,024. Rows of query
  * are q_stride, of key and value kv_stride floats apart; the roped queries go
- * to roped (roped_stride apart), which may be query itself, with its stride.
+ * to roped (roped_stride apart), which may be query itself, with its stride,
+ * and overlaps nothing else.
  * Keys and values round to the cache's format, to nearest even (F16
  * saturates at 65,504). Of rows at one request's position the last one's
  * stay; two requests must not append to a page that they share. */
@@ -261,11 +262,12 @@ int frz_op_rope_paged(frz_device* dev, const frz_pages* cache, const uint32_t* s
                       int roped_stride, int query_heads, float epsilon, uint32_t rows);
 /* Each row's attention over the keys of its request at (position - window,
  * position], its own among them (window at least 1; 0xFFFFFFFF: all): query
- * head i reads key-value head i / (query_heads / kv_heads). Within about
- * 1e-6 of the exact sums, not the reference's order. A row with no key gets
- * zeros. Cached values must be finite where a row reads them, and may be
- * anything elsewhere. out's rows are out_stride floats apart; out must not
- * overlap query. */
+ * head i reads key-value head i / (query_heads / kv_heads). Scores are scale
+ * (at most 4,096 either side of zero) times the products. Within about 1e-6 of
+ * the exact sums, not the reference's order, where products and sums of values
+ * stay in F32's range. A row with no key gets zeros. Cached values must be
+ * finite where a row reads them, and may be anything elsewhere. out's rows are
+ * out_stride floats apart; out must not overlap query. */
 int frz_op_attention_paged(frz_device* dev, const frz_pages* cache, const uint32_t* sequences,
                            const uint32_t* positions, const float* query, int q_stride,
                            float* out, int out_stride, int query_heads, uint32_t window,

@@ -77,7 +77,8 @@ def test_caches_refused(changed, text):
     (dict(out_stride=-1024), "strides"), (dict(out_stride=0), "strides"), (dict(out=P), "query"),
     (dict(heads=0), "heads"), (dict(heads=-4), "heads"), (dict(heads=1025), "heads"),
     (dict(window=0), "window"), (dict(scale=float("nan")), "scale"),
-    (dict(scale=float("inf")), "scale"), (dict(rows=0), "rows"), (dict(rows=513), "rows"),
+    (dict(scale=float("inf")), "scale"), (dict(scale=4097.0), "scale"),
+    (dict(scale=-1e30), "scale"), (dict(rows=0), "rows"), (dict(rows=513), "rows"),
     (dict(rows=NONE), "rows"),
 ])
 def test_attention_refused(more, text):
@@ -91,7 +92,8 @@ def test_attention_refused(more, text):
     (dict(turns=P + 4), "16 bytes"), (dict(key=P + 4), "16 bytes"), (dict(value=P + 8), "16 bytes"),
     (dict(positions=P + 3), "16 bytes"), (dict(q_stride=1000), "strides"),
     (dict(kv_stride=252), "strides"), (dict(kv_stride=258), "strides"),
-    (dict(roped_stride=1023), "strides"), (dict(roped=P, roped_stride=2048), "in place"),
+    (dict(roped_stride=1023), "strides"), (dict(query=3 * P, roped=3 * P, roped_stride=2048), "in place"),
+    (dict(key=3 * P, roped=3 * P), "key or value"), (dict(value=3 * P, roped=3 * P), "key or value"),
     (dict(heads=5000), "heads"), (dict(rows=0), "rows"), (dict(rows=513), "rows"),
 ])
 def test_rope_refused(more, text):
@@ -118,7 +120,8 @@ def test_null_structures_refused():
     (dict(base=P + 8), "16 bytes"), (dict(y=P + 12), "16 bytes"), (dict(x_stride=60), "strides"),
     (dict(x_stride=66), "strides"), (dict(base_stride=96), "strides"),
     (dict(y_stride=99), "strides"), (dict(y_stride=-100), "strides"),
-    (dict(y=P, y_stride=104), "another stride"),
+    (dict(x=3 * P, y=P, y_stride=104), "another stride"),
+    (dict(x=3 * P, y=3 * P), "y is x"),
 ])
 def test_adapters_refused(more, text):
     refused(adapters(**more), text)

@@ -5,7 +5,8 @@ import threading
 import numpy as np
 import pytest
 
-from _batch import (BF16, F16, NONE, Paged, attention, attention_exact, check_attention, to_format)
+from _batch import (BF16, F16, NONE, Paged, attention, attention_exact, check_attention, of_format,
+                    to_format)
 
 pytestmark = pytest.mark.gpu
 
@@ -129,6 +130,19 @@ def test_queries_and_keys_of_any_size(device, fmt, query_scale, key_scale):
     paged, query, positions = batch(device, 15, [150, 33, 1], 4, 1, 256, 16, fmt, scale=key_scale)
     query = (query * query_scale).astype(np.float32)
     check_attention(device, paged, positions, query, 4, NONE, 1 / 16)
+
+
+@pytest.mark.parametrize("fmt,query_scale,key_scale,value_scale", [
+    (F16, 1e36, 1e-4, 1.0), (F16, 1.0, 1.0, 1e4), (BF16, 1e36, 1e-25, 1e25),
+    (BF16, 1e-30, 1e30, 1.0), (BF16, 1.0, 1.0, 1e34), (BF16, 1.0, 1e36, 1e-6)])
+def test_values_near_the_ends_of_the_range(device, fmt, query_scale, key_scale, value_scale):
+    # Largest queries, keys and values whose products and sums F32 still holds.
+    paged, query, positions = batch(device, 20, [150, 33, 1], 4, 1, 256, 16, fmt, scale=key_scale)
+    query = (query * query_scale).astype(np.float32)
+    paged.values[:] = to_format(of_format(paged.values, fmt) * value_scale, fmt)
+    paged.upload()
+    check_attention(device, paged, positions, query, 4, NONE,
+                    1 / (16 * max(1.0, query_scale * key_scale)))
 
 
 def test_negative_and_zero_scale(device):
