@@ -215,8 +215,9 @@ __device__ __forceinline__ void low_rank(const AdapterArgs& a, const Run& run, i
 }
 
 // The low-rank rows of each run: a workgroup an item (run, ranks of kTiles
-// tiles, split of K). Workgroups go round the eight dies: numbered by eights
-// of runs, a run's meet on one die, whose L2 then holds its rows of x alone.
+// tiles, split of K). Workgroups go round the eight dies, and a split stays on
+// as few of them as there are: each die's L2 then takes in its own columns of
+// x and D alone (D on every die had been most of what the dies read).
 template <int kFormat, int kTiles>
 __global__ __launch_bounds__(64 * kDownWaves, 4) void adapter_down_kernel(AdapterArgs a) {
   __shared__ f32x4 sums[kDownWaves][kTiles][64];
@@ -224,14 +225,18 @@ __global__ __launch_bounds__(64 * kDownWaves, 4) void adapter_down_kernel(Adapte
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int n = lane & 15, g = lane >> 4;
   const Runs runs = find_runs<16>(a, lane);
-  const uint32_t places = runs.count < 8 ? runs.count : (runs.count + 7) / 8 * 8;
   const uint32_t groups = (a.rank + 16 * kTiles - 1) / (16 * kTiles);
-  const uint32_t items = places * groups * a.splits;
+  // Splits are a power of two: `beside` of them go round the dies together,
+  // with as many runs as the dies then have room for.
+  const uint32_t splits = a.splits, beside = min(splits, 8u), rows = 8 / beside;
+  const uint32_t items = (runs.count + rows - 1) / rows * rows * groups * splits;
   for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
-    if (item % places >= runs.count) continue;
-    const Run run = run_at(a, runs, item % places);
+    const uint32_t die = item % 8, piece = item / 8, later = piece / groups;
+    const uint32_t split = die % beside + later % (splits / beside) * 8;
+    const uint32_t want = later / (splits / beside) * rows + die / beside;
+    if (want >= runs.count) continue;
+    const Run run = run_at(a, runs, want);
     if (run.adapter == kNone) continue;
-    const uint32_t piece = item / places, split = piece / groups;
     const int rank0 = piece % groups * 16 * kTiles;
     const int from = split * a.split_cols, to = min(from + a.split_cols, a.cols);
     f32x4 acc[kTiles];
@@ -486,15 +491,18 @@ hipError_t launch_up(hipStream_t s, const AdapterArgs& a) {
 // Sets the splits.
 template <int kFormat, int kTiles>
 hipError_t launch_down(hipStream_t s, AdapterArgs& a) {
-  // Splits of whole turns of a workgroup's waves, so many that the runs'
-  // workgroups fill the chip.
+  // So many splits that the runs' workgroups fill the chip, a power of two, of
+  // whole steps of a wave and not below a turn of a workgroup's waves; the last
+  // may be short, or have no columns.
   const uint32_t groups = (a.rank + 16 * kTiles - 1) / (16 * kTiles);
-  uint32_t splits = 256 / ((a.tokens + 15) / 16 * groups);
-  splits = splits < 1 ? 1 : splits > kMostAdapterSplits ? kMostAdapterSplits : splits;
-  const int turns = (a.cols + kTurnCols - 1) / kTurnCols;
-  a.split_cols = kTurnCols * ((turns + (int)splits - 1) / (int)splits);
-  a.splits = (a.cols + a.split_cols - 1) / a.split_cols;
-  const uint64_t items = (uint64_t)((a.tokens + 7) / 8 * 8) * groups * a.splits;
+  const uint32_t wanted = 256 / ((a.tokens + 15) / 16 * groups);
+  uint32_t splits = 1;
+  while (2 * splits <= wanted && 2 * splits <= kMostAdapterSplits &&
+         2 * splits * kTurnCols <= (uint32_t)a.cols)
+    splits *= 2;
+  a.split_cols = 32 * (((a.cols + 31) / 32 + (int)splits - 1) / (int)splits);
+  a.splits = (int)splits;
+  const uint64_t items = (uint64_t)((a.tokens + 7) / 8 * 8) * groups * splits;
   hipLaunchKernelGGL((adapter_down_kernel<kFormat, kTiles>),
                      dim3((uint32_t)(items < kMostDown ? items : kMostDown)),
                      dim3(64 * kDownWaves), 0, s, a);
