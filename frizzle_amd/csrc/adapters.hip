@@ -9,14 +9,18 @@
 // wave finds for itself from the tokens' adapters, so that a batch of one
 // adapter and one of an adapter a token both fill the chip.
 //
-// The products of runs are on the F32 matrix cores (v_mfma_f32_16x16x4_f32),
-// weights of any format widened exactly on the way: products and sums are F32
-// in both forms, and rounded nowhere else. The weights are the instruction's A
-// operand, 16 rows by 4 columns: lane (m, g) holds 8 columns of row m as they
-// lie in memory, and instruction j of 8 takes the j-th of each. Loads are a
-// step ahead of the products, and all of a step's loads are requested at once:
-// the kernels are compiled for 1 or 2 (D) and 2, 4 or 8 (U) tiles of 16 ranks,
-// so that no branch parts them.
+// The products of runs are on the matrix cores, D's in F32
+// (v_mfma_f32_16x16x4_f32), weights of any format widened exactly on the way,
+// U's mostly of parts of BF16 that add up to the weights (kUpInParts). Sums are
+// F32 in both forms, and nothing is rounded to less. The weights are the
+// instruction's A operand, 16 rows of as many columns as it takes: lane (m, g)
+// holds 8 columns of row m as they lie in memory, and of F32's eight
+// instructions the j-th takes the j-th of each. Loads are a step ahead of the
+// products, and all of a step's loads are requested at once: the kernels are
+// compiled for 1 or 2 (D) and 2, 4 or 8 (U) tiles of 16 ranks, so that no
+// branch parts them.
+
+#include <type_traits>
 
 #include "batch_rules.h"
 #include "kernels.h"
@@ -60,6 +64,26 @@ struct Raw {
     return bits_to_float(i & 1 ? w & 0xFFFF0000u : w << 16);
   }
 };
+
+// F32 values as parts of BF16 that add up to them (three hold 24 bits; their
+// exponents are F32's), each what rounding left to the parts before.
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+template <int kParts>
+__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&part)[kParts]) {
+  float rest[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) rest[j] = x[j];
+#pragma unroll
+  for (int p = 0; p < kParts; ++p)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      part[p][j] = (__bf16)rest[j];
+      if (p + 1 < kParts) rest[j] -= (float)part[p][j];
+    }
+}
+// Parts that hold a format's weights exactly: F16's 11 bits take two.
+template <int kFormat>
+constexpr int kWeightParts = kFormat == 0 ? 3 : kFormat == 1 ? 2 : 1;
 
 struct Run {
   uint32_t first, tokens;
@@ -256,15 +280,32 @@ __global__ __launch_bounds__(64 * kDownWaves, 4) void adapter_down_kernel(Adapte
   }
 }
 
+// Whether the up products are of BF16 parts on the 16-bit matrix cores, 3, 5 or
+// 6 instructions of 16 cycles for 32 ranks where F32's eight take 256. What it
+// costs is the parts of U, some 150 cycles for 8 weights a lane of F16 or F32,
+// which a run's tiles of tokens share: rank 128, 1,152 to 6,912, 512 tokens of
+// one adapter, the call 24.0 -> 20.6 us in F16 and 24.5 -> 23 in F32 (440 ->
+// 467 of an F32 adapter each); not for F32 in runs of 32: rank 128, 6,912 to
+// 1,152, 200 tokens, 22.6 -> 24.3 us.
+template <int kFormat, int kRun>
+constexpr bool kUpInParts = kFormat != 0 || kRun == 64;
+
 // base + s U times the low-rank rows, as the splits left them: a workgroup an
 // item (run of up to kRun tokens, 128 outputs), a wave two tiles of 16 outputs
-// by the run's tiles of 16 tokens. U is read once a run.
+// by the run's tiles of 16 tokens. U is read once a run. The low-rank rows lie
+// in LDS as the matrix instructions take them, as three parts of BF16 or F32.
 template <int kFormat, int kTiles, int kRun>
 __global__ __launch_bounds__(64 * kUpWaves, 3) void adapter_up_kernel(AdapterArgs a) {
   constexpr int kChunks = (kTiles + 1) / 2;
-  constexpr int kPitch = 32 * kChunks + 4;  // floats a token's row takes in LDS
   constexpr int kRunTiles = kRun / 16;
-  __shared__ __attribute__((aligned(16))) float low[kRun][kPitch];
+  constexpr bool kInParts = kUpInParts<kFormat, kRun>;
+  constexpr int kWeights = kInParts ? kWeightParts<kFormat> : 1;
+  typedef typename std::conditional<kInParts, __bf16, float>::type Low;
+  typedef Low Low4 __attribute__((ext_vector_type(4)));
+  constexpr int kLowParts = kInParts ? 3 : 1;
+  // Values that a token's row takes in LDS: 16 bytes past a multiple of 64.
+  constexpr int kPitch = 32 * kChunks + 16 / sizeof(Low);
+  __shared__ __attribute__((aligned(16))) Low low[kLowParts][kRun][kPitch];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int n = lane & 15, g = lane >> 4;
@@ -318,10 +359,19 @@ __global__ __launch_bounds__(64 * kUpWaves, 3) void adapter_up_kernel(AdapterArg
     for (int i = 0; i < kPieces; ++i) {
       const int at = threadIdx.x + i * 64 * kUpWaves;
       const int t = at / (8 * kChunks), r = at % (8 * kChunks) * 4;
-      f32x4 row;
+      float rest[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) row[e] = r + e < rank ? piece[i][e] * scale : 0.0f;
-      *reinterpret_cast<f32x4*>(&low[t][r]) = row;
+      for (int e = 0; e < 4; ++e) rest[e] = r + e < rank ? piece[i][e] * scale : 0.0f;
+#pragma unroll
+      for (int p = 0; p < kLowParts; ++p) {
+        Low4 part;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          part[e] = (Low)rest[e];
+          rest[e] -= (float)part[e];
+        }
+        *reinterpret_cast<Low4*>(&low[p][t][r]) = part;
+      }
     }
     __syncthreads();
     // Lane (n, g): outputs 4 g .. + 3 of each tile, of token n of each 16.
@@ -341,18 +391,44 @@ __global__ __launch_bounds__(64 * kUpWaves, 3) void adapter_up_kernel(AdapterArg
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
       if (c + 1 < kChunks) load(c + 1, w[(c + 1) & 1]);
+      float weight[2][8];
+      bf16x8 part[2][kWeights];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          weight[i][j] = 32 * c + 8 * g + j < rank ? w[c & 1][i].at(j) : 0.0f;
+        if constexpr (kInParts) split8<kWeights>(weight[i], part[i]);
+      }
 #pragma unroll
       for (int t = 0; t < kRunTiles; ++t) {
         if (t >= run_tiles) break;
-        const f32x4 h0 = *reinterpret_cast<const f32x4*>(&low[16 * t + n][32 * c + 8 * g]);
-        const f32x4 h1 = *reinterpret_cast<const f32x4*>(&low[16 * t + n][32 * c + 8 * g + 4]);
+        const int at = 32 * c + 8 * g;
+        if constexpr (kInParts) {
+          // The products of parts down to 2^-16 of the largest: what is left
+          // out is as small as F32's rounding.
+          bf16x8 h[3];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+          for (int p = 0; p < 3; ++p)
+            h[p] = *reinterpret_cast<const bf16x8*>(&low[p][16 * t + n][at]);
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-            acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                32 * c + 8 * g + j < rank ? w[c & 1][i].at(j) : 0.0f, j < 4 ? h0[j & 3] : h1[j & 3],
-                acc[i][t], 0, 0, 0);
+          for (int q = kWeights - 1; q >= 0; --q)
+#pragma unroll
+            for (int p = 2 - q; p >= 0; --p)
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+                acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(part[i][q], h[p], acc[i][t], 0,
+                                                                    0, 0);
+        } else {
+          const f32x4 h0 = *reinterpret_cast<const f32x4*>(&low[0][16 * t + n][at]);
+          const f32x4 h1 = *reinterpret_cast<const f32x4*>(&low[0][16 * t + n][at + 4]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                  weight[i][j], j < 4 ? h0[j & 3] : h1[j & 3], acc[i][t], 0, 0, 0);
+        }
       }
     }
 #pragma unroll
