@@ -15,7 +15,8 @@ from .runtime import (CAPTURE_SLOTS, PREFILL_BF16, PREFILL_EXACT, Q4_0, Q4_1, Q8
                       tensor_bytes)
 
 __all__ = [
-    "Adapters", "FrzError", "Pages", "exported_symbols", "load", "CAPTURE_SLOTS", "PREFILL_BF16", "PREFILL_EXACT",
+    "Adapters", "FrzError", "Pages", "exported_symbols", "load",
+    "CAPTURE_SLOTS", "PREFILL_BF16", "PREFILL_EXACT",
     "Q4_0", "Q4_1", "Q8_0",
     "capture_layout", "capture_words",
     "TO_THE_END", "Device", "block_split",

@@ -89,8 +89,8 @@ const char* refuse_pages(const frz_pages* c, int query_heads, uint32_t rows) {
   if (c->page_stride % 8 ||
       c->page_stride < (uint64_t)c->page_slots * c->kv_heads * c->head_dim)
     return "page_stride (a multiple of 8, at least a page)";
-  // Addresses are 64 bits; a page's byte offset stays below 2^63.
-  if (c->page_stride > (1ull << 40)) return "page_stride (at most 2^40)";
+  // Their product is an offset in 64 bits.
+  if (c->page_stride > (1ull << 48) / c->pages) return "page_stride (a pool of at most 2^48 values)";
   if (rows < 1 || rows > rules::kMostRows) return "rows (1 to 512)";
   return nullptr;
 }

@@ -218,9 +218,10 @@ int frz_op_draw(frz_device* dev, const uint32_t* candidates_dev,
  * most 512, row r one token of the request sequences[r] (null: request r) at
  * positions[r]; a row at FRZ_NO_POSITION is none, and its outputs are left as
  * they are. These calls enqueue and return, in order on the device's stream;
- * frz_sync waits. They may be made from several threads, and with any device
- * current. Pointers to floats or 16-bit values must be multiples of 16 bytes
- * and strides of 4 floats. */
+ * frz_sync waits. They may be made from several threads at once, though not
+ * while one of the device's models is made or runs in another (it captures
+ * its steps on the stream), and with any device current. Pointers to floats
+ * or 16-bit values must be multiples of 16 bytes and strides of 4 floats. */
 #define FRZ_FORMAT_F16 1
 #define FRZ_FORMAT_BF16 30
 #define FRZ_NO_POSITION 0xFFFFFFFFu
@@ -241,7 +242,8 @@ typedef struct frz_pages {
   int head_dim;           /* 64, 128 or 256 */
   uint32_t page_slots;    /* a multiple of 16 */
   uint32_t pages;         /* pages in the pool */
-  uint64_t page_stride;   /* values from a page to the next, a multiple of 8 */
+  uint64_t page_stride;   /* values from a page to the next, a multiple of 8;
+                           * pages * page_stride at most 2^48 */
   const uint32_t* table;  /* dev: sequences rows of width entries */
   uint32_t sequences;
   uint32_t width;         /* width * page_slots at most 2^24 */

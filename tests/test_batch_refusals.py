@@ -60,6 +60,7 @@ CACHES = [
     (dict(width=0), "width"), (dict(width=(1 << 20) + 1), "width"), (dict(width=NONE), "width"),
     (dict(page_stride=16 * 256 - 8), "page_stride"), (dict(page_stride=16 * 256 + 4), "page_stride"),
     (dict(page_stride=0), "page_stride"), (dict(page_stride=1 << 60), "page_stride"),
+    (dict(page_stride=1 << 40, pages=(1 << 8) + 1), "page_stride"),
 ]
 
 

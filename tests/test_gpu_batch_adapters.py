@@ -8,7 +8,7 @@ import pytest
 
 import frizzle_amd as fz
 from _batch import (BF16, F16, F32, NONE, Paged, Pool, adapters, adapters_exact, attention_exact,
-                    check_adapters, of_format, rope_exact)
+                    check_adapters, of_format, rope_exact, to_format)
 from frizzle_amd import _lib
 from helpers import q4_blocks
 
@@ -158,6 +158,34 @@ def test_the_same_bits_every_time_and_from_threads(device):
     for t in threads:
         t.join()
     assert not bad
+
+
+@pytest.mark.parametrize("tokens", [3, 300])
+def test_a_pool_past_32_bits(device, tokens):
+    # Down matrices of 2^23 values: the last adapter's lie past 2^32 of them.
+    rng = np.random.default_rng(7)
+    count, rank, cols, rows = 514, 128, 1 << 16, 24
+    big = fz.runtime.DeviceArray(device, 2 * count * rank * cols, np.uint8, (1,))
+    down = to_format(rng.normal(0, cols ** -0.5, (rank, cols)), F16)
+    up = np.full((count, rows, rank), 0x7E00, np.uint16)  # NaN
+    up[513] = to_format(rng.normal(0, rank ** -0.5, (rows, rank)), F16)
+    _lib.check(fz.load().frz_write(device.handle, big.ptr + 2 * 513 * rank * cols,
+                                   down.ctypes.data, down.nbytes))
+    dev_up, which = device.array(up), device.array(np.full(tokens, 513, np.uint32))
+    x = rng.normal(0, 1, (tokens, cols)).astype(np.float32)
+    base = rng.normal(0, 1, (tokens, rows)).astype(np.float32)
+    dx, db = device.array(x), device.array(base)
+    p = fz.Adapters(F16, count, rank, cols, rows, big.ptr, dev_up.ptr, None, None)
+    _lib.check(fz.load().frz_op_adapters(device.handle, p, which.ptr, dx.ptr, cols, db.ptr, rows,
+                                         db.ptr, rows, tokens))
+    device.sync()
+    got = db.numpy()
+    big.free()
+    d, u = of_format(down, F16), of_format(up[513], F16)
+    want = base + x.astype(np.float64) @ d.T @ u.T
+    far = (abs(x).astype(np.float64) @ abs(d).T @ abs(u).T) * (cols + rank + 8) * 2.0 ** -24
+    assert (abs(got - want) <= far + 2.0 ** -22 * abs(want)).all()
+    assert np.linalg.norm(got - want) <= 3e-6 * np.linalg.norm(want)
 
 
 # ---- together ------------------------------------------------------------------

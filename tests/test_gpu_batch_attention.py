@@ -58,6 +58,12 @@ def test_rows_of_several_parts(device, lengths, heads, kv, dim, slots, fmt):
     check_attention(device, paged, positions, query, heads, NONE, dim ** -0.5)
 
 
+@pytest.mark.parametrize("heads,kv", [(1024, 1024), (1024, 2), (1024, 1), (1008, 63)])
+def test_the_most_heads(device, heads, kv):
+    paged, query, positions = batch(device, heads + kv, [33, 0, 150, 1, 18], heads, kv, 64, 16, F16)
+    check_attention(device, paged, positions, query, heads, 100, 0.125)
+
+
 def test_the_most_rows(device):
     rng = np.random.default_rng(5)
     lengths = [int(n) for n in rng.integers(0, 90, 512)]
