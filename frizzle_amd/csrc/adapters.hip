@@ -241,7 +241,10 @@ __device__ __forceinline__ void low_rank(const AdapterArgs& a, const Run& run, i
 // The low-rank rows of each run: a workgroup an item (run, ranks of kTiles
 // tiles, split of K). Workgroups go round the eight dies, and a split stays on
 // as few of them as there are: each die's L2 then takes in its own columns of
-// x and D alone (D on every die had been most of what the dies read).
+// x and D alone (D on every die had been most of what the dies read). Bound by
+// loads of few steps that a launch, the adapters' search and a sum over the
+// waves frame: 333 tokens of three F16 adapters, rank 64, 6,912 columns (12 MB)
+// some 10.5 us, 512 tokens of an F32 one, rank 128, 1,152 columns some 6.
 template <int kFormat, int kTiles>
 __global__ __launch_bounds__(64 * kDownWaves, 4) void adapter_down_kernel(AdapterArgs a) {
   __shared__ f32x4 sums[kDownWaves][kTiles][64];
@@ -294,6 +297,8 @@ constexpr bool kUpInParts = kFormat != 0 || kRun == 64;
 // item (run of up to kRun tokens, 128 outputs), a wave two tiles of 16 outputs
 // by the run's tiles of 16 tokens. U is read once a run. The low-rank rows lie
 // in LDS as the matrix instructions take them, as three parts of BF16 or F32.
+// Bound by what a compute unit takes in of base, U and the low-rank rows (70 MB
+// in all for 512 tokens, rank 128 in F32, 6,912 outputs: 14 us).
 template <int kFormat, int kTiles, int kRun>
 __global__ __launch_bounds__(64 * kUpWaves, 3) void adapter_up_kernel(AdapterArgs a) {
   constexpr int kChunks = (kTiles + 1) / 2;
@@ -598,13 +603,13 @@ TokenBlocks token_blocks(const AdapterArgs& a, uint32_t turn) {
 }
 
 // Whether it takes a call: where what its workgroups read, each D whole and its
-// part of U, stays below kTokenBytes. Against two launches over runs, 16-bit
-// weights, tokens of one adapter and of an adapter each: rank 64, 1,152 to
-// 6,912, 32 tokens (61 MB) 9.8 and 12.4 us against 10.5 and 14.3, 64 (94 MB) 13.1
-// and 18.2 against 11.4 and 31.1, 128 (151 MB) 20.9 and 28.2 against 11.7 and 31.6;
-// rank 32, 6,912 to 1,152, 128 tokens (122 MB) 9.7 and 14.4 against 17.4 and
-// 33.5, 512 (264 MB) 21.3 and 44.1 against 16.0 and 22.2; rank 16, 1,152 to
-// 1,536, 1 to 256 tokens 7 to 8 against 10 to 12.
+// part of U, stays below kTokenBytes. Against two launches over runs, F16
+// weights, tokens of one adapter and of one each (or of 64): rank 64, 1,152 to
+// 6,912, 16 tokens (50 MB) 8.0 and 8.6 us against 11.0 and 14.0, 64 (90 MB) 13.2
+// and 18.5 against 11.2 and 28.3, 128 (144 MB) 20.8 and 28.5 against 11.6 and
+// 28.7; rank 32, 6,912 to 1,152, 128 tokens (117 MB) 9.7 and 14.4 against 14.8
+// and 26.1, 512 (252 MB) 18.6 and 42.6 against 15.8 and 22.7; rank 16, 1,152 to
+// 1,536, 1 to 256 tokens 7 to 8 against 9 to 12.
 template <int kFormat, int kLanes>
 bool takes_tokens(const AdapterArgs& a) {
   const TokenBlocks b = token_blocks(a, 64 * kTokenWaves / kLanes);

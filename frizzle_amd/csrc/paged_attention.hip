@@ -32,6 +32,12 @@
 //
 // Keys outside the row's range or in no page are never read: their rows are
 // zeros, and their scores -inf.
+//
+// Whole calls, 256 wide, F16 but where said: three requests of 98,001 to
+// 131,072 keys over 4 key-value heads (1.4 GB) 235 us, 6.0 TB/s; 61 of 40 to
+// 8,192 keys (99 MB) 24.6 us, 4.0 TB/s; 32 of 1 to 4,001 keys, 8 BF16 key-value
+// heads of 128 (70 MB), 20.4 us, 3.5 TB/s; one of 5,004 keys (5 MB) 11.5 us,
+// two launches of dependent loads.
 
 #include "batch_rules.h"
 #include "kernels.h"
@@ -594,7 +600,10 @@ __global__ __launch_bounds__(kThreads, (kWorkgroups<kD, kBf16, kW>)) void paged_
 
 // The parts of the rows that have several, joined in order: a workgroup a
 // (record, head, 64 dimensions), 16 lanes of it the dimensions, four each,
-// and its 16 groups every sixteenth part.
+// and its 16 groups every sixteenth part. Some 2 us, a launch and five loads one
+// after another. (The last part's workgroup joining them itself would save the
+// launch, but read all of a row's states, 640 KB for 157 parts of four heads,
+// through one compute unit: 16 us.)
 constexpr uint32_t kJoinGroups = kThreads / 16;
 template <int kD>
 __global__ __launch_bounds__(kThreads) void paged_attention_join_kernel(PagedAttentionArgs a) {
