@@ -452,12 +452,14 @@ __global__ __launch_bounds__(64 * kUpWaves, 3) void adapter_up_kernel(AdapterArg
 // D, a lane 8 columns of each 512, and rows of U, kLanes lanes a row and 8
 // ranks a lane, so that a load is one contiguous piece (a row a lane had been
 // 64 lines a load: 20 to 23 us where this takes 13 to 18, rank 64, 1,152 to
-// 6,912, 64 tokens). Bound by latency at few tokens (two chains of loads and a
-// launch: 3 us of the call's 6) and by what a compute unit takes in, about
-// 40 GB/s, at more: 48 tokens of 41 adapters, BF16, rank 32, 1,152 to 6,912
-// (18.5 MB), 9.2 us a call. Each of a
-// token's workgroups forms all of D x for itself, from L2; numbered by eights
-// of tokens, they are on one die.
+// 6,912, 64 tokens). Each of a token's workgroups forms all of D x for itself,
+// from L2: workgroups go round the eight dies, and each die takes an eighth of
+// the tokens, next to each other, so that they are on one, as are most tokens
+// of one adapter (256 tokens of 64 adapters, rank 32, 6,912 to 1,152: 12.7 us,
+// with every eighth token on a die 23.7). Bound by latency at few tokens (two
+// chains of loads and a launch: 3 us of the call's 6) and by what a compute
+// unit takes in, about 40 GB/s, at more: 48 tokens of 41 adapters, BF16, rank
+// 32, 1,152 to 6,912 (18.5 MB), 9.1 us a call.
 template <int kFormat, int kLanes>
 __global__ __launch_bounds__(64 * kTokenWaves, kFormat == 0 ? 2 : 4)
 void adapter_token_kernel(AdapterArgs a) {
@@ -467,7 +469,8 @@ void adapter_token_kernel(AdapterArgs a) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t places = a.tokens < 8 ? a.tokens : (a.tokens + 7) / 8 * 8;
-  const uint32_t token = blockIdx.x % places;
+  const uint32_t spot = blockIdx.x % places;
+  const uint32_t token = places < 8 ? spot : spot % 8 * (places / 8) + spot / 8;
   if (token >= a.tokens) return;
   const int from = blockIdx.x / places * a.block_rows, to = min(from + a.block_rows, a.rows);
   const uint32_t adapter = a.which[token];
@@ -604,12 +607,12 @@ TokenBlocks token_blocks(const AdapterArgs& a, uint32_t turn) {
 
 // Whether it takes a call: where what its workgroups read, each D whole and its
 // part of U, stays below kTokenBytes. Against two launches over runs, F16
-// weights, tokens of one adapter and of one each (or of 64): rank 64, 1,152 to
-// 6,912, 16 tokens (50 MB) 8.0 and 8.6 us against 11.0 and 14.0, 64 (90 MB) 13.2
-// and 18.5 against 11.2 and 28.3, 128 (144 MB) 20.8 and 28.5 against 11.6 and
-// 28.7; rank 32, 6,912 to 1,152, 128 tokens (117 MB) 9.7 and 14.4 against 14.8
-// and 26.1, 512 (252 MB) 18.6 and 42.6 against 15.8 and 22.7; rank 16, 1,152 to
-// 1,536, 1 to 256 tokens 7 to 8 against 9 to 12.
+// weights, tokens of one adapter and of one each, at most 64: rank 64, 1,152 to
+// 6,912, 16 tokens (50 MB) 7.9 and 8.5 us against 10.8 and 13.8, 64 (90 MB) 13.2
+// and 18.3 against 11.2 and 28.5, 128 (144 MB) 20.4 and 23.5 against 11.8 and
+// 28.5; rank 32, 6,912 to 1,152, 128 tokens (117 MB) 9.7 and 11.4 against 14.6
+// and 26.2, 512 (252 MB) 18.7 and 19.2 against 15.6 and 22.7; rank 16, 1,152 to
+// 1,536, 1 to 256 tokens 7 against 9 to 12.
 template <int kFormat, int kLanes>
 bool takes_tokens(const AdapterArgs& a) {
   const TokenBlocks b = token_blocks(a, 64 * kTokenWaves / kLanes);
