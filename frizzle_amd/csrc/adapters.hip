@@ -9,16 +9,15 @@
 // wave finds for itself from the tokens' adapters, so that a batch of one
 // adapter and one of an adapter a token both fill the chip.
 //
-// The products of runs are on the matrix cores, D's in F32
-// (v_mfma_f32_16x16x4_f32), weights of any format widened exactly on the way,
-// U's mostly of parts of BF16 that add up to the weights (kUpInParts). Sums are
-// F32 in both forms, and nothing is rounded to less. The weights are the
-// instruction's A operand, 16 rows of as many columns as it takes: lane (m, g)
-// holds 8 columns of row m as they lie in memory, and of F32's eight
-// instructions the j-th takes the j-th of each. Loads are a step ahead of the
-// products, and all of a step's loads are requested at once: the kernels are
-// compiled for 1 or 2 (D) and 2, 4 or 8 (U) tiles of 16 ranks, so that no
-// branch parts them.
+// The products of runs are on the matrix cores: with 16-bit weights, and U's of
+// long runs with F32 ones, of parts of 16 bits that add up to the operands, else
+// F32's own (v_mfma_f32_16x16x4_f32). Sums are F32 in both forms, and nothing is
+// rounded to less than 22 bits. The weights are the instruction's A operand, 16
+// rows of as many columns as it takes: lane (m, g) holds 8 columns of row m as
+// they lie in memory, and of F32's eight instructions the j-th takes the j-th of
+// each. Loads are a step ahead of the products, and all of a step's loads are
+// requested at once: the kernels are compiled for 1, 2 or 4 (D) and 2, 4 or 8
+// (U) tiles of 16 ranks, so that no branch parts them.
 
 #include <type_traits>
 
@@ -40,6 +39,11 @@ constexpr int kBlockRows = 32 * kUpWaves;    // outputs of a workgroup
 // many items: ones without an item would wait for a place, then for the tokens'
 // adapters, after all others.
 constexpr uint32_t kMostDown = 512, kMostUp = 768;
+// Columns from which a workgroup of the D kernel takes four tiles of ranks with
+// 16-bit weights, for half of the reads of x: 333 tokens of one adapter, rank 64,
+// 6,912 to 1,152, a call 17.4 -> 15.7 us, though 22.3 -> 24.4 of 32 adapters, as
+// fewer workgroups run at once; 512 tokens, 1,152 columns, rank 128, 20.0 -> 22.5.
+constexpr int kLongCols = 4096;
 constexpr int kTokenWaves = 8;
 constexpr uint32_t kTokenWorkgroups = 256;    // that one launch by tokens is cut into, about
 constexpr uint64_t kTokenBytes = 128u << 20;  // the most that it reads: takes_tokens
@@ -65,11 +69,13 @@ struct Raw {
   }
 };
 
-// F32 values as parts of BF16 that add up to them (three hold 24 bits; their
-// exponents are F32's), each what rounding left to the parts before.
+// F32 values as parts of 16 bits that add up to them (three of BF16 hold F32's
+// 24 bits and its exponents, two of F16 22 bits), each what rounding left to the
+// parts before.
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-template <int kParts>
-__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&part)[kParts]) {
+template <typename T, typename Part, int kParts>
+__device__ __forceinline__ void split8(const float (&x)[8], Part (&part)[kParts]) {
   float rest[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) rest[j] = x[j];
@@ -77,7 +83,7 @@ __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&part)[kPart
   for (int p = 0; p < kParts; ++p)
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      part[p][j] = (__bf16)rest[j];
+      part[p][j] = (T)rest[j];
       if (p + 1 < kParts) rest[j] -= (float)part[p][j];
     }
 }
@@ -194,13 +200,23 @@ __device__ __forceinline__ void copy_base(const AdapterArgs& a, uint32_t first, 
   }
 }
 
+// Whether D's products are of parts of x on the 16-bit matrix cores, the
+// weights as they lie in memory: 2 instructions of 16 cycles for 32 columns
+// where F32's eight take 256 with F16 weights, 3 with BF16 ones. 512 tokens,
+// rank 32, 6,912 to 1,152, F16, of one adapter 15.4 -> 14.6 us a call, of one
+// each 114 -> 105; rank 128, 4,096 to 4,096, 300 of one each 172 -> 158. BF16's
+// parts hold all of x. F16's hold 22 bits of what is within 2^-16 or so of the
+// largest of a token's columns that a wave takes at once, below that 2^-40 of it.
+template <int kFormat>
+constexpr bool kDownInParts = kFormat != 0;
+
 // A wave's share of D x for a run of up to 16 tokens, over the columns
 // [from, to) and kTiles tiles of 16 ranks from `rank0` on: every eighth 32 of
-// the columns. acc[t] has, in lane (n, g), token n's ranks rank0 + 16 t + 4 g
+// the columns. sum[t] has, in lane (n, g), token n's ranks rank0 + 16 t + 4 g
 // .. + 3.
 template <int kFormat, int kTiles>
 __device__ __forceinline__ void low_rank(const AdapterArgs& a, const Run& run, int rank0, int from,
-                                         int to, int wave, int n, int g, f32x4 (&acc)[kTiles]) {
+                                         int to, int wave, int n, int g, f32x4 (&sum)[kTiles]) {
   // Steps whose loads are in flight at once.
   constexpr int kDepth = kTiles == 1 ? 5 : kFormat == 0 ? 3 : 4;
   Raw<0> x[kDepth];
@@ -209,7 +225,7 @@ __device__ __forceinline__ void low_rank(const AdapterArgs& a, const Run& run, i
       a.x + (uint64_t)(run.first + ((uint32_t)n < run.tokens ? n : 0)) * a.x_stride;
   const uint64_t pool = (uint64_t)run.adapter * a.rank * (uint64_t)a.cols;
 #pragma unroll
-  for (int t = 0; t < kTiles; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int t = 0; t < kTiles; ++t) sum[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   for (int k0 = from + 32 * wave; k0 < to; k0 += kDepth * kTurnCols) {
 #pragma unroll
     for (int i = 0; i < kDepth; ++i) {
@@ -222,19 +238,72 @@ __device__ __forceinline__ void low_rank(const AdapterArgs& a, const Run& run, i
         w[i][t].load(a.down,
                      pool + (uint64_t)min(rank0 + 16 * t + n, a.rank - 1) * (uint64_t)a.cols + k);
     }
+    // F16 parts of x scaled by a power of two, token by token, to lie below
+    // 2^15, so that the second ones stay clear of the format's smallest values.
+    float factor = 1.0f, back = 1.0f;
+    f32x4 scaled[kTiles];
+    f32x4(&acc)[kTiles] = kFormat == 1 ? scaled : sum;
+    if constexpr (kFormat == 1) {
+      float most = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kDepth; ++i) {
+        if (k0 + i * kTurnCols >= to) continue;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = __builtin_fmaxf(most, __builtin_fabsf(x[i].at(j)));
+      }
+      most = __builtin_fmaxf(most, __shfl_xor(most, 16));
+      most = __builtin_fmaxf(most, __shfl_xor(most, 32));
+      int up = 141 - (int)(float_to_bits(most) >> 23);
+      up = up > 100 ? 100 : up;
+      factor = bits_to_float((uint32_t)(127 + up) << 23);
+      back = bits_to_float((uint32_t)(127 - up) << 23);
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) scaled[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
 #pragma unroll
     for (int i = 0; i < kDepth; ++i) {
       if (k0 + i * kTurnCols >= to) continue;
       const bool in = k0 + i * kTurnCols + 8 * g < to;
+      if constexpr (kDownInParts<kFormat>) {
+        float xs[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float xj = in ? x[i].at(j) : 0.0f;
+        for (int j = 0; j < 8; ++j) xs[j] = in ? x[i].at(j) * factor : 0.0f;
+        uint4 weight[kTiles];
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t)
-          acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(in ? w[i][t].at(j) : 0.0f, xj, acc[t], 0,
-                                                        0, 0);
+        for (int t = 0; t < kTiles; ++t) weight[t] = in ? w[i][t].r[0] : make_uint4(0, 0, 0, 0);
+        if constexpr (kFormat == 1) {
+          half8 part[2];
+          split8<_Float16>(xs, part);
+#pragma unroll
+          for (int p = 1; p >= 0; --p)
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+              acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                  __builtin_bit_cast(half8, weight[t]), part[p], acc[t], 0, 0, 0);
+        } else {
+          bf16x8 part[3];
+          split8<__bf16>(xs, part);
+#pragma unroll
+          for (int p = 2; p >= 0; --p)
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+              acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                  __builtin_bit_cast(bf16x8, weight[t]), part[p], acc[t], 0, 0, 0);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float xj = in ? x[i].at(j) : 0.0f;
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t)
+            acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(in ? w[i][t].at(j) : 0.0f, xj, acc[t],
+                                                          0, 0, 0);
+        }
       }
     }
+    if constexpr (kFormat == 1)
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) sum[t] += scaled[t] * back;
   }
 }
 
@@ -244,9 +313,10 @@ __device__ __forceinline__ void low_rank(const AdapterArgs& a, const Run& run, i
 // x and D alone (D on every die had been most of what the dies read). Bound by
 // loads of few steps that a launch, the adapters' search and a sum over the
 // waves frame: 333 tokens of three F16 adapters, rank 64, 6,912 columns (12 MB)
-// some 10.5 us, 512 tokens of an F32 one, rank 128, 1,152 columns some 6.
+// some 8.5 us, 512 tokens of an F32 one, rank 128, 1,152 columns some 6.
 template <int kFormat, int kTiles>
-__global__ __launch_bounds__(64 * kDownWaves, 4) void adapter_down_kernel(AdapterArgs a) {
+__global__ __launch_bounds__(64 * kDownWaves, kTiles == 4 ? 2 : 4)
+void adapter_down_kernel(AdapterArgs a) {
   __shared__ f32x4 sums[kDownWaves][kTiles][64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -342,9 +412,10 @@ __global__ __launch_bounds__(64 * kUpWaves, 3) void adapter_up_kernel(AdapterArg
     const float scale = a.scales ? a.scales[run.adapter] : 1.0f;
     const int run_tiles = (int)((run.tokens + 15) / 16);
     __syncthreads();  // the last item's rows are read
-    // Four ranks a thread and piece, the splits of all its pieces asked for
+    // Four ranks a thread and piece, several splits of all its pieces asked for
     // together; ranks past the adapter's own, and tokens past the run, are zero.
-    constexpr int kPieces = kRun * 8 * kChunks / (64 * kUpWaves);
+    constexpr int kFull = kRun * 8 * kChunks, kPieces = kFull < 256 ? 1 : kFull / (64 * kUpWaves);
+    constexpr int kTogether = kPieces <= 2 ? 8 : kPieces <= 4 ? 4 : 2;
     f32x4 piece[kPieces];
     const float* src[kPieces];
 #pragma unroll
@@ -354,16 +425,27 @@ __global__ __launch_bounds__(64 * kUpWaves, 3) void adapter_up_kernel(AdapterArg
       const uint32_t t = min(at / (8 * kChunks), run.tokens - 1);
       const int r = min((int)(at % (8 * kChunks) * 4), a.rank - 4);
       src[i] = a.low + (uint64_t)(run.first + t) * a.rank + r;
-      piece[i] = *reinterpret_cast<const f32x4*>(src[i]);
+      piece[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    for (int s = 1; s < a.splits; ++s)
+    for (int s0 = 0; s0 < a.splits; s0 += kTogether) {
+      f32x4 part[kTogether][kPieces];
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i)
-        piece[i] += *reinterpret_cast<const f32x4*>(src[i] + (uint64_t)s * a.tokens * a.rank);
+      for (int s = 0; s < kTogether; ++s)
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i)
+          part[s][i] = *reinterpret_cast<const f32x4*>(
+              src[i] + (uint64_t)min(s0 + s, a.splits - 1) * a.tokens * a.rank);
+#pragma unroll
+      for (int s = 0; s < kTogether; ++s)
+        if (s0 + s < a.splits)
+#pragma unroll
+          for (int i = 0; i < kPieces; ++i) piece[i] += part[s][i];
+    }
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       const int at = threadIdx.x + i * 64 * kUpWaves;
       const int t = at / (8 * kChunks), r = at % (8 * kChunks) * 4;
+      if (kFull < 256 && t >= kRun) break;
       float rest[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) rest[e] = r + e < rank ? piece[i][e] * scale : 0.0f;
@@ -403,7 +485,7 @@ __global__ __launch_bounds__(64 * kUpWaves, 3) void adapter_up_kernel(AdapterArg
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           weight[i][j] = 32 * c + 8 * g + j < rank ? w[c & 1][i].at(j) : 0.0f;
-        if constexpr (kInParts) split8<kWeights>(weight[i], part[i]);
+        if constexpr (kInParts) split8<__bf16>(weight[i], part[i]);
       }
 #pragma unroll
       for (int t = 0; t < kRunTiles; ++t) {
@@ -566,10 +648,12 @@ template <int kFormat, int kTiles>
 hipError_t launch_up(hipStream_t s, const AdapterArgs& a) {
   // Runs of 64 tokens read U half as often as runs of 32; but a compute unit
   // takes in about 40 GB/s, so shorter ones where the long ones' workgroups
-  // leave compute units idle.
+  // leave compute units idle (333 tokens, rank 64, 1,152 outputs: runs of 16
+  // 3.9 us, of 32 4.3).
   const uint32_t blocks = (a.rows + kBlockRows - 1) / kBlockRows;
-  return (a.tokens + 63) / 64 * blocks < 256 ? launch_runs<kFormat, kTiles, 32>(s, a, blocks)
-                                             : launch_runs<kFormat, kTiles, 64>(s, a, blocks);
+  if ((a.tokens + 63) / 64 * blocks >= 256) return launch_runs<kFormat, kTiles, 64>(s, a, blocks);
+  if ((a.tokens + 31) / 32 * blocks >= 256) return launch_runs<kFormat, kTiles, 32>(s, a, blocks);
+  return launch_runs<kFormat, kTiles, 16>(s, a, blocks);
 }
 
 // Sets the splits.
@@ -591,6 +675,14 @@ hipError_t launch_down(hipStream_t s, AdapterArgs& a) {
                      dim3((uint32_t)(items < kMostDown ? items : kMostDown)),
                      dim3(64 * kDownWaves), 0, s, a);
   return hipGetLastError();
+}
+
+template <int kFormat>
+hipError_t launch_down_tiles(hipStream_t s, AdapterArgs& a) {
+  if (a.rank <= 16) return launch_down<kFormat, 1>(s, a);
+  if constexpr (kFormat != 0)
+    if (a.rank > 32 && a.cols >= kLongCols) return launch_down<kFormat, 4>(s, a);
+  return launch_down<kFormat, 2>(s, a);
 }
 
 // A token's workgroups in adapter_token_kernel, each of so many whole turns of
@@ -641,7 +733,7 @@ hipError_t launch_format(hipStream_t s, AdapterArgs a) {
   } else if (takes_tokens<kFormat, 16>(a)) {
     return launch_token<kFormat, 16>(s, a);
   }
-  const hipError_t e = a.rank <= 16 ? launch_down<kFormat, 1>(s, a) : launch_down<kFormat, 2>(s, a);
+  const hipError_t e = launch_down_tiles<kFormat>(s, a);
   if (e != hipSuccess) return e;
   if (a.rank <= 32) return launch_up<kFormat, 2>(s, a);
   if (a.rank <= 64) return launch_up<kFormat, 4>(s, a);

@@ -56,17 +56,18 @@ def test_columns_at_the_splits(device, cols):
 
 
 # Calls that read over 128 MB a token at a time go by runs of tokens with one
-# adapter, in two launches: each compiled number of ranks, both run lengths
-# (over 255 blocks of 128 outputs for 64 tokens at a time: 64), K in one split
-# and in many, the last of them short.
+# adapter, in two launches: each compiled number of ranks (1, 2 or 4 tiles of D,
+# 2, 4 or 8 of U) and run length (16, 32 and 64), K in one split and in up to 32,
+# the last of them short or without columns.
 @pytest.mark.parametrize("fmt,tokens,rank,cols,rows", [
     (F16, 512, 16, 264, 8100), (BF16, 450, 24, 6912, 300), (F32, 512, 40, 264, 4300),
     (BF16, 333, 64, 8200, 101), (F16, 512, 64, 40, 4500), (F16, 300, 128, 1152, 1901),
-    (F32, 200, 128, 8, 2600), (BF16, 512, 128, 1000, 5002)])
+    (F32, 200, 128, 8, 2600), (BF16, 512, 128, 1000, 5002), (F32, 480, 24, 1504, 2200),
+    (BF16, 512, 8, 14400, 2100), (F16, 511, 128, 200, 2300), (F32, 500, 64, 96, 2100),
+    (F16, 300, 40, 6920, 515), (BF16, 16, 128, 8224, 1000), (F16, 9, 128, 65536, 24),
+    (F32, 40, 16, 30008, 900)])
 @pytest.mark.parametrize("pattern", ["one", "requests", "mixed"])
 def test_runs_of_large_calls(device, fmt, tokens, rank, cols, rows, pattern):
-    size = 4 if fmt == F32 else 2
-    assert tokens * rank * (cols + rows) * size > 128 << 20
     rng = np.random.default_rng(rank + cols)
     pool = Pool(device, rng, 5, rank, cols, rows, fmt, ranks=[rank, 1, rank - 3, 0, 7],
                 scales=[1.0, -0.5, 2.0, 3.0, 0.25])
@@ -78,6 +79,24 @@ def test_runs_of_large_calls(device, fmt, tokens, rank, cols, rows, pattern):
         which = [int(i) for i in rng.choice([0, 0, 1, 2, 4, 9], tokens)]
     x, base = inputs(rng, tokens, pool)
     check_adapters(device, pool, which, x, base)
+
+
+@pytest.mark.parametrize("fmt,tokens,rank,cols,rows", [
+    (F16, 300, 128, 1152, 1901), (BF16, 333, 64, 8200, 101), (F32, 500, 64, 96, 2100),
+    (F16, 20, 16, 264, 500), (BF16, 20, 16, 264, 500)])
+def test_tokens_of_any_size(device, fmt, tokens, rank, cols, rows):
+    # Tokens of 10^-25 to 10^25 side by side, one of zeros, and a column 2^15 times
+    # the others whose weights are zeros: it must cost them none of their bits.
+    rng = np.random.default_rng(rows)
+    pool = Pool(device, rng, 2, rank, cols, rows, fmt)
+    pool.down[:, :, 3] = 0
+    pool.dev[0] = device.array(pool.down)
+    x, base = inputs(rng, tokens, pool)
+    x[1::3, 3] = 2.0 ** 15
+    size = (10.0 ** rng.uniform(-25, 25, (tokens, 1))).astype(np.float32)
+    size[1] = 0.0
+    which = [int(i) for i in np.sort(rng.integers(0, 2, tokens))]
+    check_adapters(device, pool, which, x * size, base * size)
 
 
 def test_runs_in_place_and_strided(device):
