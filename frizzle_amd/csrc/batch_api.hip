@@ -13,7 +13,7 @@
 namespace frz {
 namespace {
 
-constexpr size_t kStateFloats = (size_t)kMostJoinedParts * rules::kHeadBlock * 256;
+constexpr size_t kStateFloats = (size_t)kMostStateValues * rules::kHeadBlock;
 constexpr size_t kStatFloats = (size_t)kMostJoinedParts * rules::kHeadBlock * 2;
 constexpr size_t kRecords = kMostJoinedParts / 2;
 constexpr size_t kAttentionBytes =

@@ -79,14 +79,20 @@ FRZ_RULE uint32_t row_blocks(KeyRange r) {
 // fewest are between the batch's blocks shared out evenly and those shared
 // over what the `units` (rows times head blocks) leave, as each has at most one
 // part that is not full; `parts` counts a chunk's parts, and six halvings come
-// near enough. Where the units alone are more than run at once, an even share.
+// near enough. Where the units alone are more than run at once, an even share
+// of half as many parts more, so that what runs last is shorter (300 requests
+// of 1,000 to 2,000 keys 112 us by shares of as many, 103 by these; of twice as
+// many 113).
+FRZ_RULE uint32_t shares(uint32_t units, uint32_t at_once) {
+  return units < at_once ? at_once : at_once + at_once / 2;
+}
 FRZ_RULE uint32_t even_chunk(uint64_t blocks, uint32_t share) {
   const uint64_t even = (blocks + share - 1) / share;
   return (uint32_t)(even <= 2 ? even : (even + kPartWaves - 1) / kPartWaves * kPartWaves);
 }
 template <typename Count>
 FRZ_RULE uint32_t part_chunk(uint64_t blocks, uint32_t units, uint32_t at_once, Count parts) {
-  uint32_t low = even_chunk(blocks, at_once);
+  uint32_t low = even_chunk(blocks, shares(units, at_once));
   if (units >= at_once) return low;
   while (low < kPartWaves && parts(low) > at_once) low = low < 2 ? 2 : kPartWaves;
   if (parts(low) <= at_once) return low;
@@ -102,10 +108,10 @@ FRZ_RULE uint32_t part_chunk(uint64_t blocks, uint32_t units, uint32_t at_once, 
 // The most parts there can be, and the most that belong to rows of several
 // parts: such a row has fewer than twice the parts that its blocks fill.
 FRZ_RULE uint32_t most_parts(uint32_t units, uint32_t at_once) {
-  return units < at_once ? at_once : at_once + units;
+  return units < at_once ? at_once : shares(units, at_once) + units;
 }
 FRZ_RULE uint32_t most_joined_parts(uint32_t units, uint32_t at_once) {
-  return units < at_once ? at_once : 2 * at_once;
+  return units < at_once ? at_once : 2 * shares(units, at_once);
 }
 
 }  // namespace rules

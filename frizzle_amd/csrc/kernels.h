@@ -476,8 +476,8 @@ struct PagedAttentionArgs {
   uint32_t window;
   float scale_log2e;
   uint32_t rows;
-  // The states of rows cut into several parts: [kMostJoinedParts][16 heads]
-  // of head_dim outputs, and of (m, l); a record of each such row and head
+  // The states of rows cut into several parts, at most kMostJoinedParts of them
+  // of 16 heads: head_dim outputs each, and (m, l); a record of each row and head
   // block, and their number.
   float* states;
   float* stats;
@@ -487,7 +487,11 @@ struct PagedAttentionArgs {
 };
 constexpr int kMostComputeUnits = 256;  // gfx950's
 constexpr int kAttentionWorkgroups = 4;  // a compute unit's at once, at most
-constexpr int kMostJoinedParts = 2 * kAttentionWorkgroups * kMostComputeUnits;
+constexpr int kMostJoinedParts = 3 * kAttentionWorkgroups * kMostComputeUnits;
+// Values of one head in all of their states: workgroups of a compute unit take
+// kAttentionWidth of them together, at most.
+constexpr int kAttentionWidth = 384;
+constexpr int kMostStateValues = 3 * kAttentionWidth * kMostComputeUnits;
 hipError_t launch_paged_attention(hipStream_t s, const PagedAttentionArgs& a, int compute_units);
 
 struct AdapterArgs {

@@ -4,7 +4,8 @@
 // key-value head and up to 16 of its query heads. A wave takes every fourth
 // of the part's blocks of 32 keys with a running maximum m, sum l and output
 // O of its own; the part's waves are joined through LDS, the parts of a row
-// that has several by a second launch, in order.
+// that has several by a second launch, in order. Short rows are not cut, and
+// many short ones a wave each (launch_shape).
 //
 // What bounds it is the stream of key and value rows, so nothing of it waits:
 // both go from memory to the registers that the matrix instructions read,
@@ -52,8 +53,10 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kThreads = 64 * kPartWaves;
 constexpr float kMinusInf = -__builtin_inff();
+// Rows of no more blocks than these, or blocks times head_dim, are not cut: see
+// launch_shape.
+constexpr uint64_t kWaveBlocks = 32, kFewValues = 2048, kManyValues = 8192;
 constexpr int kBufferWord3 = 0x00020000;  // raw 32-bit data
 
 template <bool kBf16>
@@ -100,7 +103,9 @@ template <int kD, bool kBf16, int kW>
 constexpr int kWorkgroups = kD == 256   ? 1
                             : kD == 128 ? (Shape<kD, kBf16, kW>::kTiles == 1 ? 3 : 2)
                                         : (Shape<kD, kBf16, kW>::kTiles <= 2 ? 4 : 3);
-static_assert(kWorkgroups<64, false, 8> <= kAttentionWorkgroups, "the workspace holds their parts");
+template <int kD, bool kBf16, int kW>
+constexpr bool kFits = kWorkgroups<kD, kBf16, kW> <= kAttentionWorkgroups &&
+                       kWorkgroups<kD, kBf16, kW> * kD <= kAttentionWidth;
 
 // A column's part of a value: what rounding it left to the parts before, taken
 // off (`less` holds -1 for each of those, 0 for the others), rounded in its turn.
@@ -266,23 +271,34 @@ __device__ __forceinline__ bool find_part(const PagedAttentionArgs& a, uint32_t 
   return true;
 }
 
-template <int kD, bool kBf16, int kW>
-__global__ __launch_bounds__(kThreads, (kWorkgroups<kD, kBf16, kW>)) void paged_attention_kernel(
-    PagedAttentionArgs a) {
+template <int kD, bool kBf16, int kW, int kWaves, bool kWhole>
+__global__ __launch_bounds__(64 * kWaves, (kWorkgroups<kD, kBf16, kW>))
+void paged_attention_kernel(PagedAttentionArgs a) {
   typedef Shape<kD, kBf16, kW> S;
   typedef Types<kBf16> T;
   constexpr int kPitch = kD + 8;  // floats a head's outputs take in LDS
-  __shared__ __attribute__((aligned(16))) float joined_out[kPartWaves][kW * kPitch];
-  __shared__ float joined_m[kPartWaves][kW], joined_l[kPartWaves][kW];
+  __shared__ __attribute__((aligned(16))) float joined_out[kWaves][kW * kPitch];
+  __shared__ float joined_m[kWaves][kW], joined_l[kWaves][kW];
   const int lane = threadIdx.x & 63;
   const uint32_t wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int n = lane & 15, g = lane >> 4;
 
   Part part;
-  const bool found = a.rows <= 64 ? find_part<1>(a, blockIdx.x, lane, &part)
-                                  : find_part<kMostRows / 64>(a, blockIdx.x, lane, &part);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *a.record_count = part.records;
-  if (!found) return;
+  if constexpr (kWhole) {
+    part.row = blockIdx.x / a.units;
+    part.unit = blockIdx.x % a.units;
+    part.position = a.positions[part.row];
+    if (part.position == kNone) return;
+    part.sequence = a.sequences ? a.sequences[part.row] : part.row;
+    part.index = 0;
+    part.parts = 1;
+    part.chunk = kMostKeys / kBlockKeys;
+  } else {
+    const bool found = a.rows <= 64 ? find_part<1>(a, blockIdx.x, lane, &part)
+                                    : find_part<kMostRows / 64>(a, blockIdx.x, lane, &part);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.record_count = part.records;
+    if (!found) return;
+  }
   const uint32_t head_blocks = a.units / a.cache.kv_heads;
   const uint32_t kv = part.unit / head_blocks;
   const uint32_t group = a.query_heads / a.cache.kv_heads;
@@ -301,7 +317,7 @@ __global__ __launch_bounds__(kThreads, (kWorkgroups<kD, kBf16, kW>)) void paged_
   // that half's first key lies in the pool, in values, or ~0.
   const uint32_t row_values = a.cache.kv_heads * kD, row_bytes = 2 * row_values;
   auto find_pages = [&](uint32_t block) {
-    const uint32_t key = (block + kPartWaves * (lane >> 1)) * kBlockKeys + 16 * (lane & 1);
+    const uint32_t key = (block + kWaves * (lane >> 1)) * kBlockKeys + 16 * (lane & 1);
     uint64_t at = ~0ull;
     if (key < keys.end && key + 16 > keys.first) {
       const uint32_t index = key / a.cache.page_slots;
@@ -411,7 +427,7 @@ __global__ __launch_bounds__(kThreads, (kWorkgroups<kD, kBf16, kW>)) void paged_
   // The first block from `block` on that holds a key; `turn` counts the
   // blocks whose pages are known.
   auto seek = [&](Block* k) {
-    for (; block < last_block; block += kPartWaves, ++turn) {
+    for (; block < last_block; block += kWaves, ++turn) {
       if (turn == 32) {
         pages = find_pages(block);
         turn = 0;
@@ -468,7 +484,7 @@ __global__ __launch_bounds__(kThreads, (kWorkgroups<kD, kBf16, kW>)) void paged_
       hold();
       // After the last block, of no rows: a branch around the loads would make
       // each wait one for all that are under way.
-      block += kPartWaves;
+      block += kWaves;
       ++turn;
       more = seek(&next);
       load_keys(next);
@@ -560,16 +576,16 @@ __global__ __launch_bounds__(kThreads, (kWorkgroups<kD, kBf16, kW>)) void paged_
       }
     }
   __syncthreads();
-  const bool whole = part.parts == 1;
-  for (uint32_t i = threadIdx.x; i < heads * (kD / 4); i += kThreads) {
+  const bool whole = kWhole || part.parts == 1;
+  for (uint32_t i = threadIdx.x; i < heads * (kD / 4); i += 64 * kWaves) {
     const uint32_t h = i / (kD / 4), d = i % (kD / 4) * 4;
     float top = joined_m[0][h];
 #pragma unroll
-    for (uint32_t w = 1; w < kPartWaves; ++w) top = __builtin_fmaxf(top, joined_m[w][h]);
+    for (uint32_t w = 1; w < kWaves; ++w) top = __builtin_fmaxf(top, joined_m[w][h]);
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float weights = 0.0f;
 #pragma unroll
-    for (uint32_t w = 0; w < kPartWaves; ++w) {
+    for (uint32_t w = 0; w < kWaves; ++w) {
       // A wave without a key holds zeros, and so does a row without one.
       const float f = top == kMinusInf ? 0.0f : __builtin_amdgcn_exp2f(joined_m[w][h] - top);
       const float4 o = *reinterpret_cast<const float4*>(&joined_out[w][h * kPitch + d]);
@@ -604,10 +620,10 @@ __global__ __launch_bounds__(kThreads, (kWorkgroups<kD, kBf16, kW>)) void paged_
 // after another. (The last part's workgroup joining them itself would save the
 // launch, but read all of a row's states, 640 KB for 157 parts of four heads,
 // through one compute unit: 16 us.)
-constexpr uint32_t kJoinGroups = kThreads / 16;
+constexpr uint32_t kJoinWaves = 4, kThreads = 64 * kJoinWaves, kJoinGroups = kThreads / 16;
 template <int kD>
 __global__ __launch_bounds__(kThreads) void paged_attention_join_kernel(PagedAttentionArgs a) {
-  __shared__ float wave_top[kPartWaves], wave_sum[kPartWaves];
+  __shared__ float wave_top[kJoinWaves], wave_sum[kJoinWaves];
   __shared__ float factors[kMostJoinedParts];
   __shared__ float4 sums[kJoinGroups][16];
   const uint32_t count = *a.record_count;
@@ -625,7 +641,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_join_kernel(PagedAtt
     __syncthreads();  // the last record's reads are done
     if (lane == 0) wave_top[wave] = top;
     __syncthreads();
-    for (uint32_t w = 0; w < kPartWaves; ++w) top = __builtin_fmaxf(top, wave_top[w]);
+    for (uint32_t w = 0; w < kJoinWaves; ++w) top = __builtin_fmaxf(top, wave_top[w]);
     float weights = 0.0f;
     for (uint32_t p = t; p < parts; p += kThreads) {
       const float2 s =
@@ -665,19 +681,41 @@ __global__ __launch_bounds__(kThreads) void paged_attention_join_kernel(PagedAtt
 
 template <int kD, bool kBf16, int kW>
 hipError_t launch_shape(hipStream_t s, PagedAttentionArgs a, uint32_t heads, int compute_units) {
+  static_assert(kFits<kD, kBf16, kW>, "the workspace holds their parts");
   const uint32_t units = a.rows * a.units;
   a.at_once = kWorkgroups<kD, kBf16, kW> * (uint32_t)compute_units;
-  // No more parts than the rows have blocks.
+  // The most blocks that a row can have. Where they are few, each unit is one
+  // workgroup's (kWhole), which then need not find its part, nor leave a state
+  // to a second launch: always to kFewValues (64 requests of up to 250 keys, 256
+  // wide, 12.6 us cut, 10.8 whole), and to kManyValues where enough units are
+  // there to keep the compute units at work (100 of a window of 512: 22.6 and
+  // 17.2; but 16: 11.9 and 16.0). Where more units are there than workgroups run
+  // at once, a unit is a wave's: four waves would each have had a block or two
+  // of a short row (483 rows of 16 to 31 keys, 8 key-value heads, 256 wide, 137
+  // us and 35; 512 of a window of 512 67 and 52; not of 63 blocks, 400 rows of 8
+  // heads 128 wide: 214 by workgroups, 257 by waves).
   const uint64_t capacity = (uint64_t)a.cache.width * a.cache.page_slots;
   const uint64_t held = (capacity + kBlockKeys - 1) / kBlockKeys;
   const uint64_t seen = (uint64_t)a.window / kBlockKeys + 2;
   const uint64_t blocks = held < seen ? held : seen;
+  if (units >= a.at_once && blocks <= kWaveBlocks) {
+    hipLaunchKernelGGL((paged_attention_kernel<kD, kBf16, kW, 1, true>), dim3(units), dim3(64), 0,
+                       s, a);
+    return hipGetLastError();
+  }
+  const bool few = 8 * units < 3 * (uint32_t)compute_units;
+  if (blocks * kD <= (few ? kFewValues : kManyValues)) {
+    hipLaunchKernelGGL((paged_attention_kernel<kD, kBf16, kW, kPartWaves, true>), dim3(units),
+                       dim3(64 * kPartWaves), 0, s, a);
+    return hipGetLastError();
+  }
+  // No more parts than the rows have blocks.
   const uint64_t fill = units * blocks;
   const uint64_t bound = most_parts(units, a.at_once);
-  hipLaunchKernelGGL((paged_attention_kernel<kD, kBf16, kW>),
-                     dim3((uint32_t)(fill < bound ? fill : bound)), dim3(kThreads), 0, s, a);
+  hipLaunchKernelGGL((paged_attention_kernel<kD, kBf16, kW, kPartWaves, false>),
+                     dim3((uint32_t)(fill < bound ? fill : bound)), dim3(64 * kPartWaves), 0, s, a);
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || blocks == 1) return e;  // no row has two parts
+  if (e != hipSuccess) return e;
   const uint32_t joins = most_joined_parts(units, a.at_once) / 2;
   const uint32_t records = units < joins ? units : joins;
   hipLaunchKernelGGL(paged_attention_join_kernel<kD>,

@@ -130,6 +130,6 @@ def test_every_block_in_one_part_within_the_grid(rules, lengths, window, capacit
     assert chunk % 4 == 0 or chunk <= 2
     assert parts <= most
     # The workspace holds the parts of rows that have several.
-    assert joined <= most_joined <= 2 * at_once
+    assert joined <= most_joined <= 3 * at_once
     if any(lengths):
         assert chunk >= 1

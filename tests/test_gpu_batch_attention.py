@@ -21,29 +21,41 @@ def batch(device, seed, lengths, heads, kv, dim, slots, fmt, **more):
     return paged, query, positions
 
 
+# Tables of no more pages than the rows have, whose rows go uncut, a workgroup
+# each; and of LONG keys, which could hold rows that are cut into parts.
+LONG = 20000
+TABLES = pytest.mark.parametrize("keys", [0, LONG])
+
+
 # Every compiled shape, groups that leave columns free and such that take two
 # head blocks.
 @pytest.mark.parametrize("heads,kv,dim", [
     (4, 1, 256), (1, 1, 64), (3, 3, 128), (6, 2, 128), (8, 1, 256), (9, 1, 64), (10, 2, 256),
     (16, 1, 128), (32, 2, 256), (20, 1, 64), (66, 2, 128), (40, 8, 64), (17, 1, 256)])
 @pytest.mark.parametrize("fmt", [F16, BF16])
-def test_head_layouts(device, heads, kv, dim, fmt):
+@TABLES
+def test_head_layouts(device, heads, kv, dim, fmt, keys):
     lengths = [1, 40, 0, 130, 17, 300]
-    paged, query, positions = batch(device, heads + dim, lengths, heads, kv, dim, 32, fmt)
+    paged, query, positions = batch(device, heads + dim, lengths, heads, kv, dim, 32, fmt,
+                                    wide=keys // 32)
     check_attention(device, paged, positions, query, heads, NONE, dim ** -0.5)
 
 
 @pytest.mark.parametrize("slots", [16, 48, 64, 1024])
 @pytest.mark.parametrize("window", [1, 31, 33, 100, 512, NONE])
-def test_lengths_windows_and_pages(device, slots, window):
-    paged, query, positions = batch(device, slots + window % 1000, EDGES, 4, 1, 256, slots, F16)
+@TABLES
+def test_lengths_windows_and_pages(device, slots, window, keys):
+    paged, query, positions = batch(device, slots + window % 1000, EDGES, 4, 1, 256, slots, F16,
+                                    wide=keys // slots)
     check_attention(device, paged, positions, query, 4, window, 1 / 16)
 
 
 @pytest.mark.parametrize("dim,fmt", [(64, F16), (128, BF16)])
 @pytest.mark.parametrize("window", [40, NONE])
-def test_lengths_of_other_widths(device, dim, fmt, window):
-    paged, query, positions = batch(device, dim + window % 999, EDGES, 6, 2, dim, 16, fmt)
+@TABLES
+def test_lengths_of_other_widths(device, dim, fmt, window, keys):
+    paged, query, positions = batch(device, dim + window % 999, EDGES, 6, 2, dim, 16, fmt,
+                                    wide=keys // 16)
     check_attention(device, paged, positions, query, 6, window, dim ** -0.5)
 
 
@@ -59,9 +71,33 @@ def test_rows_of_several_parts(device, lengths, heads, kv, dim, slots, fmt):
 
 
 @pytest.mark.parametrize("heads,kv", [(1024, 1024), (1024, 2), (1024, 1), (1008, 63)])
-def test_the_most_heads(device, heads, kv):
-    paged, query, positions = batch(device, heads + kv, [33, 0, 150, 1, 18], heads, kv, 64, 16, F16)
+@TABLES
+def test_the_most_heads(device, heads, kv, keys):
+    paged, query, positions = batch(device, heads + kv, [33, 0, 150, 1, 18], heads, kv, 64, 16, F16,
+                                    wide=keys // 16)
     check_attention(device, paged, positions, query, heads, 100, 0.125)
+
+
+# More rows and key-value heads than workgroups run at once: a wave each.
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("group,fmt", [(1, F16), (6, F16), (12, F16), (17, F16), (4, BF16),
+                                       (7, BF16), (16, BF16)])
+@pytest.mark.parametrize("window", [40, NONE])
+def test_many_short_rows(device, dim, group, fmt, window):
+    rng = np.random.default_rng(dim + group)
+    lengths = [int(n) for n in rng.integers(0, 100, 270)]
+    paged, query, positions = batch(device, group, lengths, 4 * group, 4, dim, 16, fmt)
+    check_attention(device, paged, positions, query, 4 * group, window, dim ** -0.5)
+
+
+# The same over long tables: more units than parts run at once, several parts.
+@pytest.mark.parametrize("dim,fmt,window", [(256, F16, NONE), (128, BF16, 1100), (64, F16, NONE)])
+def test_many_rows_some_long(device, dim, fmt, window):
+    rng = np.random.default_rng(dim)
+    lengths = [int(n) for n in rng.integers(0, 60, 270)]
+    lengths[7], lengths[100], lengths[269] = 9000, 4097, 1500
+    paged, query, positions = batch(device, dim, lengths, 4, 4, dim, 16, fmt)
+    check_attention(device, paged, positions, query, 4, window, dim ** -0.5)
 
 
 def test_the_most_rows(device):
@@ -79,9 +115,10 @@ def test_no_row_after_rows_of_several_parts(device):
     assert (got == 7.0).all()
 
 
-def test_several_rows_of_a_request_in_any_order(device):
+@TABLES
+def test_several_rows_of_a_request_in_any_order(device, keys):
     rng = np.random.default_rng(9)
-    paged, _, _ = batch(device, 10, [700, 0, 333, 64], 4, 1, 256, 16, F16)
+    paged, _, _ = batch(device, 10, [700, 0, 333, 64], 4, 1, 256, 16, F16, wide=keys // 16)
     requests = [2, 0, 3, 0, 2, 0, 9, 1, NONE]
     positions = [332, 699, 63, 5, 100, NONE, 20, 10, 4]
     query = rng.normal(0, 1, (9, 1024)).astype(np.float32)
@@ -90,8 +127,10 @@ def test_several_rows_of_a_request_in_any_order(device):
     assert (got[6:] == 0.0).all()
 
 
-def test_pages_that_are_not_there(device):
-    paged, query, positions = batch(device, 11, [400, 400, 400, 400, 90], 4, 1, 256, 16, F16)
+@TABLES
+def test_pages_that_are_not_there(device, keys):
+    paged, query, positions = batch(device, 11, [400, 400, 400, 400, 90], 4, 1, 256, 16, F16,
+                                    wide=keys // 16)
     paged.table[0, 3] = NONE           # a hole
     paged.table[0, 24] = paged.pages   # the last page, and so the row's own key
     paged.table[1, :] = 4000000000     # none at all
@@ -128,12 +167,14 @@ def test_shared_prefix_pages(device):
     check_attention(device, paged, positions, query, 4, NONE, 1 / 16)
 
 
+@TABLES
 @pytest.mark.parametrize("fmt", [F16, BF16])
 @pytest.mark.parametrize("query_scale,key_scale", [
     (1e4, 1e-4), (1e-30, 1.0), (3e6, 1e-6), (0.0, 1.0), (1.0, 1e-5), (30.0, 1.0)])
-def test_queries_and_keys_of_any_size(device, fmt, query_scale, key_scale):
+def test_queries_and_keys_of_any_size(device, fmt, query_scale, key_scale, keys):
     # F16 keys of 1e-5 and 1e-6 are subnormal; scores of 30 make peaked weights.
-    paged, query, positions = batch(device, 15, [150, 33, 1], 4, 1, 256, 16, fmt, scale=key_scale)
+    paged, query, positions = batch(device, 15, [150, 33, 1], 4, 1, 256, 16, fmt, scale=key_scale,
+                                    wide=keys // 16)
     query = (query * query_scale).astype(np.float32)
     check_attention(device, paged, positions, query, 4, NONE, 1 / 16)
 
@@ -167,8 +208,9 @@ def test_rising_scores(device):
     check_attention(device, paged, positions, query, 4, NONE, 1 / 16)
 
 
-def test_a_query_that_is_no_number_stays_in_its_row(device):
-    paged, query, positions = batch(device, 18, [100, 100, 3000], 4, 1, 256, 16, F16)
+@pytest.mark.parametrize("length", [200, 3000])
+def test_a_query_that_is_no_number_stays_in_its_row(device, length):
+    paged, query, positions = batch(device, 18, [100, 100, length], 4, 1, 256, 16, F16)
     bad = query.copy()
     bad[1, 300] = np.nan
     bad[2, 1000] = np.inf
