@@ -46,7 +46,8 @@ constexpr uint32_t kMostDown = 512, kMostUp = 768;
 constexpr int kLongCols = 4096;
 constexpr int kTokenWaves = 8;
 constexpr uint32_t kTokenWorkgroups = 256;    // that one launch by tokens is cut into, about
-constexpr uint64_t kTokenBytes = 128u << 20;  // the most that it reads: takes_tokens
+// The most that it reads, and the most of it that is one D: takes_tokens.
+constexpr uint64_t kTokenBytes = 128u << 20, kTokenDown = 600u << 10;
 
 // Eight weights as they lie in memory, from element `at` (a multiple of 8).
 template <int kFormat>
@@ -697,8 +698,12 @@ TokenBlocks token_blocks(const AdapterArgs& a, uint32_t turn) {
   return {each * turn, (turns + each - 1) / each};
 }
 
-// Whether it takes a call: where what its workgroups read, each D whole and its
-// part of U, stays below kTokenBytes. Against two launches over runs, F16
+// Whether it takes a call: where a D, which each of its workgroups reads whole,
+// a load after another, stays below kTokenDown (one token, 4,000 outputs, rank
+// 128, F16, of 1,152 columns, 295 kB, 9.7 us against 11.8 over runs, of 2,304 12.5
+// against 11.0, of 6,912 25.9 against 13.9; rank 32 of 9,216, 590 kB, 10.4 against
+// 11.8, of 16,384 15.2 against 12.1), and what all of them read, U with it, below
+// kTokenBytes. Against two launches over runs, F16
 // weights, tokens of one adapter and of one each, at most 64: rank 64, 1,152 to
 // 6,912, 16 tokens (50 MB) 7.9 and 8.5 us against 10.8 and 13.8, 64 (90 MB) 13.2
 // and 18.3 against 11.2 and 28.5, 128 (144 MB) 20.4 and 23.5 against 11.8 and
@@ -708,8 +713,9 @@ TokenBlocks token_blocks(const AdapterArgs& a, uint32_t turn) {
 template <int kFormat, int kLanes>
 bool takes_tokens(const AdapterArgs& a) {
   const TokenBlocks b = token_blocks(a, 64 * kTokenWaves / kLanes);
-  const uint64_t weights = (uint64_t)a.rank * ((uint64_t)b.count * a.cols + a.rows);
-  return a.tokens * weights * (kFormat == 0 ? 4 : 2) <= kTokenBytes;
+  const uint64_t size = kFormat == 0 ? 4 : 2, down = (uint64_t)a.rank * a.cols * size;
+  return down <= kTokenDown &&
+         a.tokens * (b.count * down + (uint64_t)a.rank * a.rows * size) <= kTokenBytes;
 }
 
 template <int kFormat, int kLanes>

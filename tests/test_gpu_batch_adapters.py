@@ -55,8 +55,8 @@ def test_columns_at_the_splits(device, cols):
     check_adapters(device, pool, which, x, base)
 
 
-# Calls that read over 128 MB a token at a time go by runs of tokens with one
-# adapter, in two launches: each compiled number of ranks (1, 2 or 4 tiles of D,
+# Calls that read over 128 MB a token at a time, or over 600 kB of one token's D,
+# go by runs of tokens with one adapter, in two launches: each compiled number of ranks (1, 2 or 4 tiles of D,
 # 2, 4 or 8 of U) and run length (16, 32 and 64), K in one split and in up to 32,
 # the last of them short or without columns.
 @pytest.mark.parametrize("fmt,tokens,rank,cols,rows", [
@@ -65,7 +65,8 @@ def test_columns_at_the_splits(device, cols):
     (F32, 200, 128, 8, 2600), (BF16, 512, 128, 1000, 5002), (F32, 480, 24, 1504, 2200),
     (BF16, 512, 8, 14400, 2100), (F16, 511, 128, 200, 2300), (F32, 500, 64, 96, 2100),
     (F16, 300, 40, 6920, 515), (BF16, 16, 128, 8224, 1000), (F16, 9, 128, 65536, 24),
-    (F32, 40, 16, 30008, 900)])
+    (F32, 40, 16, 30008, 900), (F16, 1, 128, 4280, 701), (BF16, 3, 64, 9000, 130),
+    (F32, 17, 128, 2304, 1), (F16, 2, 16, 20000, 257), (F32, 1, 8, 19400, 33)])
 @pytest.mark.parametrize("pattern", ["one", "requests", "mixed"])
 def test_runs_of_large_calls(device, fmt, tokens, rank, cols, rows, pattern):
     rng = np.random.default_rng(rank + cols)
