@@ -38,7 +38,9 @@ constexpr int kBlockRows = 32 * kUpWaves;    // outputs of a workgroup
 // Workgroups that run at once; a launch has no more, and each takes every so
 // many items: ones without an item would wait for a place, then for the tokens'
 // adapters, after all others.
-constexpr uint32_t kMostDown = 512, kMostUp = 768;
+constexpr uint32_t kMostDown = 512;
+template <int kRun>
+constexpr uint32_t kUpPlaces = kRun == 16 ? 4 : 3;  // of the U kernel, a compute unit's
 // Columns from which a workgroup of the D kernel takes four tiles of ranks with
 // 16-bit weights, for half of the reads of x: 333 tokens of one adapter, rank 64,
 // 6,912 to 1,152, a call 17.4 -> 15.7 us, though 22.3 -> 24.4 of 32 adapters, as
@@ -371,7 +373,7 @@ constexpr bool kUpInParts = kFormat != 0 || kRun == 64;
 // Bound by what a compute unit takes in of base, U and the low-rank rows (70 MB
 // in all for 512 tokens, rank 128 in F32, 6,912 outputs: 14 us).
 template <int kFormat, int kTiles, int kRun>
-__global__ __launch_bounds__(64 * kUpWaves, 3) void adapter_up_kernel(AdapterArgs a) {
+__global__ __launch_bounds__(64 * kUpWaves, kUpPlaces<kRun>) void adapter_up_kernel(AdapterArgs a) {
   constexpr int kChunks = (kTiles + 1) / 2;
   constexpr int kRunTiles = kRun / 16;
   constexpr bool kInParts = kUpInParts<kFormat, kRun>;
@@ -637,10 +639,11 @@ void adapter_token_kernel(AdapterArgs a) {
 
 template <int kFormat, int kTiles, int kRun>
 hipError_t launch_runs(hipStream_t s, const AdapterArgs& a, uint32_t blocks) {
+  constexpr uint32_t kMost = 256 * kUpPlaces<kRun>;
   // As many workgroups as items where every token is a run.
   const uint64_t items = (uint64_t)a.tokens * (blocks < 8 ? blocks : (blocks + 7) / 8 * 8);
   hipLaunchKernelGGL((adapter_up_kernel<kFormat, kTiles, kRun>),
-                     dim3((uint32_t)(items < kMostUp ? items : kMostUp)), dim3(64 * kUpWaves), 0, s,
+                     dim3((uint32_t)(items < kMost ? items : kMost)), dim3(64 * kUpWaves), 0, s,
                      a);
   return hipGetLastError();
 }
