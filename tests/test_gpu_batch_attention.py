@@ -247,6 +247,33 @@ def test_the_same_bits_every_time_and_from_threads(device):
     assert not bad
 
 
+def test_two_handles_of_one_device_at_once(device):
+    # Each has its own stream and workspace.
+    import frizzle_amd as fz
+    other = fz.Device(0)
+    try:
+        sets = [(d, *batch(d, 24 + i, [5000 + 300 * i, 20, 0, 900], 4, 1, 256, 64, F16))
+                for i, d in enumerate((device, other))]
+        want = [attention(d, p, at, q, 4, NONE, 1 / 16) for d, p, q, at in sets]
+        bad = []
+
+        def work(i):
+            d, p, q, at = sets[i]
+            for _ in range(30):
+                if not np.array_equal(attention(d, p, at, q, 4, NONE, 1 / 16), want[i]):
+                    bad.append(i)
+
+        threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert not bad
+        sets.clear()
+    finally:
+        other.close()
+
+
 def test_batch_does_not_change_a_row_much(device):
     # A row's cut goes by the batch, so its bits may; its values stay in bounds.
     paged, query, positions = batch(device, 21, [3000] * 40, 4, 1, 256, 64, F16)
