@@ -35,12 +35,13 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int kDownWaves = 8, kUpWaves = 4;  // of a workgroup
 constexpr int kTurnCols = 32 * kDownWaves;   // columns that its waves take a turn
 constexpr int kBlockRows = 32 * kUpWaves;    // outputs of a workgroup
-// Workgroups that run at once; a launch has no more, and each takes every so
-// many items: ones without an item would wait for a place, then for the tokens'
-// adapters, after all others.
-constexpr uint32_t kMostDown = 512;
+// Workgroups that a compute unit runs at once; a launch has no more, and each
+// takes every so many items: ones without an item would wait for a place, then
+// for the tokens' adapters, after all others.
+template <int kTiles>
+constexpr uint32_t kDownPlaces = kTiles == 4 ? 1 : 2;  // of the D kernel
 template <int kRun>
-constexpr uint32_t kUpPlaces = kRun == 16 ? 4 : 3;  // of the U kernel, a compute unit's
+constexpr uint32_t kUpPlaces = kRun == 16 ? 4 : 3;  // of the U kernel
 // Columns from which a workgroup of the D kernel takes four tiles of ranks with
 // 16-bit weights, for half of the reads of x: 333 tokens of one adapter, rank 64,
 // 6,912 to 1,152, a call 17.4 -> 15.7 us, though 22.3 -> 24.4 of 32 adapters, as
@@ -318,7 +319,7 @@ __device__ __forceinline__ void low_rank(const AdapterArgs& a, const Run& run, i
 // waves frame: 333 tokens of three F16 adapters, rank 64, 6,912 columns (12 MB)
 // some 8.5 us, 512 tokens of an F32 one, rank 128, 1,152 columns some 6.
 template <int kFormat, int kTiles>
-__global__ __launch_bounds__(64 * kDownWaves, kTiles == 4 ? 2 : 4)
+__global__ __launch_bounds__(64 * kDownWaves, 2 * kDownPlaces<kTiles>)
 void adapter_down_kernel(AdapterArgs a) {
   __shared__ f32x4 sums[kDownWaves][kTiles][64];
   const int lane = threadIdx.x & 63;
@@ -674,9 +675,10 @@ hipError_t launch_down(hipStream_t s, AdapterArgs& a) {
     splits *= 2;
   a.split_cols = 32 * (((a.cols + 31) / 32 + (int)splits - 1) / (int)splits);
   a.splits = (int)splits;
+  constexpr uint32_t kMost = 256 * kDownPlaces<kTiles>;
   const uint64_t items = (uint64_t)((a.tokens + 7) / 8 * 8) * groups * splits;
   hipLaunchKernelGGL((adapter_down_kernel<kFormat, kTiles>),
-                     dim3((uint32_t)(items < kMostDown ? items : kMostDown)),
+                     dim3((uint32_t)(items < kMost ? items : kMost)),
                      dim3(64 * kDownWaves), 0, s, a);
   return hipGetLastError();
 }
