@@ -129,6 +129,7 @@ _S = ctypes.c_char_p
 _SIGS = {
     "frz_last_error": (ctypes.c_char_p, []),
     "frz_open": (c_int, [c_int, POINTER(c_void_p), POINTER(Limits)]),
+    "frz_open_on": (c_int, [c_int, c_void_p, POINTER(c_void_p), POINTER(Limits)]),
     "frz_close": (None, [_P]),
     "frz_sync": (c_int, [_P]),
     "frz_alloc": (c_int, [_P, c_uint64, POINTER(c_void_p)]),

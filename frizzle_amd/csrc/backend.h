@@ -18,6 +18,7 @@ struct frz_device {
   int ordinal = 0;
   hipDeviceProp_t props{};
   hipStream_t stream = nullptr;
+  bool callers_stream = false;   // frz_open_on's, left as it is when the handle closes
   frz::DevStep* step = nullptr;  // the one-kernel ops' step record
   // This device's copy of the static decode-attention workspace (the
   // address hipGetSymbolAddress gave at frz_open, with this device current).
@@ -27,7 +28,8 @@ struct frz_device {
   // its free, which waits for the device, cost more than the selection.
   uint32_t* topk_scratch = nullptr;
   // The workspace of the ops over a batch of requests (batch_api.hip), there
-  // from the first of them on; their work, and so its use, is in stream order.
+  // from the first of them on (on a caller's stream from the start); their
+  // work, and so its use, is in stream order.
   void* batch_scratch = nullptr;
   // Held while a one-kernel op enqueues its launches, so that ops of several
   // threads run one after another: they share the stream and what is above.
@@ -40,6 +42,31 @@ namespace frz {
 int fail(int status, const std::string& message);
 // FRZ_OK, or FRZ_ERR_DEVICE with the HIP error's text.
 int check_hip(hipError_t e, const char* what);
+// The handle's device is the current one while this lives.
+class OnDevice {
+ public:
+  explicit OnDevice(int ordinal) {
+    error_ = hipGetDevice(&before_);
+    if (error_ == hipSuccess && before_ != ordinal) {
+      error_ = hipSetDevice(ordinal);
+      changed_ = error_ == hipSuccess;
+    }
+  }
+  ~OnDevice() {
+    if (changed_) (void)hipSetDevice(before_);
+  }
+  OnDevice(const OnDevice&) = delete;
+  OnDevice& operator=(const OnDevice&) = delete;
+  hipError_t error() const { return error_; }
+
+ private:
+  hipError_t error_;
+  int before_ = 0;
+  bool changed_ = false;
+};
+
+// The workspace of the ops over a batch of requests, made if it is not there.
+int device_batch_scratch(frz_device* dev);
 // Puts a step record without its ids on the device, in stream order.
 int device_put_step(frz_device* dev, const DevStep& s);
 // Copies a whole step record to the device and waits.

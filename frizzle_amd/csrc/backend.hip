@@ -140,6 +140,7 @@ namespace {
 // them - and the wait for it, with the lock given back.
 template <typename Launch>
 int run_op(frz_device* dev, const DevStep& s, const char* what, Launch launch) {
+  OnDevice on(dev->ordinal);
   hipError_t e;
   {
     std::lock_guard<std::mutex> lock(dev->ops);
@@ -175,52 +176,65 @@ extern "C" {
 
 const char* frz_last_error(void) { return g_last_error.c_str(); }
 
-int frz_open(int ordinal, frz_device** out, frz_limits* limits) {
-  if (!out) return fail(FRZ_ERR_ARGUMENT, "frz_open: null out");
+// A handle on a stream of its own, or (`on`) on the caller's `stream`.
+static int open_device(const char* what, int ordinal, bool on, hipStream_t stream,
+                       frz_device** out, frz_limits* limits) {
+  auto refuse = [what](int status, const char* why) {
+    return fail(status, std::string(what) + ": " + why);
+  };
+  if (!out) return refuse(FRZ_ERR_ARGUMENT, "null out");
   *out = nullptr;
+  // Every thread has another behind that name, and a handle's work is in one
+  // stream's order.
+  if (on && stream == hipStreamPerThread) return refuse(FRZ_ERR_ARGUMENT, "a stream a thread");
   int count = 0;
   if (hipGetDeviceCount(&count) != hipSuccess || count == 0) {
-    return fail(FRZ_ERR_DEVICE, "frz_open: no HIP device");
+    return refuse(FRZ_ERR_DEVICE, "no HIP device");
   }
-  if (ordinal < 0 || ordinal >= count) return fail(FRZ_ERR_ARGUMENT, "frz_open: no such device");
+  if (ordinal < 0 || ordinal >= count) return refuse(FRZ_ERR_ARGUMENT, "no such device");
   if (int rc = check_hip(hipSetDevice(ordinal), "hipSetDevice")) return rc;
   hipDeviceProp_t prop;
   if (int rc = check_hip(hipGetDeviceProperties(&prop, ordinal), "hipGetDeviceProperties")) return rc;
   if (std::strncmp(prop.gcnArchName, "gfx950", 6) != 0) {
-    return fail(FRZ_ERR_DEVICE, std::string("frz_open: built for gfx950, device is ") +
-                                    prop.gcnArchName);
+    return fail(FRZ_ERR_DEVICE,
+                std::string(what) + ": built for gfx950, device is " + prop.gcnArchName);
+  }
+  if (on && stream) {
+    hipDevice_t of = -1;
+    if (int rc = check_hip(hipStreamGetDevice(stream, &of), "hipStreamGetDevice")) return rc;
+    if (of != ordinal) return refuse(FRZ_ERR_ARGUMENT, "a stream of another device");
   }
   frz_device* dev = new frz_device();
   dev->ordinal = ordinal;
   dev->props = prop;
-  if (int rc = check_hip(hipStreamCreateWithFlags(&dev->stream, hipStreamNonBlocking),
-                         "hipStreamCreate")) {
+  dev->callers_stream = on;
+  auto bail = [dev](int rc) {
+    if (dev->batch_scratch) (void)hipFree(dev->batch_scratch);
+    if (dev->topk_scratch) (void)hipFree(dev->topk_scratch);
+    if (dev->step) (void)hipFree(dev->step);
+    if (dev->stream && !dev->callers_stream) (void)hipStreamDestroy(dev->stream);
     delete dev;
     return rc;
+  };
+  if (on) {
+    dev->stream = stream;
+    // Here and not in the first op, which the caller may capture.
+    if (int rc = device_batch_scratch(dev)) return bail(rc);
+  } else if (int rc = check_hip(hipStreamCreateWithFlags(&dev->stream, hipStreamNonBlocking),
+                                "hipStreamCreate")) {
+    return bail(rc);
   }
-  if (int rc = check_hip(hipMalloc(&dev->step, sizeof(DevStep)), "hipMalloc(step)")) {
-    (void)hipStreamDestroy(dev->stream);
-    delete dev;
-    return rc;
-  }
+  if (int rc = check_hip(hipMalloc(&dev->step, sizeof(DevStep)), "hipMalloc(step)"))
+    return bail(rc);
   // This device's address of the static workspace (each device holds its own
   // copy of the array; the name itself is no device address on the host).
   void* workspace = nullptr;
   if (int rc = check_hip(hipGetSymbolAddress(&workspace, HIP_SYMBOL(scratch)),
-                         "hipGetSymbolAddress(scratch)")) {
-    (void)hipFree(dev->step);
-    (void)hipStreamDestroy(dev->stream);
-    delete dev;
-    return rc;
-  }
+                         "hipGetSymbolAddress(scratch)"))
+    return bail(rc);
   dev->static_workspace = static_cast<float*>(workspace);
-  if (int rc = check_hip(hipMalloc(&dev->topk_scratch, kTopkScratchWords * 4),
-                         "hipMalloc(topk)")) {
-    (void)hipFree(dev->step);
-    (void)hipStreamDestroy(dev->stream);
-    delete dev;
-    return rc;
-  }
+  if (int rc = check_hip(hipMalloc(&dev->topk_scratch, kTopkScratchWords * 4), "hipMalloc(topk)"))
+    return bail(rc);
   if (limits) {
     std::memset(limits, 0, sizeof *limits);
     std::strncpy(limits->name, prop.gcnArchName, sizeof(limits->name) - 1);
@@ -232,6 +246,14 @@ int frz_open(int ordinal, frz_device** out, frz_limits* limits) {
   return FRZ_OK;
 }
 
+int frz_open(int ordinal, frz_device** out, frz_limits* limits) {
+  return open_device("frz_open", ordinal, false, nullptr, out, limits);
+}
+
+int frz_open_on(int ordinal, void* stream, frz_device** out, frz_limits* limits) {
+  return open_device("frz_open_on", ordinal, true, static_cast<hipStream_t>(stream), out, limits);
+}
+
 void frz_close(frz_device* dev) {
   if (!dev) return;
   (void)hipSetDevice(dev->ordinal);
@@ -239,11 +261,12 @@ void frz_close(frz_device* dev) {
   if (dev->batch_scratch) (void)hipFree(dev->batch_scratch);
   (void)hipFree(dev->topk_scratch);
   (void)hipFree(dev->step);
-  (void)hipStreamDestroy(dev->stream);
+  if (!dev->callers_stream) (void)hipStreamDestroy(dev->stream);
   delete dev;
 }
 
 int frz_sync(frz_device* dev) {
+  OnDevice on(dev->ordinal);  // a default stream is the current device's
   return check_hip(hipStreamSynchronize(dev->stream), "hipStreamSynchronize");
 }
 
@@ -259,6 +282,7 @@ int frz_free(frz_device* dev, void* dev_ptr) {
 }
 
 int frz_write(frz_device* dev, void* dev_dst, const void* host_src, uint64_t bytes) {
+  OnDevice on(dev->ordinal);
   if (int rc = check_hip(hipMemcpyAsync(dev_dst, host_src, bytes, hipMemcpyHostToDevice,
                                         dev->stream),
                          "hipMemcpyAsync(H2D)"))
@@ -267,6 +291,7 @@ int frz_write(frz_device* dev, void* dev_dst, const void* host_src, uint64_t byt
 }
 
 int frz_read(frz_device* dev, void* host_dst, const void* dev_src, uint64_t bytes) {
+  OnDevice on(dev->ordinal);
   if (int rc = check_hip(hipMemcpyAsync(host_dst, dev_src, bytes, hipMemcpyDeviceToHost,
                                         dev->stream),
                          "hipMemcpyAsync(D2H)"))
@@ -275,6 +300,7 @@ int frz_read(frz_device* dev, void* host_dst, const void* dev_src, uint64_t byte
 }
 
 int frz_fill_zero(frz_device* dev, void* dev_dst, uint64_t bytes) {
+  OnDevice on(dev->ordinal);
   if (int rc = check_hip(hipMemsetAsync(dev_dst, 0, bytes, dev->stream), "hipMemsetAsync"))
     return rc;
   return frz_sync(dev);
@@ -604,6 +630,7 @@ int frz_op_gather_format(frz_device* dev, int format, const void* codes, const v
   }
   DevStep s = host_step(0, tokens);
   std::memcpy(s.ids, ids, tokens * sizeof(uint32_t));
+  OnDevice on(dev->ordinal);
   hipError_t e;
   {
     // As run_op, with the record's ids.
@@ -627,6 +654,7 @@ int frz_op_edit(frz_device* dev, const uint32_t* edits_dev, int layer, float* ac
 
 int frz_op_topk(frz_device* dev, const float* logits, int count, uint32_t* candidates_dev) {
   if (count < kCandidates) return fail(FRZ_ERR_ARGUMENT, "frz_op_topk: fewer than 64 logits");
+  OnDevice on(dev->ordinal);
   const size_t words = topk_scratch_words(count);
   if (words <= kTopkScratchWords) {
     // The device's own: calls from several threads enqueue whole selections
@@ -661,6 +689,7 @@ int frz_op_draw(frz_device* dev, const uint32_t* candidates_dev, const frz_sampl
 
 int frz_op_numerics(frz_device* dev, int which, const float* in_dev, float* out_dev, int n) {
   if (n <= 0) return fail(FRZ_ERR_ARGUMENT, "frz_op_numerics: n <= 0");
+  OnDevice on(dev->ordinal);
   hipLaunchKernelGGL(numerics_kernel, dim3((n + 255) / 256), dim3(256), 0, dev->stream, which,
                      in_dev, out_dev, n);
   return device_finish(dev, hipGetLastError(), "frz_op_numerics");
@@ -677,6 +706,7 @@ namespace frz {
 template <typename Launch>
 static int bench_graph(frz_device* dev, int copies, int iters, int graph_mode, Launch launch,
                        const char* what, double* us_per_launch) {
+  OnDevice on(dev->ordinal);
   hipStream_t s = dev->stream;
   for (int i = 0; i < copies; ++i) {  // warm: every copy once
     if (int rc = check_hip(launch(i), what)) return rc;
@@ -737,6 +767,7 @@ int frz_bench_gemv(frz_device* dev, const void* const* codes, const void* const*
   }
   // The timed launches all read the device's step record.
   std::lock_guard<std::mutex> lock(dev->ops);
+  OnDevice on(dev->ordinal);
   if (int rc = device_put_step(dev, host_step(0, 1))) return rc;
   return bench_graph(dev, copies, iters, graph, [&](int c) {
     return launch_gemv(dev->stream, dev->step, q4(codes[c], scales[c], rows, cols), x, cols, y,
@@ -753,6 +784,7 @@ int frz_bench_gated(frz_device* dev, const void* const* gate_codes,
   }
   // The timed launches all read the device's step record.
   std::lock_guard<std::mutex> lock(dev->ops);
+  OnDevice on(dev->ordinal);
   if (int rc = device_put_step(dev, host_step(0, 1))) return rc;
   return bench_graph(dev, copies, iters, graph, [&](int c) {
     return launch_gated(dev->stream, dev->step, q4(gate_codes[c], gate_scales[c], rows, cols),
@@ -788,6 +820,7 @@ int frz_bench_stream(frz_device* dev, const void* const* buffers, int copies, ui
 
 int frz_copy(frz_device* dev, void* dev_dst, const void* dev_src, uint64_t bytes) {
   if (!dev || (bytes && (!dev_dst || !dev_src))) return fail(FRZ_ERR_ARGUMENT, "frz_copy: null");
+  OnDevice on(dev->ordinal);
   return device_finish(
       dev, hipMemcpyAsync(dev_dst, dev_src, bytes, hipMemcpyDeviceToDevice, dev->stream),
       "frz_copy");

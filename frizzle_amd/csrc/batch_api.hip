@@ -28,29 +28,6 @@ constexpr float kMostScale = 4096.0f;  // 2^13 in log2 units, as the kernel take
 bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 bool aligned_word(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
 
-// The handle's device is the current one while this lives.
-class OnDevice {
- public:
-  explicit OnDevice(int ordinal) {
-    error_ = hipGetDevice(&before_);
-    if (error_ == hipSuccess && before_ != ordinal) {
-      error_ = hipSetDevice(ordinal);
-      changed_ = error_ == hipSuccess;
-    }
-  }
-  ~OnDevice() {
-    if (changed_) (void)hipSetDevice(before_);
-  }
-  OnDevice(const OnDevice&) = delete;
-  OnDevice& operator=(const OnDevice&) = delete;
-  hipError_t error() const { return error_; }
-
- private:
-  hipError_t error_;
-  int before_ = 0;
-  bool changed_ = false;
-};
-
 // Enqueues one op with the lock held and the workspace there; nothing throws
 // past it.
 template <typename Launch>
@@ -59,12 +36,7 @@ int enqueue(frz_device* dev, const char* what, Launch launch) {
     OnDevice on(dev->ordinal);
     if (on.error() != hipSuccess) return check_hip(on.error(), what);
     std::lock_guard<std::mutex> lock(dev->ops);
-    if (!dev->batch_scratch) {
-      if (int rc = check_hip(hipMalloc(&dev->batch_scratch, kScratchBytes), what)) {
-        dev->batch_scratch = nullptr;
-        return rc;
-      }
-    }
+    if (int rc = device_batch_scratch(dev)) return rc;
     return check_hip(launch(), what);
   } catch (const std::exception& e) {
     return fail(FRZ_ERR_DEVICE, std::string(what) + ": " + e.what());
@@ -119,6 +91,14 @@ int refuse(const char* what, const char* why) {
 bool stride_ok(int stride, int64_t width) { return stride % 4 == 0 && stride >= width; }
 
 }  // namespace
+
+int device_batch_scratch(frz_device* dev) {
+  if (dev->batch_scratch) return FRZ_OK;
+  const int rc = check_hip(hipMalloc(&dev->batch_scratch, kScratchBytes), "hipMalloc(batch)");
+  if (rc != FRZ_OK) dev->batch_scratch = nullptr;
+  return rc;
+}
+
 }  // namespace frz
 
 using namespace frz;

@@ -947,6 +947,11 @@ QMatrix matrix_at(uint8_t* at, int rows, int cols, int format) {
 // buffers it names), or with every buffer its own allocation.
 int create_model(frz_device* dev, const frz_model_config& c, const frz_plan* plan,
                  frz_model** out) {
+  if (dev->callers_stream) {
+    return fail(FRZ_ERR_ARGUMENT,
+                "frz_model_create: a handle on a caller's stream (a model's steps are captured, on "
+                "a stream of the handle's own)");
+  }
   // The kernels are built for Gemma-3's attention shape (d = 256, four query
   // heads on one key-value head), rows the norm prologues take (hidden at most
   // 2,048) and contexts up to the trained 32,768 tokens. A sliding ring holds

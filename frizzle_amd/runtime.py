@@ -214,14 +214,34 @@ def _launches(out, count):
              float(out[i].microseconds)) for i in range(count)]
 
 
-class Device:
-    """One GPU (frz_open). Raises when there is none."""
+def _hip_runtimes():
+    """The HIP runtimes that the process has loaded."""
+    with open("/proc/self/maps") as maps:
+        return {line.split()[-1] for line in maps if "libamdhip64.so" in line}
 
-    def __init__(self, ordinal=0):
+
+class Device:
+    """One GPU (frz_open). Raises when there is none.
+
+    `stream`: a stream of the caller's to work on, in order with what the caller
+    enqueues there (frz_open_on), as torch.cuda.current_stream().cuda_stream; 0
+    is the default stream. A stream belongs to one HIP runtime: torch brings its
+    own, which this library shares when torch is imported before it is loaded,
+    and a stream is refused where the process has two."""
+
+    def __init__(self, ordinal=0, stream=None):
         self.lib = load()
         h = c_void_p()
         self.limits = Limits()
-        check(self.lib.frz_open(ordinal, byref(h), byref(self.limits)))
+        if stream is None:
+            check(self.lib.frz_open(ordinal, byref(h), byref(self.limits)))
+        else:
+            runtimes = _hip_runtimes()
+            if len(runtimes) > 1:
+                raise _lib.FrzError(1, "Device: a stream, with two HIP runtimes in the process ("
+                                    + ", ".join(sorted(runtimes)) + "): import torch before the "
+                                    "library is loaded")
+            check(self.lib.frz_open_on(ordinal, stream, byref(h), byref(self.limits)))
         self.handle = h.value
 
     def array(self, array):

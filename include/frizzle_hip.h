@@ -10,9 +10,14 @@
  * plain pointers and sizes, an int status (0 = ok) and a thread-local message
  * from frz_last_error(). Nothing throws across this boundary.
  *
- * Device pointers ("dev") are addresses from frz_alloc on the same device.
- * Host pointers are ordinary memory. Unless stated, calls enqueue work on the
- * device's one stream and return without waiting; frz_sync waits.
+ * Device pointers ("dev") are addresses from frz_alloc on the same device, or
+ * from another allocator of the process's HIP runtime. Host pointers are
+ * ordinary memory. Unless stated, calls enqueue work on the handle's one
+ * stream and return without waiting; frz_sync waits. A handle's own stream is
+ * ordered with no other, the default one included: what other streams write
+ * must be there before a call that reads it, and what a call writes is there
+ * once frz_sync returns. frz_open_on's handle works on the caller's stream,
+ * in order with all that the caller enqueues there.
  */
 #ifndef FRIZZLE_HIP_H
 #define FRIZZLE_HIP_H
@@ -50,6 +55,16 @@ typedef struct frz_limits {
 } frz_limits;
 
 int frz_open(int ordinal, frz_device** out, frz_limits* limits);
+/* A handle whose work goes on `stream`, a hipStream_t of that device and of the
+ * HIP runtime that this library runs on (null: the device's default stream;
+ * not hipStreamPerThread, which is another in each thread). The stream must
+ * outlive the handle; frz_close waits for it and leaves it. Buffers and single
+ * kernels: a model captures its steps, and is refused (FRZ_ERR_ARGUMENT). The
+ * ops over a step of many requests, which allocate nothing on such a handle
+ * and never wait, may be captured into the caller's graphs: their pointers and
+ * sizes are the graph's, the workspace is the handle's, so replays must run in
+ * order with one another and with the handle's calls. */
+int frz_open_on(int ordinal, void* stream, frz_device** out, frz_limits* limits);
 void frz_close(frz_device* dev);
 int frz_sync(frz_device* dev);
 
