@@ -247,7 +247,9 @@ def run(s):
 @functools.lru_cache(None)
 def _frizzle():
     import frizzle_amd
-    return frizzle_amd, frizzle_amd._lib.check, frizzle_amd.load(), frizzle_amd.Device(0)
+    # On torch's stream: the calls read what torch writes there, and torch reads what they write.
+    device = frizzle_amd.Device(0, stream=torch.cuda.current_stream().cuda_stream)
+    return frizzle_amd, frizzle_amd._lib.check, frizzle_amd.load(), device
 
 
 def _pages(fz, s):
