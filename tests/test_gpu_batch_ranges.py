@@ -1,0 +1,30 @@
+"""The ops over requests at the ends of their operands' ranges, and beside
+values far larger than the ones that count, against values in 64 bits."""
+import numpy as np
+import pytest
+
+from _batch import BF16, NONE, Paged, check_attention, of_format, to_format
+
+pytestmark = pytest.mark.gpu
+
+
+def batch(device, seed, lengths, heads, kv, dim, fmt, **more):
+    rng = np.random.default_rng(seed)
+    paged = Paged(device, rng, lengths, kv, dim, 16, fmt, **more)
+    query = rng.normal(0, 1.0, (len(lengths), heads * dim)).astype(np.float32)
+    return paged, query, [n - 1 for n in lengths]
+
+
+# Ten thousand BF16 values near the type's largest (3.4e38), alike and of either
+# sign, whose weights are about the same: their sum is far out of F32's range, the
+# output, a mean of them, is in it.
+@pytest.mark.parametrize("heads,kv,dim", [(4, 1, 64), (16, 2, 128), (12, 1, 256)])
+@pytest.mark.parametrize("lengths", [[200, 31, 1], [10000, 700]])
+@pytest.mark.parametrize("spread", [0.1, 2.0])
+def test_sums_of_the_largest_values(device, heads, kv, dim, lengths, spread):
+    paged, query, positions = batch(device, dim, lengths, heads, kv, dim, BF16, scale=0.02)
+    values = of_format(paged.values, BF16) / 0.02
+    values = np.clip(2e38 * (1.0 if spread < 1 else 0.0) + 5e37 * spread * values, -3e38, 3e38)
+    paged.values[:] = to_format(values, BF16)
+    paged.upload()
+    check_attention(device, paged, positions, query, heads, NONE, dim ** -0.5)
