@@ -27,9 +27,10 @@
 // one head, W the next of 4, 8 or 16 above the heads. A head's query is
 // scaled by a power of two, for F16 to lie below 2^15, and weights by 2^14, so
 // that their low parts stay clear of the format's smallest values; for BF16,
-// whose range is F32's, the query lies below 2, so that large keys' products
-// stay in range, and weights are at most 2^-24, so that no sum of finite values
-// leaves it. Both scales are exact, products are exact in F32, sums F32.
+// whose range is F32's, the query lies below 2^-8 (one past 2^104 2^113 below
+// itself) and weights are at most 2^-24, so that no sum of finite keys' or
+// values' products leaves it where scores do not. Both scales are exact,
+// products are exact in F32, sums F32.
 //
 // Keys outside the row's range or in no page are never read: their rows are
 // zeros, and their scores -inf.
@@ -78,7 +79,7 @@ struct Types<true> {
   typedef bf16x8 vec;
   typedef __bf16 scalar;
   static constexpr int kParts = 3;
-  static constexpr int kQueryTop = 0;
+  static constexpr int kQueryTop = -9;            // the sum of 256 products of any key is finite
   static constexpr float kWeightScale = -24.0f;  // the sum of 2^24 such weights of any value is finite
   static __device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),

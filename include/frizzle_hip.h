@@ -281,8 +281,8 @@ int frz_op_rope_paged(frz_device* dev, const frz_pages* cache, const uint32_t* s
  * position], its own among them (window at least 1; 0xFFFFFFFF: all): query
  * head i reads key-value head i / (query_heads / kv_heads). Scores are scale
  * (at most 4,096 either side of zero) times the products. Within about 1e-6 of
- * the exact sums, not the reference's order, where products stay in F32's
- * range. A row with no key gets zeros. Cached values must be
+ * the exact sums, not the reference's order, where scores, before scale and after, stay in
+ * F32's range. A row with no key gets zeros. Cached values must be
  * finite where a row reads them, and may be anything elsewhere. out's rows are
  * out_stride floats apart; out must not overlap query. */
 int frz_op_attention_paged(frz_device* dev, const frz_pages* cache, const uint32_t* sequences,

@@ -28,3 +28,14 @@ def test_sums_of_the_largest_values(device, heads, kv, dim, lengths, spread):
     paged.values[:] = to_format(values, BF16)
     paged.upload()
     check_attention(device, paged, positions, query, heads, NONE, dim ** -0.5)
+
+
+# Small queries over BF16 keys near the type's largest (3.4e38): products and
+# their sums fit F32, though those of a query of ordinary size would not.
+@pytest.mark.parametrize("heads,kv,dim", [(4, 1, 64), (8, 1, 128), (16, 1, 256), (3, 3, 256)])
+@pytest.mark.parametrize("query_scale", [1e-3, 1e-20, 1e-37])
+def test_small_queries_over_the_largest_keys(device, heads, kv, dim, query_scale):
+    paged, query, positions = batch(device, dim, [150, 33, 1], heads, kv, dim, BF16, scale=6e37)
+    query = (query * query_scale).astype(np.float32)
+    check_attention(device, paged, positions, query, heads, NONE,
+                    1 / (dim ** 0.5 * query_scale * 6e37))
