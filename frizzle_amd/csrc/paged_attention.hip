@@ -22,15 +22,20 @@
 //
 // The matrix cores take 16-bit operands, the cache's type; the query and the
 // weights are F32. Each is split into parts that add up to it, hi + lo of F16
-// (to 2^-22) or three of BF16 (2^-24), which are further columns of the same
-// instruction where the heads leave some free: columns n and n + W belong to
-// one head, W the next of 4, 8 or 16 above the heads. A head's query is
-// scaled by a power of two, for F16 to lie below 2^15, and weights by 2^14, so
-// that their low parts stay clear of the format's smallest values; for BF16,
-// whose range is F32's, the query lies below 2^-8 (one past 2^104 2^113 below
-// itself) and weights are at most 2^-24, so that no sum of finite keys' or
-// values' products leaves it where scores do not. Both scales are exact,
-// products are exact in F32, sums F32.
+// (to one F32 ulp, 2^-23) or three of BF16 (all 24 bits), which are further
+// columns of the same instruction where the heads leave some free: columns n and
+// n + W belong to one head, W the next of 4, 8 or 16 above the heads. A third
+// part of F16 had cost 61 requests of 40 to 8,192 keys 23.2 -> 24.9 us, groups of
+// 16 heads up to 19%, for that last ulp, which is less than the scores' sums
+// round. A head's query is scaled by a power of two, for F16 to lie below 2^15,
+// and its low part by 2^12 more, which that column's scores are divided by: a
+// value down to 2^-28 of the head's largest is held to its ulp, and one below
+// to 2^-51 of that (as it was, rounded by F16's smallest values to 2^-40). Weights
+// are 2^14 at the running maximum, for the same reason, and held to 2^-39 of it.
+// For BF16, whose range is F32's, the query lies below 2^-8 (one past 2^104 2^113
+// below itself) and weights are at most 2^-24, so that no sum of finite keys' or
+// values' products leaves it where scores do not. All scales are exact, products
+// are exact in F32, sums F32.
 //
 // Keys outside the row's range or in no page are never read: their rows are
 // zeros, and their scores -inf.
@@ -68,6 +73,7 @@ struct Types<false> {
   typedef _Float16 scalar;
   static constexpr int kParts = 2;
   static constexpr int kQueryTop = 14;          // the query's largest lies in [2^14, 2^15)
+  static constexpr float kPartScale = 4096.0f;  // of a query's part to the one before
   static constexpr float kWeightScale = 14.0f;  // the running maximum's weight: 2^14
   static __device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a),
@@ -79,7 +85,8 @@ struct Types<true> {
   typedef bf16x8 vec;
   typedef __bf16 scalar;
   static constexpr int kParts = 3;
-  static constexpr int kQueryTop = -9;            // the sum of 256 products of any key is finite
+  static constexpr int kQueryTop = -9;  // the sum of 256 products of any key is finite
+  static constexpr float kPartScale = 1.0f;
   static constexpr float kWeightScale = -24.0f;  // the sum of 2^24 such weights of any value is finite
   static __device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
@@ -93,6 +100,8 @@ struct Shape {
   static constexpr int kParts = Types<kBf16>::kParts;
   static constexpr int kPerTile = 16 / kW;                              // parts a column tile holds
   static constexpr int kTiles = (kParts + kPerTile - 1) / kPerTile;     // column tiles
+  // Tiles whose query is not scaled alike, and so whose sums are apart.
+  static constexpr int kScales = kBf16 ? 1 : kTiles;
   static constexpr bool kSpare = kTiles * kPerTile > kParts;            // columns of no part
   static constexpr int kChunks = kD / 32;                               // of a key row
   static constexpr int kVec = kD >= 128 ? 8 : 4;                        // values a lane loads at once
@@ -114,17 +123,24 @@ template <bool kBf16>
 struct Column {
   float keep;     // 1; 0 for a column past the format's parts
   float less[2];
+  float scale;    // of a query's part
   Column() = default;
   __device__ __forceinline__ explicit Column(int part) {
     keep = part < Types<kBf16>::kParts ? 1.0f : 0.0f;
     less[0] = part >= 1 ? -1.0f : 0.0f;
     less[1] = part >= 2 ? -1.0f : 0.0f;
+    scale = !kBf16 && part == 1 ? Types<kBf16>::kPartScale : 1.0f;
   }
   __device__ __forceinline__ typename Types<kBf16>::scalar part_of(float x) const {
     typedef typename Types<kBf16>::scalar T;
     x = fmaf_(less[0], (float)(T)x, x);
     if constexpr (kBf16) x = fmaf_(less[1], (float)(T)x, x);
     return (T)x;
+  }
+  __device__ __forceinline__ typename Types<kBf16>::scalar scaled_part_of(float x) const {
+    typedef typename Types<kBf16>::scalar T;
+    if constexpr (kBf16) return part_of(x);
+    return (T)(fmaf_(less[0], (float)(T)x, x) * scale);
   }
 };
 
@@ -443,7 +459,7 @@ void paged_attention_kernel(PagedAttentionArgs a) {
     load_keys(now);
     load_values(now);
     hold();
-    float scale;  // what turns the scaled query's products into log2 units
+    float scale[S::kTiles];  // what turns the scaled query's products into log2 units
     uint4 q[S::kTiles][S::kChunks];
     {
       float most = 0.0f;
@@ -458,29 +474,33 @@ void paged_attention_kernel(PagedAttentionArgs a) {
       int up = 127 + T::kQueryTop - (int)(float_to_bits(most) >> 23);
       up = up > 100 ? 100 : up < -113 ? -113 : up;
       const float factor = bits_to_float((uint32_t)(127 + up) << 23);
-      scale = a.scale_log2e * bits_to_float((uint32_t)(127 - up) << 23);
+      const float back = a.scale_log2e * bits_to_float((uint32_t)(127 - up) << 23);
 #pragma unroll
       for (int t = 0; t < S::kTiles; ++t) {
+        scale[t] = back / columns[t].scale;
         const float kept = factor * columns[t].keep;
 #pragma unroll
         for (int c = 0; c < S::kChunks; ++c) {
           typename T::vec v;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = columns[t].part_of(x[c][i] * kept);
+          for (int i = 0; i < 8; ++i) v[i] = columns[t].scaled_part_of(x[c][i] * kept);
           q[t][c] = __builtin_bit_cast(uint4, v);
         }
       }
     }
     for (bool more = true; more;) {
-      f32x4 scores[2];
+      f32x4 scores[2][S::kScales];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        scores[h] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < S::kScales; ++i) scores[h][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int c = 0; c < S::kChunks; ++c)
 #pragma unroll
-          for (int t = 0; t < S::kTiles; ++t)
-            scores[h] = T::mfma(key_rows[h][c], q[t][c], scores[h]);
+          for (int t = 0; t < S::kTiles; ++t) {
+            f32x4& sum = scores[h][t % S::kScales];
+            sum = T::mfma(key_rows[h][c], q[t][c], sum);
+          }
       }
       hold();
       // After the last block, of no rows: a branch around the loads would make
@@ -491,15 +511,18 @@ void paged_attention_kernel(PagedAttentionArgs a) {
       load_keys(next);
       hold();
 
-      float most = kMinusInf;
+      float most = kMinusInf, weight[8];  // scores first
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float s = across_columns<kW>(scores[h][e]) * scale;
+          float s = scores[h][0][e] * scale[0];
+#pragma unroll
+          for (int i = 1; i < S::kScales; ++i) s = fmaf_(scores[h][i][e], scale[i], s);
+          s = across_columns<kW>(s);
           const bool live = 4 * g + e >= now.lo[h] && 4 * g + e < now.hi[h];
-          scores[h][e] = live ? s : kMinusInf;
-          most = __builtin_fmaxf(most, scores[h][e]);
+          weight[4 * h + e] = live ? s : kMinusInf;
+          most = __builtin_fmaxf(most, weight[4 * h + e]);
         }
       most = across_groups(most, [](float p, float r) { return __builtin_fmaxf(p, r); });
       // A block that is worked on holds a key, so `most` is a number but where
@@ -514,10 +537,9 @@ void paged_attention_kernel(PagedAttentionArgs a) {
           for (int j = 0; j < S::kVec; ++j) out[s][j] *= old;
         m = to;
       }
-      float weight[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        weight[i] = __builtin_amdgcn_exp2f(scores[i >> 2][i & 3] - m);
+        weight[i] = __builtin_amdgcn_exp2f(weight[i] - m);
         l += weight[i];
       }
       uint4 w[S::kTiles];

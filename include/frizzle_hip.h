@@ -280,9 +280,13 @@ int frz_op_rope_paged(frz_device* dev, const frz_pages* cache, const uint32_t* s
 /* Each row's attention over the keys of its request at (position - window,
  * position], its own among them (window at least 1; 0xFFFFFFFF: all): query
  * head i reads key-value head i / (query_heads / kv_heads). Scores are scale
- * (at most 4,096 either side of zero) times the products. Within about 1e-6 of
- * the exact sums, not the reference's order, where scores, before scale and after, stay in
- * F32's range. A row with no key gets zeros. Cached values must be
+ * (at most 4,096 either side of zero) times the products, and must stay in
+ * F32's range, as they must before scale. Sums are F32, not in the reference's
+ * order, over keys and values as they are and a query of 24 bits (BF16 caches)
+ * or to 2^-23 of itself, or 2^-51 of its head's largest (F16): a score is off by
+ * some 2^-22 of the sum of its products' sizes, and an output by twice as much of
+ * the largest value that is read as its scores are off, and by 1e-6 of it.
+ * A row with no key gets zeros. Cached values must be
  * finite where a row reads them, and may be anything elsewhere. out's rows are
  * out_stride floats apart; out must not overlap query. */
 int frz_op_attention_paged(frz_device* dev, const frz_pages* cache, const uint32_t* sequences,

@@ -3,7 +3,7 @@ values far larger than the ones that count, against values in 64 bits."""
 import numpy as np
 import pytest
 
-from _batch import BF16, NONE, Paged, check_attention, of_format, to_format
+from _batch import BF16, F16, NONE, Paged, check_attention, of_format, to_format
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +39,17 @@ def test_small_queries_over_the_largest_keys(device, heads, kv, dim, query_scale
     query = (query * query_scale).astype(np.float32)
     check_attention(device, paged, positions, query, heads, NONE,
                     1 / (dim ** 0.5 * query_scale * 6e37))
+
+
+# One dimension of the query far above all others, over keys that are zero there:
+# it counts for nothing, and costs the others none of their bits.
+@pytest.mark.parametrize("fmt", [F16, BF16])
+@pytest.mark.parametrize("heads,kv,dim", [(4, 1, 256), (3, 3, 64), (8, 1, 128), (12, 1, 64),
+                                          (16, 1, 256)])
+@pytest.mark.parametrize("times", [2.0 ** 24, 2.0 ** 29])
+def test_a_query_beside_a_dimension_of_no_key(device, fmt, heads, kv, dim, times):
+    paged, query, positions = batch(device, heads, [150, 700, 1], heads, kv, dim, fmt)
+    query.reshape(3, heads, dim)[:, :, dim // 3] *= times
+    paged.keys[..., dim // 3] = 0
+    paged.upload()
+    check_attention(device, paged, positions, query, heads, NONE, dim ** -0.5, near=2e-6)
