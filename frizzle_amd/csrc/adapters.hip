@@ -257,8 +257,9 @@ __device__ __forceinline__ void low_rank(const AdapterArgs& a, const Run& run, i
       }
       most = __builtin_fmaxf(most, __shfl_xor(most, 16));
       most = __builtin_fmaxf(most, __shfl_xor(most, 32));
+      // To 2^126, which keeps all of F32's smallest values.
       int up = 141 - (int)(float_to_bits(most) >> 23);
-      up = up > 100 ? 100 : up;
+      up = up > 126 ? 126 : up;
       factor = bits_to_float((uint32_t)(127 + up) << 23);
       back = bits_to_float((uint32_t)(127 - up) << 23);
 #pragma unroll

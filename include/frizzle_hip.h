@@ -313,7 +313,8 @@ typedef struct frz_adapters {
  * most 512 tokens: beside a product that all tokens share, whose output is
  * base. y may be base itself, with its stride; otherwise no two of x, base
  * and y may overlap. Sums are in F32; with F16 weights an x counts to 2^-22 of
- * itself, or 2^-40 of the token's largest. */
+ * itself, or 2^-40 of the token's largest, and with any weights an x or a low-rank
+ * sum to 2^-134 at least. */
 int frz_op_adapters(frz_device* dev, const frz_adapters* adapters, const uint32_t* which,
                     const float* x, int x_stride, const float* base, int base_stride, float* y,
                     int y_stride, uint32_t tokens);

@@ -3,7 +3,8 @@ values far larger than the ones that count, against values in 64 bits."""
 import numpy as np
 import pytest
 
-from _batch import BF16, F16, NONE, Paged, check_attention, of_format, to_format
+from _batch import (BF16, F16, F32, NONE, Paged, Pool, check_adapters, check_attention, of_format,
+                    to_format)
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +54,36 @@ def test_a_query_beside_a_dimension_of_no_key(device, fmt, heads, kv, dim, times
     paged.keys[..., dim // 3] = 0
     paged.upload()
     check_attention(device, paged, positions, query, heads, NONE, dim ** -0.5, near=2e-6)
+
+
+# Calls by tokens, and over runs of 16, 32 and 64: one and two tiles of ranks a
+# workgroup, and four over long rows of 16-bit weights.
+SHAPES = pytest.mark.parametrize("tokens,rank,cols,rows", [
+    (20, 16, 264, 500), (300, 16, 20008, 515), (333, 64, 1152, 3001), (300, 40, 6920, 515),
+    (511, 128, 200, 2300), (512, 64, 264, 4200)])
+
+
+def adapters_of(device, rng, fmt, tokens, rank, cols, rows):
+    pool = Pool(device, rng, 2, rank, cols, rows, fmt)
+    # A column that no adapter takes.
+    pool.down[:, :, 3] = 0
+    pool.dev[0] = device.array(pool.down)
+    which = [int(i) for i in np.sort(rng.integers(0, 2, tokens))]
+    return pool, which, rng.normal(0, 1, (tokens, cols)).astype(np.float32)
+
+
+# Small tokens keep their bits in every form. Parts of BF16, of x over BF16 weights
+# and of the low-rank sums over all, end at 2^-134, so that 2^-23 of 2^-103 (1e-31)
+# is still held, and of the low-rank sums of 1e-36 with weights 1,024 times as large
+# as 1 / sqrt(cols), about 2^-110.
+@pytest.mark.parametrize("fmt,size", [(F32, 1e-31), (BF16, 1e-28), (BF16, 1e-31), (F16, 1e-28),
+                                      (F16, 1e-31), (F16, 1e-36)])
+@SHAPES
+def test_the_smallest_tokens(device, fmt, tokens, rank, cols, rows, size):
+    rng = np.random.default_rng(rows)
+    pool, which, x = adapters_of(device, rng, fmt, tokens, rank, cols, rows)
+    for i, w in enumerate((pool.down, pool.up)):
+        w[:] = to_format(of_format(w, fmt) * 1024, fmt)
+        pool.dev[i] = device.array(w)
+    check_adapters(device, pool, which, (x * size).astype(np.float32),
+                   np.zeros((tokens, rows), np.float32), near=1e-6)
