@@ -12,7 +12,7 @@
 // The products of runs are on the matrix cores: with 16-bit weights, and U's of
 // long runs with F32 ones, of parts of 16 bits that add up to the operands, else
 // F32's own (v_mfma_f32_16x16x4_f32). Sums are F32 in both forms, and nothing is
-// rounded to less than 22 bits. The weights are the instruction's A operand, 16
+// rounded to less than F32's 24 bits. The weights are the instruction's A operand, 16
 // rows of as many columns as it takes: lane (m, g) holds 8 columns of row m as
 // they lie in memory, and of F32's eight instructions the j-th takes the j-th of
 // each. Loads are a step ahead of the products, and all of a step's loads are
@@ -73,13 +73,12 @@ struct Raw {
   }
 };
 
-// F32 values as parts of 16 bits that add up to them (three of BF16 hold F32's
-// 24 bits and its exponents, two of F16 22 bits), each what rounding left to the
-// parts before.
+// F32 values as parts of BF16 that add up to them (three hold F32's 24 bits and
+// its exponents), each what rounding left to the parts before.
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-template <typename T, typename Part, int kParts>
-__device__ __forceinline__ void split8(const float (&x)[8], Part (&part)[kParts]) {
+template <int kParts>
+__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&part)[kParts]) {
   float rest[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) rest[j] = x[j];
@@ -87,7 +86,7 @@ __device__ __forceinline__ void split8(const float (&x)[8], Part (&part)[kParts]
   for (int p = 0; p < kParts; ++p)
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      part[p][j] = (T)rest[j];
+      part[p][j] = (__bf16)rest[j];
       if (p + 1 < kParts) rest[j] -= (float)part[p][j];
     }
 }
@@ -205,14 +204,19 @@ __device__ __forceinline__ void copy_base(const AdapterArgs& a, uint32_t first, 
 }
 
 // Whether D's products are of parts of x on the 16-bit matrix cores, the
-// weights as they lie in memory: 2 instructions of 16 cycles for 32 columns
-// where F32's eight take 256 with F16 weights, 3 with BF16 ones. 512 tokens,
-// rank 32, 6,912 to 1,152, F16, of one adapter 15.4 -> 14.6 us a call, of one
-// each 114 -> 105; rank 128, 4,096 to 4,096, 300 of one each 172 -> 158. BF16's
-// parts hold all of x. F16's hold 22 bits of what is within 2^-16 or so of the
-// largest of a token's columns that a wave takes at once, below that 2^-40 of it.
+// weights as they lie in memory: 3 instructions of 16 cycles for 32 columns
+// where F32's eight take 256. 512 tokens, rank 32, 6,912 to 1,152, F16, of one
+// adapter 15.4 -> 14.6 us a call, of one each 114 -> 105; rank 128, 4,096 to
+// 4,096, 300 of one each 172 -> 158. Three parts hold all of x's 24 bits; those
+// of F16 down to 2^-28 of the largest of a token's columns that a wave takes at
+// once, and 2^-51 of it below: x is scaled, token by token, to lie below 2^15,
+// and the parts after the first by 2^12 more, in sums of their own, so that F16's
+// smallest values do not round them. (F16 weights as parts of BF16, for parts of
+// x that need no scale: 333 tokens of 3 adapters, rank 64, 6,912 to 1,152, 16.0 ->
+// 17.4 us, and 16.6 so; two parts of 23 bits 16.3.)
 template <int kFormat>
 constexpr bool kDownInParts = kFormat != 0;
+constexpr float kRestScale = 4096.0f;
 
 // A wave's share of D x for a run of up to 16 tokens, over the columns
 // [from, to) and kTiles tiles of 16 ranks from `rank0` on: every eighth 32 of
@@ -222,7 +226,7 @@ template <int kFormat, int kTiles>
 __device__ __forceinline__ void low_rank(const AdapterArgs& a, const Run& run, int rank0, int from,
                                          int to, int wave, int n, int g, f32x4 (&sum)[kTiles]) {
   // Steps whose loads are in flight at once.
-  constexpr int kDepth = kTiles == 1 ? 5 : kFormat == 0 ? 3 : 4;
+  constexpr int kDepth = kTiles == 1 ? 5 : kTiles == 2 && kFormat != 30 ? 3 : 4;
   Raw<0> x[kDepth];
   Raw<kFormat> w[kDepth][kTiles];
   const float* row =
@@ -242,11 +246,8 @@ __device__ __forceinline__ void low_rank(const AdapterArgs& a, const Run& run, i
         w[i][t].load(a.down,
                      pool + (uint64_t)min(rank0 + 16 * t + n, a.rank - 1) * (uint64_t)a.cols + k);
     }
-    // F16 parts of x scaled by a power of two, token by token, to lie below
-    // 2^15, so that the second ones stay clear of the format's smallest values.
     float factor = 1.0f, back = 1.0f;
-    f32x4 scaled[kTiles];
-    f32x4(&acc)[kTiles] = kFormat == 1 ? scaled : sum;
+    f32x4 scaled[2][kTiles];  // of F16 parts: the first's sums, the others'
     if constexpr (kFormat == 1) {
       float most = 0.0f;
 #pragma unroll
@@ -263,7 +264,7 @@ __device__ __forceinline__ void low_rank(const AdapterArgs& a, const Run& run, i
       factor = bits_to_float((uint32_t)(127 + up) << 23);
       back = bits_to_float((uint32_t)(127 - up) << 23);
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t) scaled[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int t = 0; t < kTiles; ++t) scaled[0][t] = scaled[1][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 #pragma unroll
     for (int i = 0; i < kDepth; ++i) {
@@ -277,23 +278,28 @@ __device__ __forceinline__ void low_rank(const AdapterArgs& a, const Run& run, i
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) weight[t] = in ? w[i][t].r[0] : make_uint4(0, 0, 0, 0);
         if constexpr (kFormat == 1) {
-          half8 part[2];
-          split8<_Float16>(xs, part);
 #pragma unroll
-          for (int p = 1; p >= 0; --p)
+          for (int p = 0; p < 3; ++p) {
+            half8 part;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              part[j] = (_Float16)xs[j];
+              if (p < 2) xs[j] = (xs[j] - (float)part[j]) * (p == 0 ? kRestScale : 1.0f);
+            }
 #pragma unroll
             for (int t = 0; t < kTiles; ++t)
-              acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                  __builtin_bit_cast(half8, weight[t]), part[p], acc[t], 0, 0, 0);
+              scaled[p > 0][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                  __builtin_bit_cast(half8, weight[t]), part, scaled[p > 0][t], 0, 0, 0);
+          }
         } else {
           bf16x8 part[3];
-          split8<__bf16>(xs, part);
+          split8(xs, part);
 #pragma unroll
           for (int p = 2; p >= 0; --p)
 #pragma unroll
             for (int t = 0; t < kTiles; ++t)
-              acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                  __builtin_bit_cast(bf16x8, weight[t]), part[p], acc[t], 0, 0, 0);
+              sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                  __builtin_bit_cast(bf16x8, weight[t]), part[p], sum[t], 0, 0, 0);
         }
       } else {
 #pragma unroll
@@ -301,14 +307,15 @@ __device__ __forceinline__ void low_rank(const AdapterArgs& a, const Run& run, i
           const float xj = in ? x[i].at(j) : 0.0f;
 #pragma unroll
           for (int t = 0; t < kTiles; ++t)
-            acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(in ? w[i][t].at(j) : 0.0f, xj, acc[t],
+            sum[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(in ? w[i][t].at(j) : 0.0f, xj, sum[t],
                                                           0, 0, 0);
         }
       }
     }
     if constexpr (kFormat == 1)
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t) sum[t] += scaled[t] * back;
+      for (int t = 0; t < kTiles; ++t)
+        sum[t] += (scaled[0][t] + scaled[1][t] * (1 / kRestScale)) * back;
   }
 }
 
@@ -490,7 +497,7 @@ __global__ __launch_bounds__(64 * kUpWaves, kUpPlaces<kRun>) void adapter_up_ker
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           weight[i][j] = 32 * c + 8 * g + j < rank ? w[c & 1][i].at(j) : 0.0f;
-        if constexpr (kInParts) split8<__bf16>(weight[i], part[i]);
+        if constexpr (kInParts) split8(weight[i], part[i]);
       }
 #pragma unroll
       for (int t = 0; t < kRunTiles; ++t) {

@@ -312,9 +312,9 @@ typedef struct frz_adapters {
  * token (FRZ_NO_ADAPTER, or any number from `count` on: y[t] = base[t]), at
  * most 512 tokens: beside a product that all tokens share, whose output is
  * base. y may be base itself, with its stride; otherwise no two of x, base
- * and y may overlap. Sums are in F32; with F16 weights an x counts to 2^-22 of
- * itself, or 2^-40 of the token's largest, and with any weights an x or a low-rank
- * sum to 2^-134 at least. */
+ * and y may overlap. Sums are in F32, of x and weights as they are, but that an x
+ * counts to 2^-51 of the token's largest at least with F16 weights, and an x or a
+ * low-rank sum to 2^-134 with any. */
 int frz_op_adapters(frz_device* dev, const frz_adapters* adapters, const uint32_t* which,
                     const float* x, int x_stride, const float* base, int base_stride, float* y,
                     int y_stride, uint32_t tokens);

@@ -72,6 +72,19 @@ def adapters_of(device, rng, fmt, tokens, rank, cols, rows):
     return pool, which, rng.normal(0, 1, (tokens, cols)).astype(np.float32)
 
 
+# The column far above a token's others costs them none of their bits. A value of
+# the others that is 2^-20 of them is off by 2^-51 of the column at most, which is
+# 2^-23 of the others' size, as F32's own roundings of their sum are.
+@pytest.mark.parametrize("fmt", [F32, F16, BF16])
+@SHAPES
+@pytest.mark.parametrize("times", [2.0 ** 20, 2.0 ** 24, 2.0 ** 28])
+def test_tokens_beside_a_column_of_no_weight(device, fmt, tokens, rank, cols, rows, times):
+    rng = np.random.default_rng(rows)
+    pool, which, x = adapters_of(device, rng, fmt, tokens, rank, cols, rows)
+    x[:, 3] *= times
+    check_adapters(device, pool, which, x, np.zeros((tokens, rows), np.float32), near=1e-6)
+
+
 # Small tokens keep their bits in every form. Parts of BF16, of x over BF16 weights
 # and of the low-rank sums over all, end at 2^-134, so that 2^-23 of 2^-103 (1e-31)
 # is still held, and of the low-rank sums of 1e-36 with weights 1,024 times as large
