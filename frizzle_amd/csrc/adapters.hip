@@ -74,25 +74,56 @@ struct Raw {
 };
 
 // F32 values as parts of BF16 that add up to them (three hold F32's 24 bits and
-// its exponents), each what rounding left to the parts before.
+// its exponents), each what the parts before left. The first of three is cut, not
+// rounded: neither it nor a product of it is infinite where the value's own is not.
+// Weights are finite; of an x or a low-rank sum that is infinite or no number, the
+// first two parts are finite and the last, which meets the other operand's first
+// part alone, is the value.
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-template <int kParts>
-__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&part)[kParts]) {
-  float rest[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) rest[j] = x[j];
-#pragma unroll
-  for (int p = 0; p < kParts; ++p)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      part[p][j] = (__bf16)rest[j];
-      if (p + 1 < kParts) rest[j] -= (float)part[p][j];
-    }
+template <bool kFinite>
+__device__ __forceinline__ float within(float x, float largest) {
+  return kFinite ? x : __builtin_amdgcn_fmed3f(x, -largest, largest);
 }
-// Parts that hold a format's weights exactly: F16's 11 bits take two.
+template <bool kFinite>
+__device__ __forceinline__ __bf16 first_of_three(float x, float* rest) {
+  const uint32_t finite = float_to_bits(within<kFinite>(x, 0x1.FFFFFEp127f));
+  *rest = x - bits_to_float(finite & 0xFFFF0000u);
+  return __builtin_bit_cast(__bf16, (uint16_t)(finite >> 16));
+}
+template <bool kFinite>
+__device__ __forceinline__ __bf16 second_of_three(float x, float* rest) {
+  const __bf16 part = (__bf16)within<kFinite>(x, 0x1p121f);  // what the first leaves is below
+  *rest = x - (float)part;
+  return part;
+}
+template <bool kFinite>
+__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&part)[3]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    float rest;
+    part[0][j] = first_of_three<kFinite>(x[j], &rest);
+    part[1][j] = second_of_three<kFinite>(rest, &rest);
+    part[2][j] = (__bf16)rest;
+  }
+}
+// Parts that hold a format's weights exactly: F16's 11 bits take two, BF16's one.
 template <int kFormat>
 constexpr int kWeightParts = kFormat == 0 ? 3 : kFormat == 1 ? 2 : 1;
+__device__ __forceinline__ void split_weights(const float (&x)[8], bf16x8 (&part)[3]) {
+  split8<true>(x, part);
+}
+__device__ __forceinline__ void split_weights(const float (&x)[8], bf16x8 (&part)[2]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    part[0][j] = (__bf16)x[j];
+    part[1][j] = (__bf16)(x[j] - (float)part[0][j]);
+  }
+}
+__device__ __forceinline__ void split_weights(const float (&x)[8], bf16x8 (&part)[1]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) part[0][j] = (__bf16)x[j];
+}
 
 struct Run {
   uint32_t first, tokens;
@@ -283,7 +314,7 @@ __device__ __forceinline__ void low_rank(const AdapterArgs& a, const Run& run, i
             half8 part;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              part[j] = (_Float16)xs[j];
+              part[j] = (_Float16)(p < 2 ? within<false>(xs[j], 65504.0f) : xs[j]);
               if (p < 2) xs[j] = (xs[j] - (float)part[j]) * (p == 0 ? kRestScale : 1.0f);
             }
 #pragma unroll
@@ -293,7 +324,7 @@ __device__ __forceinline__ void low_rank(const AdapterArgs& a, const Run& run, i
           }
         } else {
           bf16x8 part[3];
-          split8(xs, part);
+          split8<false>(xs, part);
 #pragma unroll
           for (int p = 2; p >= 0; --p)
 #pragma unroll
@@ -458,19 +489,18 @@ __global__ __launch_bounds__(64 * kUpWaves, kUpPlaces<kRun>) void adapter_up_ker
       const int at = threadIdx.x + i * 64 * kUpWaves;
       const int t = at / (8 * kChunks), r = at % (8 * kChunks) * 4;
       if (kFull < 256 && t >= kRun) break;
-      float rest[4];
+      Low4 part[kLowParts];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) rest[e] = r + e < rank ? piece[i][e] * scale : 0.0f;
-#pragma unroll
-      for (int p = 0; p < kLowParts; ++p) {
-        Low4 part;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          part[e] = (Low)rest[e];
-          rest[e] -= (float)part[e];
+      for (int e = 0; e < 4; ++e) {
+        float rest = r + e < rank ? piece[i][e] * scale : 0.0f;
+        if constexpr (kInParts) {
+          part[0][e] = first_of_three<false>(rest, &rest);
+          part[1][e] = second_of_three<false>(rest, &rest);
         }
-        *reinterpret_cast<Low4*>(&low[p][t][r]) = part;
+        part[kLowParts - 1][e] = (Low)rest;
       }
+#pragma unroll
+      for (int p = 0; p < kLowParts; ++p) *reinterpret_cast<Low4*>(&low[p][t][r]) = part[p];
     }
     __syncthreads();
     // Lane (n, g): outputs 4 g .. + 3 of each tile, of token n of each 16.
@@ -497,7 +527,7 @@ __global__ __launch_bounds__(64 * kUpWaves, kUpPlaces<kRun>) void adapter_up_ker
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           weight[i][j] = 32 * c + 8 * g + j < rank ? w[c & 1][i].at(j) : 0.0f;
-        if constexpr (kInParts) split8(weight[i], part[i]);
+        if constexpr (kInParts) split_weights(weight[i], part[i]);
       }
 #pragma unroll
       for (int t = 0; t < kRunTiles; ++t) {
@@ -505,7 +535,8 @@ __global__ __launch_bounds__(64 * kUpWaves, kUpPlaces<kRun>) void adapter_up_ker
         const int at = 32 * c + 8 * g;
         if constexpr (kInParts) {
           // The products of parts down to 2^-16 of the largest: what is left
-          // out is as small as F32's rounding.
+          // out, 2^-22 of a product at most and some 2^-26 mostly, is as small as
+          // F32's rounding.
           bf16x8 h[3];
 #pragma unroll
           for (int p = 0; p < 3; ++p)

@@ -314,7 +314,9 @@ typedef struct frz_adapters {
  * base. y may be base itself, with its stride; otherwise no two of x, base
  * and y may overlap. Sums are in F32, of x and weights as they are, but that an x
  * counts to 2^-51 of the token's largest at least with F16 weights, and an x or a
- * low-rank sum to 2^-134 with any. */
+ * low-rank sum to 2^-134 with any. An infinite x, or one that is no
+ * number, gives what F32 sums give, in its own token's y alone, whichever form a
+ * call takes. Weights that count must be finite. */
 int frz_op_adapters(frz_device* dev, const frz_adapters* adapters, const uint32_t* which,
                     const float* x, int x_stride, const float* base, int base_stride, float* y,
                     int y_stride, uint32_t tokens);

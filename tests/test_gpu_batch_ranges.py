@@ -3,8 +3,8 @@ values far larger than the ones that count, against values in 64 bits."""
 import numpy as np
 import pytest
 
-from _batch import (BF16, F16, F32, NONE, Paged, Pool, check_adapters, check_attention, of_format,
-                    to_format)
+from _batch import (BF16, F16, F32, NONE, Paged, Pool, adapters, adapters_exact, check_adapters,
+                    check_attention, of_format, to_format)
 
 pytestmark = pytest.mark.gpu
 
@@ -100,3 +100,61 @@ def test_the_smallest_tokens(device, fmt, tokens, rank, cols, rows, size):
         pool.dev[i] = device.array(w)
     check_adapters(device, pool, which, (x * size).astype(np.float32),
                    np.zeros((tokens, rows), np.float32), near=1e-6)
+
+
+# Values between BF16's largest, 3.3895e38, and F32's, 3.4028e38, which F32 sums take
+# like any other: x, a low-rank sum, a weight.
+@pytest.mark.parametrize("fmt,place", [(f, p) for f in (F32, F16, BF16) for p in ("x", "low")]
+                         + [(F32, "up")])
+@SHAPES
+def test_values_past_the_largest_of_16_bits(device, fmt, place, tokens, rank, cols, rows):
+    rng = np.random.default_rng(rows)
+    pool, which, x = adapters_of(device, rng, fmt, tokens, rank, cols, rows)
+    down, up = of_format(pool.down, fmt), of_format(pool.up, fmt)
+    if place == "x":
+        x[:, 5] = 3.4e38 * rng.choice([-1, 1], tokens)
+        down *= 2.0 ** -16
+    elif place == "low":
+        x[:] = 0
+        x[:, 5] = 1.7e38 * rng.choice([-1, 1], tokens)
+        down[:, :, 5], up = 2.0, up * 2.0 ** -8
+    else:
+        x *= 1e-3
+        up = 3.4e38 * np.sign(up)
+        down *= 1e-3
+    for i, w in enumerate((down, up)):
+        bits = to_format(w, fmt)
+        (pool.down, pool.up)[i][:] = bits
+        pool.dev[i] = device.array(bits)
+    check_adapters(device, pool, which, x, np.zeros((tokens, rows), np.float32), near=1e-6)
+
+
+# An infinite x, whichever form a call takes: infinite outputs of its weights' signs
+# where one rank counts, no number where infinities of both signs meet.
+@pytest.mark.parametrize("fmt", [F32, F16, BF16])
+@SHAPES
+def test_infinite_tokens(device, fmt, tokens, rank, cols, rows):
+    rng = np.random.default_rng(rows)
+    x = rng.normal(0, 1, (tokens, cols)).astype(np.float32)
+    pool = Pool(device, rng, 2, rank, cols, rows, fmt, ranks=[1, rank])
+    for i, w in enumerate((pool.down, pool.up)):  # no zeros
+        w[of_format(w, fmt) == 0] = to_format(np.array([0.5]), fmt)[0]
+        pool.dev[i] = device.array(w)
+    which = [0] * (tokens // 2) + [1] * (tokens - tokens // 2)
+    base = rng.normal(0, 1, (tokens, rows)).astype(np.float32)
+    at = rng.choice(tokens, 5, replace=False)
+    x[at, rng.integers(0, cols, 5)] = np.inf
+    x[at[0]] *= -1
+    want, far = adapters_exact(pool, which, np.where(np.isinf(x), 0, x), base)
+    got = adapters(device, pool, which, x, base)[:, :rows]
+    for t, a in enumerate(which):
+        if not np.isinf(x[t]).any():
+            assert (abs(got[t] - want[t]) <= far[t]).all(), t
+            continue
+        k = int(np.flatnonzero(np.isinf(x[t]))[0])
+        r = pool.own(a)
+        low = np.sign(of_format(pool.down[a, :r, k], fmt)) * np.sign(x[t, k])
+        signs = np.sign(of_format(pool.up[a, :, :r], fmt)) * low
+        one = abs(signs.sum(1)) == r
+        assert np.array_equal(got[t, one], np.inf * signs[one, 0]), t
+        assert np.isnan(got[t, ~one]).all(), t
