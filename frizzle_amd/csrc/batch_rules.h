@@ -105,6 +105,17 @@ FRZ_RULE uint32_t part_chunk(uint64_t blocks, uint32_t units, uint32_t at_once, 
   return high;
 }
 
+// Parts of a row of `blocks`, below 2^20, so that their quotient by the chunk is
+// right within one from F32, as a product with each = 1.0f / chunk. (No chunk, of
+// a batch without blocks: none.)
+FRZ_RULE uint32_t row_parts(uint32_t blocks, uint32_t chunk, float each) {
+  uint32_t n = (uint32_t)((float)blocks * each);
+  n += n * chunk < blocks;
+  n += n * chunk < blocks;
+  n -= n > 0 && (n - 1) * chunk >= blocks;
+  return n;
+}
+
 // The most parts there can be, and the most that belong to rows of several
 // parts: such a row has fewer than twice the parts that its blocks fill.
 FRZ_RULE uint32_t most_parts(uint32_t units, uint32_t at_once) {

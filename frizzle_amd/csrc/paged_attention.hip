@@ -231,16 +231,11 @@ __device__ __forceinline__ bool find_part(const PagedAttentionArgs& a, uint32_t 
   const uint32_t all = lane_of(wave_sum_to(mine), 63);
   uint32_t parts[kPer], total, joined;
   auto cut = [&](uint32_t chunk) {
-    // A row's blocks are below 2^20, so that their quotient is right within one
-    // from F32.
     const float each = 1.0f / (float)(chunk ? chunk : 1);
     total = joined = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      uint32_t n = (uint32_t)((float)blocks[i] * each);
-      n += n * chunk < blocks[i];
-      n += n * chunk < blocks[i];
-      n -= n > 0 && (n - 1) * chunk >= blocks[i];
+      const uint32_t n = row_parts(blocks[i], chunk, each);
       parts[i] = n;
       total += n;
       joined += n > 1 ? n + (1u << 20) : 0;  // parts, and rows above them
