@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <optional>
 #include <string>
 #include <vector>
 
@@ -192,7 +193,11 @@ static int open_device(const char* what, int ordinal, bool on, hipStream_t strea
     return refuse(FRZ_ERR_DEVICE, "no HIP device");
   }
   if (ordinal < 0 || ordinal >= count) return refuse(FRZ_ERR_ARGUMENT, "no such device");
-  if (int rc = check_hip(hipSetDevice(ordinal), "hipSetDevice")) return rc;
+  // A caller with a stream keeps its current device.
+  std::optional<OnDevice> restored;
+  if (int rc = check_hip(on ? restored.emplace(ordinal).error() : hipSetDevice(ordinal),
+                         "hipSetDevice"))
+    return rc;
   hipDeviceProp_t prop;
   if (int rc = check_hip(hipGetDeviceProperties(&prop, ordinal), "hipGetDeviceProperties")) return rc;
   if (std::strncmp(prop.gcnArchName, "gfx950", 6) != 0) {
@@ -256,7 +261,7 @@ int frz_open_on(int ordinal, void* stream, frz_device** out, frz_limits* limits)
 
 void frz_close(frz_device* dev) {
   if (!dev) return;
-  (void)hipSetDevice(dev->ordinal);
+  OnDevice on(dev->ordinal);
   (void)hipStreamSynchronize(dev->stream);
   if (dev->batch_scratch) (void)hipFree(dev->batch_scratch);
   (void)hipFree(dev->topk_scratch);
