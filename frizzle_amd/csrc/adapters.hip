@@ -11,8 +11,8 @@
 //
 // The products of runs are on the matrix cores: with 16-bit weights, and U's of
 // long runs with F32 ones, of parts of 16 bits that add up to the operands, else
-// F32's own (v_mfma_f32_16x16x4_f32). Sums are F32 in both forms, and nothing is
-// rounded to less than F32's 24 bits. The weights are the instruction's A operand, 16
+// F32's own (v_mfma_f32_16x16x4_f32). Sums are F32 in both forms, and operands
+// keep their 24 bits (kDownInParts). The weights are the instruction's A operand, 16
 // rows of as many columns as it takes: lane (m, g) holds 8 columns of row m as
 // they lie in memory, and of F32's eight instructions the j-th takes the j-th of
 // each. Loads are a step ahead of the products, and all of a step's loads are
@@ -44,8 +44,9 @@ template <int kRun>
 constexpr uint32_t kUpPlaces = kRun == 16 ? 4 : 3;  // of the U kernel
 // Columns from which a workgroup of the D kernel takes four tiles of ranks with
 // 16-bit weights, for half of the reads of x: 333 tokens of one adapter, rank 64,
-// 6,912 to 1,152, a call 17.4 -> 15.7 us, though 22.3 -> 24.4 of 32 adapters, as
-// fewer workgroups run at once; 512 tokens, 1,152 columns, rank 128, 20.0 -> 22.5.
+// 6,912 to 1,152, a call 17.7 -> 16.7 us, though 23.2 -> 23.7 of 32 adapters, as
+// fewer workgroups run at once (300 of one each, rank 128, 4,096 to 4,096, 171 ->
+// 180); 512 tokens, 1,152 columns, rank 128, 21.1 -> 22.7.
 constexpr int kLongCols = 4096;
 constexpr int kTokenWaves = 8;
 constexpr uint32_t kTokenWorkgroups = 256;    // that one launch by tokens is cut into, about
@@ -237,8 +238,8 @@ __device__ __forceinline__ void copy_base(const AdapterArgs& a, uint32_t first, 
 // Whether D's products are of parts of x on the 16-bit matrix cores, the
 // weights as they lie in memory: 3 instructions of 16 cycles for 32 columns
 // where F32's eight take 256. 512 tokens, rank 32, 6,912 to 1,152, F16, of one
-// adapter 15.4 -> 14.6 us a call, of one each 114 -> 105; rank 128, 4,096 to
-// 4,096, 300 of one each 172 -> 158. Three parts hold all of x's 24 bits; those
+// adapter 14.4 -> 13.9 us a call, of one each 109 -> 99; rank 128, 4,096 to
+// 4,096, 300 of one each 202 -> 180. Three parts hold all of x's 24 bits; those
 // of F16 down to 2^-28 of the largest of a token's columns that a wave takes at
 // once, and 2^-51 of it below: x is scaled, token by token, to lie below 2^15,
 // and the parts after the first by 2^12 more, in sums of their own, so that F16's
@@ -356,7 +357,7 @@ __device__ __forceinline__ void low_rank(const AdapterArgs& a, const Run& run, i
 // x and D alone (D on every die had been most of what the dies read). Bound by
 // loads of few steps that a launch, the adapters' search and a sum over the
 // waves frame: 333 tokens of three F16 adapters, rank 64, 6,912 columns (12 MB)
-// some 8.5 us, 512 tokens of an F32 one, rank 128, 1,152 columns some 6.
+// some 8.7 us, 512 tokens of an F32 one, rank 128, 1,152 columns some 6.
 template <int kFormat, int kTiles>
 __global__ __launch_bounds__(64 * kDownWaves, 2 * kDownPlaces<kTiles>)
 void adapter_down_kernel(AdapterArgs a) {
@@ -400,9 +401,9 @@ void adapter_down_kernel(AdapterArgs a) {
 // 6 instructions of 16 cycles for 32 ranks where F32's eight take 256. What it
 // costs is the parts of U, some 150 cycles for 8 weights a lane of F16 or F32,
 // which a run's tiles of tokens share: rank 128, 1,152 to 6,912, 512 tokens of
-// one adapter, the call 24.0 -> 20.6 us in F16 and 24.5 -> 23 in F32 (440 ->
-// 467 of an F32 adapter each); not for F32 in runs of 32: rank 128, 6,912 to
-// 1,152, 200 tokens, 22.6 -> 24.3 us.
+// one adapter, the call 24.5 -> 21.2 us in F16 and 25.6 -> 23.9 in F32 (449 ->
+// 466 of an F32 adapter each); not for F32 in shorter runs: rank 128, 6,912 to
+// 1,152, 200 tokens, 21.6 -> 21.8 us.
 template <int kFormat, int kRun>
 constexpr bool kUpInParts = kFormat != 0 || kRun == 64;
 
@@ -456,7 +457,8 @@ __global__ __launch_bounds__(64 * kUpWaves, kUpPlaces<kRun>) void adapter_up_ker
     const int run_tiles = (int)((run.tokens + 15) / 16);
     __syncthreads();  // the last item's rows are read
     // Four ranks a thread and piece, several splits of all its pieces asked for
-    // together; ranks past the adapter's own, and tokens past the run, are zero.
+    // together; ranks past the adapter's own are zero, tokens past the run its
+    // last one, whose products nothing takes.
     constexpr int kFull = kRun * 8 * kChunks, kPieces = kFull < 256 ? 1 : kFull / (64 * kUpWaves);
     constexpr int kTogether = kPieces <= 2 ? 8 : kPieces <= 4 ? 4 : 2;
     f32x4 piece[kPieces];
@@ -584,7 +586,7 @@ __global__ __launch_bounds__(64 * kUpWaves, kUpPlaces<kRun>) void adapter_up_ker
 // with every eighth token on a die 23.7). Bound by latency at few tokens (two
 // chains of loads and a launch: 3 us of the call's 6) and by what a compute
 // unit takes in, about 40 GB/s, at more: 48 tokens of 41 adapters, BF16, rank
-// 32, 1,152 to 6,912 (18.5 MB), 9.1 us a call.
+// 32, 1,152 to 6,912 (18.5 MB), 8.9 us a call.
 template <int kFormat, int kLanes>
 __global__ __launch_bounds__(64 * kTokenWaves, kFormat == 0 ? 2 : 4)
 void adapter_token_kernel(AdapterArgs a) {
@@ -744,15 +746,15 @@ TokenBlocks token_blocks(const AdapterArgs& a, uint32_t turn) {
 
 // Whether it takes a call: where a D, which each of its workgroups reads whole,
 // a load after another, stays below kTokenDown (one token, 4,000 outputs, rank
-// 128, F16, of 1,152 columns, 295 kB, 9.7 us against 11.8 over runs, of 2,304 12.5
-// against 11.0, of 6,912 25.9 against 13.9; rank 32 of 9,216, 590 kB, 10.4 against
-// 11.8, of 16,384 15.2 against 12.1), and what all of them read, U with it, below
+// 128, F16, of 1,152 columns, 295 kB, 9.2 us against 10.7 over runs, of 2,304 12.1
+// against 10.8, of 6,912 24.6 against 13.4; rank 32 of 9,216, 590 kB, 10.2 against
+// 11.2, of 16,384 15.0 against 11.8), and what all of them read, U with it, below
 // kTokenBytes. Against two launches over runs, F16
 // weights, tokens of one adapter and of one each, at most 64: rank 64, 1,152 to
-// 6,912, 16 tokens (50 MB) 7.9 and 8.5 us against 10.8 and 13.8, 64 (90 MB) 13.2
-// and 18.3 against 11.2 and 28.5, 128 (144 MB) 20.4 and 23.5 against 11.8 and
-// 28.5; rank 32, 6,912 to 1,152, 128 tokens (117 MB) 9.7 and 11.4 against 14.6
-// and 26.2, 512 (252 MB) 18.7 and 19.2 against 15.6 and 22.7; rank 16, 1,152 to
+// 6,912, 16 tokens (50 MB) 8.5 and 9.0 us against 10.3 and 13.0, 64 (90 MB) 13.3
+// and 18.7 against 10.6 and 26.4, 128 (144 MB) 20.1 and 23.6 against 11.4 and
+// 26.3; rank 32, 6,912 to 1,152, 128 tokens (117 MB) 9.8 and 11.7 against 11.6
+// and 19.1, 512 (252 MB) 18.9 and 19.4 against 13.9 and 18.8; rank 16, 1,152 to
 // 1,536, 1 to 256 tokens 7 against 9 to 12.
 template <int kFormat, int kLanes>
 bool takes_tokens(const AdapterArgs& a) {

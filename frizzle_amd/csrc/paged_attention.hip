@@ -42,8 +42,8 @@
 //
 // Whole calls, 256 wide, F16 but where said: three requests of 98,001 to
 // 131,072 keys over 4 key-value heads (1.4 GB) 235 us, 6.0 TB/s; 61 of 40 to
-// 8,192 keys (99 MB) 24.6 us, 4.0 TB/s; 32 of 1 to 4,001 keys, 8 BF16 key-value
-// heads of 128 (70 MB), 20.4 us, 3.5 TB/s; one of 5,004 keys (5 MB) 11.5 us,
+// 8,192 keys (99 MB) 24.8 us, 4.0 TB/s; 32 of 1 to 4,001 keys, 8 BF16 key-value
+// heads of 128 (70 MB), 20.6 us, 3.4 TB/s; one of 5,004 keys (5 MB) 11.0 us,
 // two launches of dependent loads.
 
 #include "batch_rules.h"
@@ -709,9 +709,11 @@ hipError_t launch_shape(hipStream_t s, PagedAttentionArgs a, uint32_t heads, int
   // there to keep the compute units at work (100 of a window of 512: 22.6 and
   // 17.2; but 16: 11.9 and 16.0). Where more units are there than workgroups run
   // at once, a unit is a wave's: four waves would each have had a block or two
-  // of a short row (483 rows of 16 to 31 keys, 8 key-value heads, 256 wide, 137
+  // of a short row (483 rows of 16 to 31 keys, 8 key-value heads, 256 wide, 127
   // us and 35; 512 of a window of 512 67 and 52; not of 63 blocks, 400 rows of 8
-  // heads 128 wide: 214 by workgroups, 257 by waves).
+  // heads 128 wide: 214 by workgroups, 257 by waves). The host knows the table's
+  // width and the window, not the rows: short rows in a wide table without a window
+  // are cut (those 483 take the 127).
   const uint64_t capacity = (uint64_t)a.cache.width * a.cache.page_slots;
   const uint64_t held = (capacity + kBlockKeys - 1) / kBlockKeys;
   const uint64_t seen = (uint64_t)a.window / kBlockKeys + 2;

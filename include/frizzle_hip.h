@@ -271,7 +271,8 @@ typedef struct frz_pages {
  * and overlaps nothing else.
  * Keys and values round to the cache's format, to nearest even (F16
  * saturates at 65,504). Of rows at one request's position the last one's
- * stay; two requests must not append to a page that they share. */
+ * stay; two requests must not append to a page that they share, nor one through
+ * two entries of its row that name one page. */
 int frz_op_rope_paged(frz_device* dev, const frz_pages* cache, const uint32_t* sequences,
                       const uint32_t* positions, const float* turns, const float* query_gain,
                       const float* key_gain, const float* query, const float* key,
