@@ -34,8 +34,9 @@
 // are 2^14 at the running maximum, for the same reason, and held to 2^-39 of it.
 // For BF16, whose range is F32's, the query lies below 2^-8 (one past 2^104 2^113
 // below itself) and weights are at most 2^-24, so that no sum of finite keys' or
-// values' products leaves it where scores do not. All scales are exact, products
-// are exact in F32, sums F32.
+// values' products leaves it where scores do not (of scores below 2^23, from which
+// on F32 does not hold the maximum 24 above). All scales are exact, products are
+// exact in F32, sums F32.
 //
 // Keys outside the row's range or in no page are never read: their rows are
 // zeros, and their scores -inf.

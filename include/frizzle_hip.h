@@ -282,7 +282,8 @@ int frz_op_rope_paged(frz_device* dev, const frz_pages* cache, const uint32_t* s
  * position], its own among them (window at least 1; 0xFFFFFFFF: all): query
  * head i reads key-value head i / (query_heads / kv_heads). Scores are scale
  * (at most 4,096 either side of zero) times the products, and must stay in
- * F32's range, as they must before scale. Sums are F32, not in the reference's
+ * F32's range, as they must before scale (over BF16 values past 2^100: below
+ * 2^23). Sums are F32, not in the reference's
  * order, over keys and values as they are and a query of 24 bits (BF16 caches)
  * or to 2^-23 of itself, or 2^-51 of its head's largest (F16): a score is off by
  * some 2^-22 of the sum of its products' sizes, and an output by twice as much of

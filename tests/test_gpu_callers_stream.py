@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import frizzle_amd as fz
+import test_gpu_batch_adapters as layer
 from _batch import F16, NONE, adapters_exact, attention_exact, rope_exact
 from frizzle_amd import _lib
 
@@ -170,6 +171,40 @@ def test_in_a_captured_graph():
             torch.cuda.synchronize()
     finally:
         device.close()
+
+
+def test_single_kernels_beside_them_on_the_default_stream():
+    # Products, which wait for their stream, between the ops, which do not.
+    device = fz.Device(0, stream=0)
+    try:
+        layer.test_a_batch_of_requests_steps_through_a_layer(device)
+    finally:
+        device.close()
+
+
+def test_two_handles_on_one_stream():
+    # Each with a workspace of its own, their calls in the stream's order.
+    stream = torch.cuda.Stream()
+    devices = [fz.Device(0, stream=stream.cuda_stream) for _ in range(2)]
+    try:
+        with torch.cuda.stream(stream):
+            torch.manual_seed(5)
+            steps, kept = [Step(), Step()], []
+            for i in range(6):
+                step = steps[i % 2]
+                x, base = torch.randn(ROWS, HIDDEN, device="cuda"), torch.randn(ROWS, QKV,
+                                                                               device="cuda")
+                step.x.copy_(x)
+                step.base.copy_(base)
+                step.enqueue(devices[i % 2])
+                kept.append((step, x, base, step.qkv.clone(), step.out.clone(),
+                             step.keys.clone(), step.values.clone()))
+        torch.cuda.synchronize()
+        for k in kept:
+            check(*k)
+    finally:
+        for d in devices:
+            d.close()
 
 
 def test_the_stream_outlives_the_handle_and_holds_no_model():
