@@ -64,11 +64,13 @@ class LoadPolicy(ctypes.Structure):
 
 
 class Pages(ctypes.Structure):
-    """frz_pages: caches in pages, by their device addresses."""
+    """frz_pages: caches in pages, by their device addresses. The last three, a
+    cache of 8 bits' scales, are of format 24 alone."""
     _fields_ = [("keys", c_void_p), ("values", c_void_p), ("format", c_int),
                 ("kv_heads", c_int), ("head_dim", c_int), ("page_slots", c_uint32),
                 ("pages", c_uint32), ("page_stride", c_uint64), ("table", c_void_p),
-                ("sequences", c_uint32), ("width", c_uint32)]
+                ("sequences", c_uint32), ("width", c_uint32), ("key_scales", c_void_p),
+                ("value_scales", c_void_p), ("scale_stride", c_uint64)]
 
 
 class Adapters(ctypes.Structure):
@@ -174,6 +176,10 @@ _SIGS = {
                                   c_int, _P, c_int, c_int, c_float, c_uint32]),
     "frz_op_attention_paged": (c_int, [_P, POINTER(Pages), _P, _P, _P, c_int, _P, c_int, c_int,
                                        c_uint32, c_float, c_uint32]),
+    "frz_op_attention_paged_sinks": (c_int, [_P, POINTER(Pages), _P, _P, _P, c_int, _P, c_int,
+                                             c_int, c_uint32, c_uint32, c_float, c_uint32]),
+    "frz_op_read_paged": (c_int, [_P, POINTER(Pages), _P, _P, c_int, _P, _P, c_uint64,
+                                  c_uint32]),
     "frz_op_adapters": (c_int, [_P, POINTER(Adapters), _P, _P, c_int, _P, c_int, _P, c_int,
                                 c_uint32]),
     "frz_op_numerics": (c_int, [_P, c_int, _P, _P, c_int]),

@@ -23,6 +23,7 @@ constexpr size_t kAdapterBytes =
 constexpr size_t kScratchBytes = kAttentionBytes > kAdapterBytes ? kAttentionBytes : kAdapterBytes;
 
 constexpr int kMostHeads = 1024;
+constexpr uint32_t kMostReadRows = 1u << 24;
 constexpr float kMostScale = 4096.0f;  // 2^13 in log2 units, as the kernel takes
 
 bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -44,12 +45,14 @@ int enqueue(frz_device* dev, const char* what, Launch launch) {
 }
 
 // The refusal's text, or null.
-const char* refuse_pages(const frz_pages* c, int query_heads, uint32_t rows) {
+const char* refuse_pages(const frz_pages* c, int query_heads, uint32_t rows, uint32_t most_rows) {
   if (!c) return "null cache";
   if (!c->keys || !c->values || !c->table) return "null keys, values or table";
   if (!aligned(c->keys) || !aligned(c->values)) return "keys or values not at a multiple of 16 bytes";
   if (!aligned_word(c->table)) return "table not at a multiple of 4 bytes";
-  if (c->format != FRZ_FORMAT_F16 && c->format != FRZ_FORMAT_BF16) return "cache format (F16 1 or BF16 30)";
+  const bool i8 = c->format == FRZ_FORMAT_I8;
+  if (!i8 && c->format != FRZ_FORMAT_F16 && c->format != FRZ_FORMAT_BF16)
+    return "cache format (F16 1, I8 24 or BF16 30)";
   if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return "head_dim (64, 128 or 256)";
   if (c->kv_heads < 1 || query_heads < 1 || query_heads > kMostHeads || query_heads % c->kv_heads)
     return "heads (query_heads a multiple of kv_heads, at most 1,024)";
@@ -58,20 +61,31 @@ const char* refuse_pages(const frz_pages* c, int query_heads, uint32_t rows) {
   if (c->sequences < 1 || c->pages < 1 || c->pages == FRZ_NO_PAGE) return "no sequences or pages";
   if (c->width < 1 || (uint64_t)c->width * c->page_slots > rules::kMostKeys)
     return "width (width * page_slots from 1 to 2^24 keys)";
-  if (c->page_stride % 8 ||
+  if (c->page_stride % (i8 ? 16 : 8) ||
       c->page_stride < (uint64_t)c->page_slots * c->kv_heads * c->head_dim)
-    return "page_stride (a multiple of 8, at least a page)";
+    return "page_stride (a multiple of 16 bytes, at least a page)";
   // Their product is an offset in 64 bits.
   if (c->page_stride > (1ull << 48) / c->pages) return "page_stride (a pool of at most 2^48 values)";
-  if (rows < 1 || rows > rules::kMostRows) return "rows (1 to 512)";
+  if (i8) {
+    if (!c->key_scales || !c->value_scales) return "null scales";
+    if (!aligned_word(c->key_scales) || !aligned_word(c->value_scales))
+      return "scales not at a multiple of 4 bytes";
+    if (c->scale_stride < (uint64_t)c->page_slots / rules::kScaleSlots * c->kv_heads ||
+        c->scale_stride > (1ull << 48) / c->pages)
+      return "scale_stride (at least a page's scales, a pool of at most 2^48)";
+  }
+  if (rows < 1 || rows > most_rows)
+    return most_rows == rules::kMostRows ? "rows (1 to 512)" : "rows (1 to 2^24)";
   return nullptr;
 }
 
 PagedCache cache_of(const frz_pages* c) {
   PagedCache p;
-  p.keys = static_cast<uint16_t*>(c->keys);
-  p.values = static_cast<uint16_t*>(c->values);
-  p.bf16 = c->format == FRZ_FORMAT_BF16;
+  p.keys = c->keys;
+  p.values = c->values;
+  p.format = c->format == FRZ_FORMAT_I8     ? kCacheI8
+             : c->format == FRZ_FORMAT_BF16 ? kCacheBf16
+                                            : kCacheF16;
   p.kv_heads = (uint32_t)c->kv_heads;
   p.head_dim = (uint32_t)c->head_dim;
   p.page_slots = c->page_slots;
@@ -80,6 +94,10 @@ PagedCache cache_of(const frz_pages* c) {
   p.table = c->table;
   p.sequences = c->sequences;
   p.width = c->width;
+  const bool i8 = p.format == kCacheI8;  // caches of 16 bits may come without these
+  p.key_scales = i8 ? c->key_scales : nullptr;
+  p.value_scales = i8 ? c->value_scales : nullptr;
+  p.scale_stride = i8 ? c->scale_stride : 0;
   return p;
 }
 
@@ -89,6 +107,44 @@ int refuse(const char* what, const char* why) {
 
 // Whether rows of `width` floats may be `stride` apart.
 bool stride_ok(int stride, int64_t width) { return stride % 4 == 0 && stride >= width; }
+
+int attention_paged(const char* what, frz_device* dev, const frz_pages* cache,
+                    const uint32_t* sequences, const uint32_t* positions, const float* query,
+                    int q_stride, float* out, int out_stride, int query_heads, uint32_t window,
+                    uint32_t sinks, float scale, uint32_t rows) {
+  if (!dev) return refuse(what, "no device");
+  if (const char* why = refuse_pages(cache, query_heads, rows, rules::kMostRows)) return refuse(what, why);
+  if (!positions || !query || !out) return refuse(what, "null argument");
+  if (!aligned(query) || !aligned(out) || !aligned_word(positions) || !aligned_word(sequences))
+    return refuse(what, "a pointer not at a multiple of 16 bytes (positions and sequences: 4)");
+  const int64_t q = (int64_t)query_heads * cache->head_dim;
+  if (!stride_ok(q_stride, q) || !stride_ok(out_stride, q))
+    return refuse(what, "strides (multiples of 4, at least a row)");
+  if (out == query) return refuse(what, "out is query");
+  if (window == 0) return refuse(what, "window 0");
+  if (!(std::fabs(scale) <= kMostScale)) return refuse(what, "scale (a number of at most 4,096)");
+  PagedAttentionArgs a;
+  a.cache = cache_of(cache);
+  a.sequences = sequences;
+  a.positions = positions;
+  a.query = query;
+  a.q_stride = (uint32_t)q_stride;
+  a.out = out;
+  a.out_stride = (uint32_t)out_stride;
+  a.query_heads = (uint32_t)query_heads;
+  a.window = window;
+  a.sinks = sinks;
+  a.scale_log2e = (float)((double)scale * 1.4426950408889634);
+  a.rows = rows;
+  return enqueue(dev, what, [&] {
+    float* at = static_cast<float*>(dev->batch_scratch);
+    a.states = at;
+    a.stats = at + kStateFloats;
+    a.records = reinterpret_cast<uint4*>(at + kStateFloats + kStatFloats);
+    a.record_count = reinterpret_cast<uint32_t*>(a.records + kRecords);
+    return launch_paged_attention(dev->stream, a, dev->props.multiProcessorCount);
+  });
+}
 
 }  // namespace
 
@@ -112,7 +168,7 @@ int frz_op_rope_paged(frz_device* dev, const frz_pages* cache, const uint32_t* s
                       int roped_stride, int query_heads, float epsilon, uint32_t rows) {
   const char* what = "frz_op_rope_paged";
   if (!dev) return refuse(what, "no device");
-  if (const char* why = refuse_pages(cache, query_heads, rows)) return refuse(what, why);
+  if (const char* why = refuse_pages(cache, query_heads, rows, rules::kMostRows)) return refuse(what, why);
   if (!positions || !turns || !query_gain || !key_gain || !query || !key || !value || !roped)
     return refuse(what, "null argument");
   if (!aligned(turns) || !aligned(query_gain) || !aligned(key_gain) || !aligned(query) ||
@@ -150,38 +206,47 @@ int frz_op_attention_paged(frz_device* dev, const frz_pages* cache, const uint32
                            const uint32_t* positions, const float* query, int q_stride,
                            float* out, int out_stride, int query_heads, uint32_t window,
                            float scale, uint32_t rows) {
-  const char* what = "frz_op_attention_paged";
+  return attention_paged("frz_op_attention_paged", dev, cache, sequences, positions, query,
+                         q_stride, out, out_stride, query_heads, window, 0, scale, rows);
+}
+
+int frz_op_attention_paged_sinks(frz_device* dev, const frz_pages* cache,
+                                 const uint32_t* sequences, const uint32_t* positions,
+                                 const float* query, int q_stride, float* out, int out_stride,
+                                 int query_heads, uint32_t window, uint32_t sinks, float scale,
+                                 uint32_t rows) {
+  return attention_paged("frz_op_attention_paged_sinks", dev, cache, sequences, positions, query,
+                         q_stride, out, out_stride, query_heads, window, sinks, scale, rows);
+}
+
+int frz_op_read_paged(frz_device* dev, const frz_pages* cache, const uint32_t* sequences,
+                      const uint32_t* positions, int format, void* keys, void* values,
+                      uint64_t stride, uint32_t rows) {
+  const char* what = "frz_op_read_paged";
   if (!dev) return refuse(what, "no device");
-  if (const char* why = refuse_pages(cache, query_heads, rows)) return refuse(what, why);
-  if (!positions || !query || !out) return refuse(what, "null argument");
-  if (!aligned(query) || !aligned(out) || !aligned_word(positions) || !aligned_word(sequences))
+  if (const char* why = refuse_pages(cache, cache ? cache->kv_heads : 0, rows, kMostReadRows))
+    return refuse(what, why);
+  if (!positions || !keys || !values) return refuse(what, "null argument");
+  if (format != FRZ_FORMAT_F32 && format != FRZ_FORMAT_F16 && format != FRZ_FORMAT_BF16)
+    return refuse(what, "format (F32 0, F16 1 or BF16 30)");
+  if (!aligned(keys) || !aligned(values) || !aligned_word(positions) || !aligned_word(sequences))
     return refuse(what, "a pointer not at a multiple of 16 bytes (positions and sequences: 4)");
-  const int64_t q = (int64_t)query_heads * cache->head_dim;
-  if (!stride_ok(q_stride, q) || !stride_ok(out_stride, q))
-    return refuse(what, "strides (multiples of 4, at least a row)");
-  if (out == query) return refuse(what, "out is query");
-  if (window == 0) return refuse(what, "window 0");
-  if (!(std::fabs(scale) <= kMostScale)) return refuse(what, "scale (a number of at most 4,096)");
-  PagedAttentionArgs a;
+  if (stride % 8 || stride < (uint64_t)cache->kv_heads * cache->head_dim ||
+      stride > (1ull << 48) / rows)
+    return refuse(what, "stride (a multiple of 8, at least a row, at most 2^48 values in all)");
+  if (keys == values || keys == cache->keys || keys == cache->values || values == cache->keys ||
+      values == cache->values)
+    return refuse(what, "keys and values of the cache or of each other");
+  PagedReadArgs a;
   a.cache = cache_of(cache);
   a.sequences = sequences;
   a.positions = positions;
-  a.query = query;
-  a.q_stride = (uint32_t)q_stride;
-  a.out = out;
-  a.out_stride = (uint32_t)out_stride;
-  a.query_heads = (uint32_t)query_heads;
-  a.window = window;
-  a.scale_log2e = (float)((double)scale * 1.4426950408889634);
+  a.format = format;
+  a.keys = keys;
+  a.values = values;
+  a.stride = stride;
   a.rows = rows;
-  return enqueue(dev, what, [&] {
-    float* at = static_cast<float*>(dev->batch_scratch);
-    a.states = at;
-    a.stats = at + kStateFloats;
-    a.records = reinterpret_cast<uint4*>(at + kStateFloats + kStatFloats);
-    a.record_count = reinterpret_cast<uint32_t*>(a.records + kRecords);
-    return launch_paged_attention(dev->stream, a, dev->props.multiProcessorCount);
-  });
+  return enqueue(dev, what, [&] { return launch_paged_read(dev->stream, a); });
 }
 
 int frz_op_adapters(frz_device* dev, const frz_adapters* adapters, const uint32_t* which,

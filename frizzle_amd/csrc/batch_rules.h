@@ -3,8 +3,10 @@
 //
 // A request's keys lie in pages: slot s of its key p / page_slots is
 // p % page_slots, and the page's number stands in the request's row of the
-// table. A row of the batch reads the keys (p - window, p]; those past the
-// table's width, or in a page that the pool does not have, are not there.
+// table. A row of the batch reads the keys (p - window, p] and its request's
+// first `sinks`; those past the table's width, or in a page that the pool does
+// not have, are not there. Caches of 8 bits hold a scale for each block of 16
+// slots and key-value head.
 //
 // Attention's work is counted in blocks of 32 keys, which lie by position, a
 // row's keys' blocks taken by each of its head blocks (a key-value head with
@@ -49,24 +51,70 @@ constexpr uint32_t kPartWaves = 4;   // a part's workgroup
 constexpr uint32_t kHeadBlock = 16;  // query heads that share a part at most
 constexpr uint32_t kMostRows = 512;
 
-// The keys [first, end) that a row at `position` reads of a sequence whose
-// table holds `capacity`.
+// The keys [first, end) and, apart from them and before, [0, sinks) that a row
+// at `position` reads of a sequence whose table holds `capacity`.
 struct KeyRange {
-  uint32_t first, end;
+  uint32_t first, end, sinks;
 };
-FRZ_RULE KeyRange key_range(uint32_t position, uint32_t window, uint32_t capacity) {
+FRZ_RULE KeyRange key_range(uint32_t position, uint32_t window, uint32_t capacity,
+                            uint32_t sinks = 0) {
   KeyRange r;
   const uint32_t after = position + 1;  // position is not kNone
   r.first = after > window ? after - window : 0;
   r.end = after < capacity ? after : capacity;
-  if (r.first > r.end) r.first = r.end;
+  if (r.first <= sinks) {  // nothing between
+    r.first = r.sinks = 0;
+  } else {
+    r.sinks = sinks < r.end ? sinks : r.end;
+    if (r.first > r.end) r.first = r.end;
+  }
   return r;
+}
+
+// A row's blocks are counted from its first: those of its sinks, then those of
+// [first, end), though the last of the former may be the first of the latter; each
+// is looked at for its own keys, so no block has a hole.
+struct BlockKeys {
+  uint32_t block;       // by position
+  uint32_t first, end;  // the keys that its own lie among
+};
+FRZ_RULE uint32_t sink_blocks(KeyRange r) { return (r.sinks + kBlockKeys - 1) / kBlockKeys; }
+FRZ_RULE BlockKeys block_keys(KeyRange r, uint32_t counted) {
+  const uint32_t lead = sink_blocks(r);
+  BlockKeys b;
+  b.block = counted < lead ? counted : counted - lead + r.first / kBlockKeys;
+  b.first = counted < lead ? 0 : r.first;
+  b.end = counted < lead ? r.sinks : r.end;
+  return b;
 }
 
 // Blocks of a row's keys; one where it has none, so that its output is written.
 FRZ_RULE uint32_t row_blocks(KeyRange r) {
-  if (r.first >= r.end) return 1;
-  return (r.end + kBlockKeys - 1) / kBlockKeys - r.first / kBlockKeys;
+  const uint32_t lead = sink_blocks(r);
+  if (r.first >= r.end) return lead ? lead : 1;
+  return lead + (r.end + kBlockKeys - 1) / kBlockKeys - r.first / kBlockKeys;
+}
+// The most blocks of any row.
+FRZ_RULE uint64_t most_row_blocks(uint64_t capacity, uint32_t window, uint32_t sinks) {
+  const uint64_t held = (capacity + kBlockKeys - 1) / kBlockKeys + (sinks ? 1 : 0);
+  const uint64_t seen = (uint64_t)window / kBlockKeys + 2 +
+                        ((uint64_t)sinks + kBlockKeys - 1) / kBlockKeys;
+  const uint64_t most = held < seen ? held : seen;
+  return most ? most : 1;
+}
+
+// ---- caches of 8 bits ----------------------------------------------------------
+
+constexpr uint32_t kScaleSlots = 16;  // tokens that share a scale
+constexpr int kMostCode = 127;
+
+// The least power of two, from 2^-126 to 2^121, of which kMostCode reach `most`
+// (at least 0, not NaN; past 127 * 2^121 the last), as its F32 bits; 0 for 0.
+FRZ_RULE uint32_t block_scale_bits(uint32_t most_bits) {
+  if (most_bits == 0) return 0;
+  // 1.m * 2^x is 127 * 2^(x - 6) at most where 1.m is 127 / 64 at most.
+  const int power = (int)(most_bits >> 23) - 6 + ((most_bits & 0x7FFFFFu) > 0x7E0000u);
+  return (uint32_t)(power < 1 ? 1 : power > 248 ? 248 : power) << 23;
 }
 
 // Blocks of a part: as few as leave no more parts than workgroups run at once.

@@ -430,10 +430,11 @@ hipError_t launch_edit(hipStream_t s, const DevStep* step,
 
 // ---- a step of many requests ----------------------------------------------
 // Caches in pages (frz_pages), and where a row's are found (batch_rules.h).
+enum CacheFormat : int { kCacheF16, kCacheBf16, kCacheI8 };
 struct PagedCache {
-  uint16_t* keys;
-  uint16_t* values;
-  bool bf16;  // else F16
+  void* keys;
+  void* values;
+  CacheFormat format;
   uint32_t kv_heads;
   uint32_t head_dim;
   uint32_t page_slots;
@@ -442,6 +443,9 @@ struct PagedCache {
   const uint32_t* table;
   uint32_t sequences;
   uint32_t width;
+  float* key_scales;  // of 8 bits: [page][block of 16 slots][head]
+  float* value_scales;
+  uint64_t scale_stride;  // scales
 };
 
 struct PagedRopeArgs {
@@ -463,6 +467,20 @@ struct PagedRopeArgs {
   uint32_t rows;
 };
 hipError_t launch_paged_rope(hipStream_t s, const PagedRopeArgs& a);
+// The same into a cache of 8 bits (launch_paged_rope calls it).
+hipError_t launch_paged_rope_i8(hipStream_t s, const PagedRopeArgs& a);
+
+struct PagedReadArgs {
+  PagedCache cache;
+  const uint32_t* sequences;  // null: row r's is r
+  const uint32_t* positions;
+  int format;  // GGUF's: 0 F32, 1 F16, 30 BF16
+  void* keys;
+  void* values;
+  uint64_t stride;  // values
+  uint32_t rows;
+};
+hipError_t launch_paged_read(hipStream_t s, const PagedReadArgs& a);
 
 struct PagedAttentionArgs {
   PagedCache cache;
@@ -474,6 +492,7 @@ struct PagedAttentionArgs {
   uint32_t out_stride;
   uint32_t query_heads;
   uint32_t window;
+  uint32_t sinks;
   float scale_log2e;
   uint32_t rows;
   // The states of rows cut into several parts, at most kMostJoinedParts of them
@@ -490,7 +509,7 @@ constexpr int kAttentionWorkgroups = 4;  // a compute unit's at once, at most
 constexpr int kMostJoinedParts = 3 * kAttentionWorkgroups * kMostComputeUnits;
 // Values of one head in all of their states: workgroups of a compute unit take
 // kAttentionWidth of them together, at most.
-constexpr int kAttentionWidth = 384;
+constexpr int kAttentionWidth = 512;
 constexpr int kMostStateValues = 3 * kAttentionWidth * kMostComputeUnits;
 hipError_t launch_paged_attention(hipStream_t s, const PagedAttentionArgs& a, int compute_units);
 

@@ -47,6 +47,8 @@
 // heads of 128 (70 MB), 20.6 us, 3.4 TB/s; one of 5,004 keys (5 MB) 11.0 us,
 // two launches of dependent loads.
 
+#include <type_traits>
+
 #include "batch_rules.h"
 #include "kernels.h"
 #include "numerics.h"
@@ -59,17 +61,22 @@ using namespace rules;
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 
 constexpr float kMinusInf = -__builtin_inff();
+constexpr float kLargest = 0x1.fffffep127f;
 // Rows of no more blocks than these, or blocks times head_dim, are not cut: see
 // launch_shape.
 constexpr uint64_t kWaveBlocks = 32, kFewValues = 2048, kManyValues = 8192;
 constexpr int kBufferWord3 = 0x00020000;  // raw 32-bit data
+constexpr float kLeastTop = 0x1p-126f;
+constexpr float kCodeUnit = 1024.0f;  // what a value's number of 8 bits is the 2^-10 of
 
-template <bool kBf16>
+template <CacheFormat kF>
 struct Types;
 template <>
-struct Types<false> {
+struct Types<kCacheF16> {
   typedef half8 vec;
   typedef _Float16 scalar;
   static constexpr int kParts = 2;
@@ -82,7 +89,7 @@ struct Types<false> {
   }
 };
 template <>
-struct Types<true> {
+struct Types<kCacheBf16> {
   typedef bf16x8 vec;
   typedef __bf16 scalar;
   static constexpr int kParts = 3;
@@ -95,51 +102,69 @@ struct Types<true> {
   }
 };
 
+// Numbers of 8 bits are F16 to their weights.
+template <>
+struct Types<kCacheI8> : Types<kCacheF16> {
+  static constexpr int kDigits = 4;    // of a query
+  static constexpr int kQueryTop = 29;
+  static constexpr int kMostUp = 138;  // the query is at most 2^138 times itself
+  static __device__ __forceinline__ i32x4 mfma_digits(uint4 a, uint4 b, i32x4 c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a),
+                                                 __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
+  }
+};
+
 // The shapes a kernel is compiled for.
-template <int kD, bool kBf16, int kW>
+template <int kD, CacheFormat kF, int kW>
 struct Shape {
-  static constexpr int kParts = Types<kBf16>::kParts;
+  static constexpr bool kI8 = kF == kCacheI8;
+  static constexpr int kBytes = kI8 ? 1 : 2;                            // of a cached value
+  static constexpr int kParts = Types<kF>::kParts;
   static constexpr int kPerTile = 16 / kW;                              // parts a column tile holds
   static constexpr int kTiles = (kParts + kPerTile - 1) / kPerTile;     // column tiles
+  static constexpr int kQueryTiles = kI8 ? 4 / kPerTile : kTiles;
   // Tiles whose query is not scaled alike, and so whose sums are apart.
-  static constexpr int kScales = kBf16 ? 1 : kTiles;
+  static constexpr int kScales = kF == kCacheBf16 ? 1 : kQueryTiles;
   static constexpr bool kSpare = kTiles * kPerTile > kParts;            // columns of no part
-  static constexpr int kChunks = kD / 32;                               // of a key row
-  static constexpr int kVec = kD >= 128 ? 8 : 4;                        // values a lane loads at once
-  static constexpr int kSpans = kD / (16 * kVec);                       // of a value row
+  static constexpr int kPiece = 16 / kBytes;                            // of a key row that a lane loads
+  static constexpr int kChunks = kD / (4 * kPiece);                     // of a key row
+  // Values of a value row that a lane loads at once, and how often.
+  static constexpr int kVec = kI8 ? kD / 16 : kD >= 128 ? 8 : 4;
+  static constexpr int kSpans = kD / (16 * kVec);
+  static constexpr int kWords = (kVec * kBytes + 3) / 4;
 };
 
 // Workgroups a compute unit runs at once, by the registers that a shape takes.
-template <int kD, bool kBf16, int kW>
-constexpr int kWorkgroups = kD == 256   ? 1
-                            : kD == 128 ? (Shape<kD, kBf16, kW>::kTiles == 1 ? 3 : 2)
-                                        : (Shape<kD, kBf16, kW>::kTiles <= 2 ? 4 : 3);
-template <int kD, bool kBf16, int kW>
-constexpr bool kFits = kWorkgroups<kD, kBf16, kW> <= kAttentionWorkgroups &&
-                       kWorkgroups<kD, kBf16, kW> * kD <= kAttentionWidth;
+template <int kD, CacheFormat kF, int kW>
+constexpr int kWorkgroups = kD == 256   ? (kF == kCacheI8 && kW < 16 ? 2 : 1)
+                            : kD == 128 ? (Shape<kD, kF, kW>::kTiles == 1 ? 3 : 2)
+                                        : (Shape<kD, kF, kW>::kTiles <= 2 ? 4 : 3);
+template <int kD, CacheFormat kF, int kW>
+constexpr bool kFits = kWorkgroups<kD, kF, kW> <= kAttentionWorkgroups &&
+                       kWorkgroups<kD, kF, kW> * kD <= kAttentionWidth;
 
 // A column's part of a value: what rounding it left to the parts before, taken
 // off (`less` holds -1 for each of those, 0 for the others), rounded in its turn.
-template <bool kBf16>
+template <CacheFormat kF>
 struct Column {
+  static constexpr bool kBf16 = kF == kCacheBf16;
+  typedef typename Types<kF>::scalar T;
   float keep;     // 1; 0 for a column past the format's parts
   float less[2];
   float scale;    // of a query's part
   Column() = default;
   __device__ __forceinline__ explicit Column(int part) {
-    keep = part < Types<kBf16>::kParts ? 1.0f : 0.0f;
+    keep = part < Types<kF>::kParts ? 1.0f : 0.0f;
     less[0] = part >= 1 ? -1.0f : 0.0f;
     less[1] = part >= 2 ? -1.0f : 0.0f;
-    scale = !kBf16 && part == 1 ? Types<kBf16>::kPartScale : 1.0f;
+    scale = !kBf16 && part == 1 ? Types<kF>::kPartScale : 1.0f;
   }
-  __device__ __forceinline__ typename Types<kBf16>::scalar part_of(float x) const {
-    typedef typename Types<kBf16>::scalar T;
+  __device__ __forceinline__ T part_of(float x) const {
     x = fmaf_(less[0], (float)(T)x, x);
     if constexpr (kBf16) x = fmaf_(less[1], (float)(T)x, x);
     return (T)x;
   }
-  __device__ __forceinline__ typename Types<kBf16>::scalar scaled_part_of(float x) const {
-    typedef typename Types<kBf16>::scalar T;
+  __device__ __forceinline__ T scaled_part_of(float x) const {
     if constexpr (kBf16) return part_of(x);
     return (T)(fmaf_(less[0], (float)(T)x, x) * scale);
   }
@@ -226,7 +251,8 @@ __device__ __forceinline__ bool find_part(const PagedAttentionArgs& a, uint32_t 
   for (int i = 0; i < kPer; ++i) {
     if ((uint32_t)lane * kPer + i >= a.rows) position[i] = kNone;
     const uint32_t held = sequence[i] < a.cache.sequences ? capacity : 0;
-    blocks[i] = position[i] == kNone ? 0 : row_blocks(key_range(position[i], a.window, held));
+    blocks[i] =
+        position[i] == kNone ? 0 : row_blocks(key_range(position[i], a.window, held, a.sinks));
     mine += blocks[i];
   }
   const uint32_t all = lane_of(wave_sum_to(mine), 63);
@@ -284,14 +310,14 @@ __device__ __forceinline__ bool find_part(const PagedAttentionArgs& a, uint32_t 
   return true;
 }
 
-template <int kD, bool kBf16, int kW, int kWaves, bool kWhole>
-__global__ __launch_bounds__(64 * kWaves, (kWorkgroups<kD, kBf16, kW>))
+template <int kD, CacheFormat kF, int kW, int kWaves, bool kWhole>
+__global__ __launch_bounds__(64 * kWaves, (kWorkgroups<kD, kF, kW>))
 void paged_attention_kernel(PagedAttentionArgs a) {
-  typedef Shape<kD, kBf16, kW> S;
-  typedef Types<kBf16> T;
+  typedef Shape<kD, kF, kW> S;
+  typedef Types<kF> T;
   constexpr int kPitch = kD + 8;  // floats a head's outputs take in LDS
   __shared__ __attribute__((aligned(16))) float joined_out[kWaves][kW * kPitch];
-  __shared__ float joined_m[kWaves][kW], joined_l[kWaves][kW];
+  __shared__ float joined_m[kWaves][kW], joined_l[kWaves][kW], joined_top[kWaves];
   const int lane = threadIdx.x & 63;
   const uint32_t wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int n = lane & 15, g = lane >> 4;
@@ -321,76 +347,96 @@ void paged_attention_kernel(PagedAttentionArgs a) {
   // The part's keys and the wave's blocks of them.
   const uint32_t held = part.sequence < a.cache.sequences
                             ? a.cache.width * a.cache.page_slots : 0;
-  const KeyRange keys = key_range(part.position, a.window, held);
-  const uint32_t base_block = keys.first / kBlockKeys;
-  const uint32_t last_block = base_block + min((part.index + 1) * part.chunk, row_blocks(keys));
-  const uint32_t first_block = base_block + part.index * part.chunk;
+  const KeyRange keys = key_range(part.position, a.window, held, a.sinks);
+  const uint32_t last_block = min((part.index + 1) * part.chunk, row_blocks(keys));
+  const uint32_t first_block = part.index * part.chunk;
 
   // The wave's next 32 blocks' pages, a lane a half block of 16 keys: where
-  // that half's first key lies in the pool, in values, or ~0.
-  const uint32_t row_values = a.cache.kv_heads * kD, row_bytes = 2 * row_values;
-  auto find_pages = [&](uint32_t block) {
-    const uint32_t key = (block + kWaves * (lane >> 1)) * kBlockKeys + 16 * (lane & 1);
-    uint64_t at = ~0ull;
-    if (key < keys.end && key + 16 > keys.first) {
+  // that half's first key lies in the pool, in values, or ~0; of 8 bits its
+  // keys' and values' scales too.
+  const uint32_t row_values = a.cache.kv_heads * kD, row_bytes = S::kBytes * row_values;
+  uint64_t pages = ~0ull;
+  float key_scales = 0.0f, value_scales = 0.0f;
+  auto find_pages = [&](uint32_t counted) {
+    const BlockKeys b = block_keys(keys, counted + kWaves * (lane >> 1));
+    const uint32_t key = b.block * kBlockKeys + 16 * (lane & 1);
+    pages = ~0ull;
+    key_scales = value_scales = 0.0f;
+    if (key < b.end && key + 16 > b.first) {
       const uint32_t index = key / a.cache.page_slots;
       const uint32_t page = page_at(a.cache.table, a.cache.sequences, a.cache.width,
                                     a.cache.pages, part.sequence, index);
-      if (page != kNone)
-        at = page * a.cache.page_stride + (uint64_t)(key - index * a.cache.page_slots) * row_values;
+      if (page != kNone) {
+        const uint32_t slot = key - index * a.cache.page_slots;
+        pages = page * a.cache.page_stride + (uint64_t)slot * row_values;
+        if constexpr (S::kI8) {
+          const uint64_t at = page * a.cache.scale_stride +
+                              (uint64_t)(slot / kScaleSlots) * a.cache.kv_heads + kv;
+          key_scales = a.cache.key_scales[at];
+          value_scales = a.cache.value_scales[at];
+        }
+      }
     }
-    return at;
   };
   uint32_t block = first_block + wave;
-  uint64_t pages = find_pages(block);
+  find_pages(block);
 
   // The query's columns: column n of tile t is part t kPerTile + n / W of
   // head n % W; a column past the heads takes the first one's query.
   const uint32_t head = n % kW;
-  Column<kBf16> columns[S::kTiles];
+  Column<kF> columns[S::kTiles];
 #pragma unroll
-  for (int t = 0; t < S::kTiles; ++t) columns[t] = Column<kBf16>(t * S::kPerTile + n / kW);
-  float x[S::kChunks][8];
+  for (int t = 0; t < S::kTiles; ++t) columns[t] = Column<kF>(t * S::kPerTile + n / kW);
+  float x[S::kChunks][S::kPiece];
   {
     const float* src =
         a.query + (uint64_t)part.row * a.q_stride + (uint64_t)(head0 + (head < heads ? head : 0)) * kD;
 #pragma unroll
-    for (int c = 0; c < S::kChunks; ++c) {
-      const float4 lo = *reinterpret_cast<const float4*>(src + 32 * c + 8 * g);
-      const float4 hi = *reinterpret_cast<const float4*>(src + 32 * c + 8 * g + 4);
-      const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    for (int c = 0; c < S::kChunks; ++c)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[c][i] = v[i];
-    }
+      for (int i = 0; i < S::kPiece; i += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(src + S::kPiece * (4 * c + g) + i);
+        x[c][i] = v.x;
+        x[c][i + 1] = v.y;
+        x[c][i + 2] = v.z;
+        x[c][i + 3] = v.w;
+      }
   }
 
-  const uint16_t* key_pool = a.cache.keys + (uint64_t)kv * kD;
-  const uint16_t* value_pool = a.cache.values + (uint64_t)kv * kD;
+  const uint32_t head_bytes = S::kBytes * kD * kv;
+  const uint8_t* key_pool = static_cast<const uint8_t*>(a.cache.keys) + head_bytes;
+  const uint8_t* value_pool = static_cast<const uint8_t*>(a.cache.values) + head_bytes;
 
   // A block: where the rows that are read of each of its halves begin, and
   // which of its 16 keys these are, [lo, hi).
   struct Block {
     uint64_t at[2];
     int lo[2], hi[2];
+    float key_scale[2], value_scale[2];  // of 8 bits
   };
-  auto locate = [&](uint32_t b, uint32_t turn, Block* k) {
+  auto locate = [&](uint32_t counted, uint32_t turn, Block* k) {
+    const BlockKeys b = block_keys(keys, counted);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const uint64_t page = (uint64_t)lane_of((uint32_t)(pages >> 32), 2 * turn + h) << 32 |
                             lane_of((uint32_t)pages, 2 * turn + h);
-      const int key = (int)(b * kBlockKeys + 16 * h);
-      k->lo[h] = max(0, (int)keys.first - key);
-      k->hi[h] = page == ~0ull ? 0 : min(16, (int)keys.end - key);
+      const int key = (int)(b.block * kBlockKeys + 16 * h);
+      k->lo[h] = max(0, (int)b.first - key);
+      k->hi[h] = page == ~0ull ? 0 : min(16, (int)b.end - key);
       const bool some = k->lo[h] < k->hi[h];
       k->at[h] = some ? page + (uint64_t)k->lo[h] * row_values : 0;
       k->hi[h] = some ? k->hi[h] : k->lo[h];
+      if constexpr (S::kI8) {
+        k->key_scale[h] = bits_to_float(lane_of(float_to_bits(key_scales), 2 * turn + h));
+        k->value_scale[h] = bits_to_float(lane_of(float_to_bits(value_scales), 2 * turn + h));
+      }
     }
     return k->lo[0] < k->hi[0] || k->lo[1] < k->hi[1];
   };
   // Rows come through a buffer of just those that are read: a lane whose row is
   // before its start or past its end gets zeros, and no memory is touched.
-  auto rows_of = [&](const uint16_t* pool, const Block& k, int h) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(pool + k.at[h]), 0,
+  auto rows_of = [&](const uint8_t* pool, const Block& k, int h) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(pool + S::kBytes * k.at[h]), 0,
                                              (k.hi[h] - k.lo[h]) * (int)row_bytes, kBufferWord3);
   };
   uint4 key_rows[2][S::kChunks];
@@ -412,16 +458,20 @@ void paged_attention_kernel(PagedAttentionArgs a) {
       const __amdgpu_buffer_rsrc_t rows = rows_of(value_pool, k, h);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int at = (4 * g + e - k.lo[h]) * (int)row_bytes + 2 * S::kVec * n;
+        const int at = (4 * g + e - k.lo[h]) * (int)row_bytes + S::kBytes * S::kVec * n;
 #pragma unroll
         for (int s = 0; s < S::kSpans; ++s) {
-          if constexpr (S::kVec == 8) {
+          if constexpr (S::kWords == 4) {
             value_rows[h][e][s] = __builtin_bit_cast(
                 uint4, __builtin_amdgcn_raw_buffer_load_b128(rows, at + 256 * s, 0, 0));
-          } else {
+          } else if constexpr (S::kWords == 2) {
             const uint2 v = __builtin_bit_cast(
                 uint2, __builtin_amdgcn_raw_buffer_load_b64(rows, at, 0, 0));
             value_rows[h][e][s] = make_uint4(v.x, v.y, 0, 0);
+          } else {
+            value_rows[h][e][s] = make_uint4(
+                __builtin_bit_cast(uint32_t, __builtin_amdgcn_raw_buffer_load_b32(rows, at, 0, 0)),
+                0, 0, 0);
           }
         }
       }
@@ -434,6 +484,8 @@ void paged_attention_kernel(PagedAttentionArgs a) {
 #pragma unroll
     for (int j = 0; j < S::kVec; ++j) out[s][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   float m = kMinusInf, l = 0.0f;  // m less T::kWeightScale, once there is a key
+  // Of 8 bits: the largest of the values' scales so far, that the outputs are in.
+  float top_scale = kLeastTop, each_top = 1.0f / kLeastTop;
 
   uint32_t turn = 0;
   Block now, next;
@@ -442,27 +494,75 @@ void paged_attention_kernel(PagedAttentionArgs a) {
   auto seek = [&](Block* k) {
     for (; block < last_block; block += kWaves, ++turn) {
       if (turn == 32) {
-        pages = find_pages(block);
+        find_pages(block);
         turn = 0;
       }
       if (locate(block, turn, k)) return true;
     }
     k->at[0] = k->at[1] = 0;
     k->lo[0] = k->lo[1] = k->hi[0] = k->hi[1] = 0;  // no row
+    if constexpr (S::kI8)
+      k->key_scale[0] = k->key_scale[1] = k->value_scale[0] = k->value_scale[1] = 0.0f;
     return false;
   };
   if (seek(&now)) {
     load_keys(now);
     load_values(now);
     hold();
-    float scale[S::kTiles];  // what turns the scaled query's products into log2 units
-    uint4 q[S::kTiles][S::kChunks];
-    {
+    float scale[S::kQueryTiles];  // what turns the scaled query's products into log2 units
+    float key_back = 0.0f;        // of 8 bits: the key's scale aside
+    uint4 q[S::kQueryTiles][S::kChunks];
+    if constexpr (S::kI8) {
+      // The query as whole numbers below 2^30, four digits of -128 to 127 each:
+      // adding 128 of every digit makes them a word's bytes, 128 too large each,
+      // which flipping the bytes' top bits takes off again.
+      float most = 0.0f, bad = 0.0f;  // not 0 but NaN past F32's numbers
+#pragma unroll
+      for (int c = 0; c < S::kChunks; ++c)
+#pragma unroll
+        for (int i = 0; i < S::kPiece; ++i) {
+          most = __builtin_fmaxf(most, __builtin_fabsf(x[c][i]));
+          bad = fmaf_(x[c][i], 0.0f, bad);
+        }
+      most = across_groups(most, [](float p, float r) { return __builtin_fmaxf(p, r); });
+      bad = across_groups(bad, [](float p, float r) { return p + r; });
+      int up = 127 + T::kQueryTop - (int)(float_to_bits(most) >> 23);
+      up = up > T::kMostUp ? T::kMostUp : up;
+      const int far = up > 100 ? up - 100 : 0;  // in two steps, as 2^138 is past F32
+      const float factor = bits_to_float((uint32_t)(127 + up - far) << 23);
+      const float again = bits_to_float((uint32_t)(127 + far) << 23);
+      // 2^12 here and 2^-12 in the digits' scales keep both ordinary numbers.
+      key_back = a.scale_log2e * bits_to_float((uint32_t)(127 + 12 - up) << 23) + bad;
+#pragma unroll
+      for (int t = 0; t < S::kQueryTiles; ++t) {
+        const uint32_t digit = t * S::kPerTile + n / kW;
+        scale[t] = bits_to_float((127 - 12 + 8 * digit) << 23);
+        // Byte `digit` of two words, next to each other.
+        const uint32_t pick = digit | (4 + digit) << 8 | 0x0C0C0000u;
+#pragma unroll
+        for (int c = 0; c < S::kChunks; ++c) {
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t z[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int whole = (int)rint_(x[c][4 * i + j] * factor * again);
+              z[j] = ((uint32_t)whole + 0x80808080u) ^ 0x80808080u;
+            }
+            w[i] = __builtin_amdgcn_perm(z[1], z[0], pick) |
+                   __builtin_amdgcn_perm(z[3], z[2], pick) << 16;
+          }
+          q[t][c] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+    } else {
       float most = 0.0f;
 #pragma unroll
       for (int c = 0; c < S::kChunks; ++c)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) most = __builtin_fmaxf(most, __builtin_fabsf(x[c][i]));
+        for (int i = 0; i < S::kPiece; ++i)
+          most = __builtin_fmaxf(most, __builtin_fabsf(x[c][i]));
       most = across_groups(most, [](float p, float r) { return __builtin_fmaxf(p, r); });
       // 2^up takes the largest to its place; zeros and the smallest (and for
       // BF16 the largest) values as far as both factors, and the scale with its
@@ -485,17 +585,19 @@ void paged_attention_kernel(PagedAttentionArgs a) {
       }
     }
     for (bool more = true; more;) {
-      f32x4 scores[2][S::kScales];
+      typedef typename std::conditional<S::kI8, i32x4, f32x4>::type Sums;
+      Sums scores[2][S::kScales];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int i = 0; i < S::kScales; ++i) scores[h][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = 0; i < S::kScales; ++i) scores[h][i] = Sums{0, 0, 0, 0};
 #pragma unroll
         for (int c = 0; c < S::kChunks; ++c)
 #pragma unroll
-          for (int t = 0; t < S::kTiles; ++t) {
-            f32x4& sum = scores[h][t % S::kScales];
-            sum = T::mfma(key_rows[h][c], q[t][c], sum);
+          for (int t = 0; t < S::kQueryTiles; ++t) {
+            Sums& sum = scores[h][t % S::kScales];
+            if constexpr (S::kI8) sum = T::mfma_digits(key_rows[h][c], q[t][c], sum);
+            else sum = T::mfma(key_rows[h][c], q[t][c], sum);
           }
       }
       hold();
@@ -509,17 +611,25 @@ void paged_attention_kernel(PagedAttentionArgs a) {
 
       float most = kMinusInf, weight[8];  // scores first
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h) {
+        float back = 0.0f;
+        if constexpr (S::kI8) {
+          // A product past F32 of a query and numbers that are all 0 is 0.
+          back = key_back * now.key_scale[h];
+          back = __builtin_fminf(__builtin_fmaxf(back, -kLargest), kLargest) + (key_back - key_back);
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float s = scores[h][0][e] * scale[0];
+          float s = (float)scores[h][0][e] * scale[0];
 #pragma unroll
-          for (int i = 1; i < S::kScales; ++i) s = fmaf_(scores[h][i][e], scale[i], s);
+          for (int i = 1; i < S::kScales; ++i) s = fmaf_((float)scores[h][i][e], scale[i], s);
           s = across_columns<kW>(s);
+          if constexpr (S::kI8) s *= back;
           const bool live = 4 * g + e >= now.lo[h] && 4 * g + e < now.hi[h];
           weight[4 * h + e] = live ? s : kMinusInf;
           most = __builtin_fmaxf(most, weight[4 * h + e]);
         }
+      }
       most = across_groups(most, [](float p, float r) { return __builtin_fmaxf(p, r); });
       // A block that is worked on holds a key, so `most` is a number but where
       // scores are not.
@@ -538,6 +648,22 @@ void paged_attention_kernel(PagedAttentionArgs a) {
         weight[i] = __builtin_amdgcn_exp2f(weight[i] - m);
         l += weight[i];
       }
+      if constexpr (S::kI8) {
+        // A value's weight has its block's scale in it, over the largest so far.
+        const float here = __builtin_fmaxf(__builtin_fabsf(now.value_scale[0]),
+                                           __builtin_fabsf(now.value_scale[1]));
+        if (__ballot(here > top_scale)) {
+          const float old = top_scale / here;
+#pragma unroll
+          for (int s = 0; s < S::kSpans; ++s)
+#pragma unroll
+            for (int j = 0; j < S::kVec; ++j) out[s][j] *= old;
+          top_scale = here;
+          each_top = 1.0f / here;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) weight[i] *= now.value_scale[i / 4] * each_top;
+      }
       uint4 w[S::kTiles];
 #pragma unroll
       for (int t = 0; t < S::kTiles; ++t) {
@@ -553,13 +679,25 @@ void paged_attention_kernel(PagedAttentionArgs a) {
 #pragma unroll
         for (int j = 0; j < S::kVec; ++j) {
           // The lane's 8 keys at dimension j of its span.
-          const uint32_t select = j & 1 ? 0x07060302u : 0x05040100u;
+          constexpr int kIn = 4 / S::kBytes;  // values a word holds
           auto word = [&](int h, int e) {
             const uint4& r = value_rows[h][e][s];
-            return (j >> 1) == 0 ? r.x : (j >> 1) == 1 ? r.y : (j >> 1) == 2 ? r.z : r.w;
+            return j / kIn == 0 ? r.x : j / kIn == 1 ? r.y : j / kIn == 2 ? r.z : r.w;
           };
           auto pair = [&](int h, int e) {
-            return __builtin_amdgcn_perm(word(h, e + 1), word(h, e), select);
+            if constexpr (S::kI8) {
+              // Bytes of 0 to 255, as F16's smallest values u 2^-24: to (u - 128) 2^-10.
+              const uint32_t select = 0x0C040C00u + 0x00010001u * (j % 4);
+              const half2v u = __builtin_bit_cast(
+                  half2v, __builtin_amdgcn_perm(word(h, e + 1) ^ 0x80808080u,
+                                                word(h, e) ^ 0x80808080u, select));
+              const _Float16 up = (_Float16)16384.0f, less = (_Float16)-0.125f;
+              return __builtin_bit_cast(
+                  uint32_t, __builtin_elementwise_fma(u, half2v{up, up}, half2v{less, less}));
+            } else {
+              const uint32_t select = j & 1 ? 0x07060302u : 0x05040100u;
+              return __builtin_amdgcn_perm(word(h, e + 1), word(h, e), select);
+            }
           };
           const uint4 v = make_uint4(pair(0, 0), pair(0, 2), pair(1, 0), pair(1, 2));
 #pragma unroll
@@ -580,6 +718,7 @@ void paged_attention_kernel(PagedAttentionArgs a) {
     joined_m[wave][n] = m;
     joined_l[wave][n] = l;
   }
+  if (S::kI8 && lane == 0) joined_top[wave] = top_scale;
 #pragma unroll
   for (int s = 0; s < S::kSpans; ++s)
 #pragma unroll
@@ -601,6 +740,9 @@ void paged_attention_kernel(PagedAttentionArgs a) {
     float top = joined_m[0][h];
 #pragma unroll
     for (uint32_t w = 1; w < kWaves; ++w) top = __builtin_fmaxf(top, joined_m[w][h]);
+    float widest = joined_top[0];
+#pragma unroll
+    for (uint32_t w = 1; w < kWaves; ++w) widest = __builtin_fmaxf(widest, joined_top[w]);
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float weights = 0.0f;
 #pragma unroll
@@ -609,17 +751,22 @@ void paged_attention_kernel(PagedAttentionArgs a) {
       const float f = top == kMinusInf ? 0.0f : __builtin_amdgcn_exp2f(joined_m[w][h] - top);
       const float4 o = *reinterpret_cast<const float4*>(&joined_out[w][h * kPitch + d]);
       weights = fmaf_(joined_l[w][h], f, weights);
-      sum.x = fmaf_(o.x, f, sum.x);
-      sum.y = fmaf_(o.y, f, sum.y);
-      sum.z = fmaf_(o.z, f, sum.z);
-      sum.w = fmaf_(o.w, f, sum.w);
+      const float by = S::kI8 ? f * (joined_top[w] / widest) : f;
+      sum.x = fmaf_(o.x, by, sum.x);
+      sum.y = fmaf_(o.y, by, sum.y);
+      sum.z = fmaf_(o.z, by, sum.z);
+      sum.w = fmaf_(o.w, by, sum.w);
+    }
+    if (S::kI8 || whole) {
+      // (Of 8 bits a part's outputs too: their sums' range is the scales'.)
+      const float f = weights == 0.0f ? 0.0f : S::kI8 ? kCodeUnit / weights : 1.0f / weights;
+      const float unit = S::kI8 ? widest : 1.0f;
+      sum.x = sum.x * f * unit;
+      sum.y = sum.y * f * unit;
+      sum.z = sum.z * f * unit;
+      sum.w = sum.w * f * unit;
     }
     if (whole) {
-      const float f = weights == 0.0f ? 0.0f : 1.0f / weights;
-      sum.x *= f;
-      sum.y *= f;
-      sum.z *= f;
-      sum.w *= f;
       *reinterpret_cast<float4*>(a.out + (uint64_t)part.row * a.out_stride +
                                  (uint64_t)(head0 + h) * kD + d) = sum;
     } else {
@@ -640,7 +787,7 @@ void paged_attention_kernel(PagedAttentionArgs a) {
 // launch, but read all of a row's states, 640 KB for 157 parts of four heads,
 // through one compute unit: 16 us.)
 constexpr uint32_t kJoinWaves = 4, kThreads = 64 * kJoinWaves, kJoinGroups = kThreads / 16;
-template <int kD>
+template <int kD, bool kI8>
 __global__ __launch_bounds__(kThreads) void paged_attention_join_kernel(PagedAttentionArgs a) {
   __shared__ float wave_top[kJoinWaves], wave_sum[kJoinWaves];
   __shared__ float factors[kMostJoinedParts];
@@ -666,17 +813,19 @@ __global__ __launch_bounds__(kThreads) void paged_attention_join_kernel(PagedAtt
       const float2 s =
           *reinterpret_cast<const float2*>(a.stats + 2 * (first + (uint64_t)p * kHeadBlock));
       const float f = top == kMinusInf ? 0.0f : __builtin_amdgcn_exp2f(s.x - top);
-      factors[p] = f;
+      factors[p] = kI8 ? f * s.y : f;  // of 8 bits a part's outputs are over its weights
       weights = fmaf_(s.y, f, weights);
     }
     for (int o = 32; o > 0; o >>= 1) weights += __shfl_xor(weights, o);
     if (lane == 0) wave_sum[wave] = weights;
     __syncthreads();
     const uint32_t group = t / 16;
+    const float l = wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3];
+    const float each = kI8 && l != 0.0f ? 1.0f / l : 1.0f;  // so that no sum is past the outputs
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 8
     for (uint32_t p = group; p < parts; p += kJoinGroups) {
-      const float f = factors[p];
+      const float f = factors[p] * each;
       const float4 o = *reinterpret_cast<const float4*>(
           a.states + (first + (uint64_t)p * kHeadBlock) * kD + d);
       sum.x = fmaf_(o.x, f, sum.x);
@@ -691,18 +840,17 @@ __global__ __launch_bounds__(kThreads) void paged_attention_join_kernel(PagedAtt
       const float* column = reinterpret_cast<const float*>(&sums[0][0]) + t;
       float x = 0.0f;
       for (uint32_t k = 0; k < kJoinGroups; ++k) x += column[64 * k];
-      const float l = wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3];
       a.out[(uint64_t)record.x * a.out_stride + (uint64_t)((record.y & 0xFFFF) + h) * kD +
-            blockIdx.y % (kD / 64) * 64 + t] = l == 0.0f ? 0.0f : x / l;
+            blockIdx.y % (kD / 64) * 64 + t] = l == 0.0f ? 0.0f : kI8 ? x : x / l;
     }
   }
 }
 
-template <int kD, bool kBf16, int kW>
+template <int kD, CacheFormat kF, int kW>
 hipError_t launch_shape(hipStream_t s, PagedAttentionArgs a, uint32_t heads, int compute_units) {
-  static_assert(kFits<kD, kBf16, kW>, "the workspace holds their parts");
+  static_assert(kFits<kD, kF, kW>, "the workspace holds their parts");
   const uint32_t units = a.rows * a.units;
-  a.at_once = kWorkgroups<kD, kBf16, kW> * (uint32_t)compute_units;
+  a.at_once = kWorkgroups<kD, kF, kW> * (uint32_t)compute_units;
   // The most blocks that a row can have. Where they are few, each unit is one
   // workgroup's (kWhole), which then need not find its part, nor leave a state
   // to a second launch: always to kFewValues (64 requests of up to 250 keys, 256
@@ -715,31 +863,29 @@ hipError_t launch_shape(hipStream_t s, PagedAttentionArgs a, uint32_t heads, int
   // heads 128 wide: 214 by workgroups, 257 by waves). The host knows the table's
   // width and the window, not the rows: short rows in a wide table without a window
   // are cut (those 483 take the 127).
-  const uint64_t capacity = (uint64_t)a.cache.width * a.cache.page_slots;
-  const uint64_t held = (capacity + kBlockKeys - 1) / kBlockKeys;
-  const uint64_t seen = (uint64_t)a.window / kBlockKeys + 2;
-  const uint64_t blocks = held < seen ? held : seen;
+  const uint64_t blocks =
+      most_row_blocks((uint64_t)a.cache.width * a.cache.page_slots, a.window, a.sinks);
   if (units >= a.at_once && blocks <= kWaveBlocks) {
-    hipLaunchKernelGGL((paged_attention_kernel<kD, kBf16, kW, 1, true>), dim3(units), dim3(64), 0,
+    hipLaunchKernelGGL((paged_attention_kernel<kD, kF, kW, 1, true>), dim3(units), dim3(64), 0,
                        s, a);
     return hipGetLastError();
   }
   const bool few = 8 * units < 3 * (uint32_t)compute_units;
   if (blocks * kD <= (few ? kFewValues : kManyValues)) {
-    hipLaunchKernelGGL((paged_attention_kernel<kD, kBf16, kW, kPartWaves, true>), dim3(units),
+    hipLaunchKernelGGL((paged_attention_kernel<kD, kF, kW, kPartWaves, true>), dim3(units),
                        dim3(64 * kPartWaves), 0, s, a);
     return hipGetLastError();
   }
   // No more parts than the rows have blocks.
   const uint64_t fill = units * blocks;
   const uint64_t bound = most_parts(units, a.at_once);
-  hipLaunchKernelGGL((paged_attention_kernel<kD, kBf16, kW, kPartWaves, false>),
+  hipLaunchKernelGGL((paged_attention_kernel<kD, kF, kW, kPartWaves, false>),
                      dim3((uint32_t)(fill < bound ? fill : bound)), dim3(64 * kPartWaves), 0, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const uint32_t joins = most_joined_parts(units, a.at_once) / 2;
   const uint32_t records = units < joins ? units : joins;
-  hipLaunchKernelGGL(paged_attention_join_kernel<kD>,
+  hipLaunchKernelGGL((paged_attention_join_kernel<kD, kF == kCacheI8>),
                      dim3(records < 256 ? records : 256, heads * (kD / 64)), dim3(kThreads), 0, s,
                      a);
   return hipGetLastError();
@@ -750,13 +896,20 @@ hipError_t launch_heads(hipStream_t s, PagedAttentionArgs a, int compute_units) 
   const uint32_t group = a.query_heads / a.cache.kv_heads;
   const uint32_t heads = group < kHeadBlock ? group : kHeadBlock;
   a.units = a.cache.kv_heads * ((group + kHeadBlock - 1) / kHeadBlock);
-  if (a.cache.bf16) {
-    if (heads <= 4) return launch_shape<kD, true, 4>(s, a, heads, compute_units);
-    if (heads <= 8) return launch_shape<kD, true, 8>(s, a, heads, compute_units);
-    return launch_shape<kD, true, 16>(s, a, heads, compute_units);
+  switch (a.cache.format) {
+    case kCacheF16:
+      if (heads <= 8) return launch_shape<kD, kCacheF16, 8>(s, a, heads, compute_units);
+      return launch_shape<kD, kCacheF16, 16>(s, a, heads, compute_units);
+    case kCacheBf16:
+      if (heads <= 4) return launch_shape<kD, kCacheBf16, 4>(s, a, heads, compute_units);
+      if (heads <= 8) return launch_shape<kD, kCacheBf16, 8>(s, a, heads, compute_units);
+      return launch_shape<kD, kCacheBf16, 16>(s, a, heads, compute_units);
+    case kCacheI8:
+      if (heads <= 4) return launch_shape<kD, kCacheI8, 4>(s, a, heads, compute_units);
+      if (heads <= 8) return launch_shape<kD, kCacheI8, 8>(s, a, heads, compute_units);
+      return launch_shape<kD, kCacheI8, 16>(s, a, heads, compute_units);
   }
-  if (heads <= 8) return launch_shape<kD, false, 8>(s, a, heads, compute_units);
-  return launch_shape<kD, false, 16>(s, a, heads, compute_units);
+  return hipErrorInvalidValue;
 }
 
 }  // namespace

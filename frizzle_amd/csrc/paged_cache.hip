@@ -1,0 +1,342 @@
+// Caches in pages of 8 bits as a step writes them, and caches read back.
+//
+// Append. A block's 16 slots of one key-value head share a scale s, a power of
+// two, so the step's rows in a block are taken together by one workgroup, which
+// the first of them in the step finds itself to be:
+//   need = least 2^e with max |x| <= 127 2^e over those rows
+//   s'   = need where the block is begun anew, else max(s, need)
+//   x    -> rint(x / s'), what the block held -> rint(c s / s')
+// As scales grow by a factor of 2 at least, all roundings of a number come to
+// s' (1/2 + 1/4 + ...) at most. Of keys, x is the normed and turned row, with
+// rope_kernel's arithmetic and order of addition (rope_common.h); a head's D
+// values are D / 8 lanes, as in paged_rope.hip, and its rows the workgroup's
+// groups of lanes. Queries are turned by workgroups of their own.
+//
+// Read. A thread takes 16 numbers of a row's keys and of its values, both loads
+// under way together; what bounds it is memory.
+
+#include "batch_rules.h"
+#include "kernels.h"
+#include "rope_common.h"
+
+namespace frz {
+namespace {
+
+using namespace rules;
+
+constexpr uint32_t kThreads = 256;
+
+// A number of the block's scale, rounded to nearest even; NaN is 0.
+__device__ __forceinline__ int code_of(float x) {
+  const float top = (float)kMostCode;
+  return x == x ? (int)rint_(__builtin_fminf(__builtin_fmaxf(x, -top), top)) : 0;
+}
+__device__ __forceinline__ uint32_t codes_of(float4 v, float scale) {
+  return (uint32_t)(code_of(v.x / scale) & 0xFF) | (uint32_t)(code_of(v.y / scale) & 0xFF) << 8 |
+         (uint32_t)(code_of(v.z / scale) & 0xFF) << 16 | (uint32_t)code_of(v.w / scale) << 24;
+}
+// Four numbers by a scale `ratio` times as large (at most 1).
+__device__ __forceinline__ uint32_t rescaled(uint32_t codes, float ratio) {
+  uint32_t r = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    r |= ((uint32_t)(int)rint_((float)(int8_t)(codes >> 8 * i) * ratio) & 0xFF) << 8 * i;
+  return r;
+}
+
+__device__ __forceinline__ float most_of(float4 v) {
+  return __builtin_fmaxf(
+      __builtin_fmaxf(__builtin_fabsf(v.x), __builtin_fabsf(v.y)),
+      __builtin_fmaxf(__builtin_fabsf(v.z), __builtin_fabsf(v.w)));
+}
+
+// A lane's eight values of a head normed and turned to position p; all lanes of
+// a head call it together, those of a head that is not there with zeros.
+template <int kD>
+__device__ __forceinline__ void norm_and_turn(float4& va, float4& vb, const float* gain,
+                                              const float* turns_at, uint32_t l, uint32_t p,
+                                              float epsilon) {
+  constexpr int kLanes = kD / 8, kHalf = kD / 2;
+  const float4 ga = ld4f(gain + 4 * l), gb = ld4f(gain + kHalf + 4 * l);
+  const float4 turns = ld4f(turns_at + 4 * l);
+  float cosine[4], sine[4];
+  rope_angle(turns.x, p, &sine[0], &cosine[0]);
+  rope_angle(turns.y, p, &sine[1], &cosine[1]);
+  rope_angle(turns.z, p, &sine[2], &cosine[2]);
+  rope_angle(turns.w, p, &sine[3], &cosine[3]);
+  float squares = rope_lane_squares(va, vb);
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) squares = squares + __shfl_xor(squares, o);
+  rope_normalize(va, vb, squares, kD, epsilon, ga, gb);
+  rope_rotate(va, vb, 0, cosine, sine);
+}
+
+// blockIdx.y: the groups of query heads, then each head's keys, then its values.
+template <int kD>
+__global__ __launch_bounds__(kThreads) void paged_rope_i8_kernel(PagedRopeArgs a,
+                                                                 uint32_t query_groups) {
+  constexpr uint32_t kLanes = kD / 8, kHalf = kD / 2;
+  constexpr uint32_t kGroups = kThreads / kLanes;  // heads, or rows of a block, at once
+  constexpr uint32_t kTurns = kGroups < kScaleSlots ? kScaleSlots / kGroups : 1;
+  __shared__ uint32_t member[kScaleSlots];  // the row that writes a slot, and 1
+  __shared__ float wave_most[kThreads / 64];
+  const uint32_t row = blockIdx.x, t = threadIdx.x;
+  const uint32_t group = t / kLanes, l = t % kLanes;
+  const uint32_t p = a.positions[row];
+  if (p == kNone) return;
+
+  if (blockIdx.y < query_groups) {
+    const uint32_t h = blockIdx.y * kGroups + group;
+    const bool active = h < a.query_heads;
+    float4 va = make_float4(0.f, 0.f, 0.f, 0.f), vb = va;
+    if (active) {
+      const float* src = a.query + (uint64_t)row * a.q_stride + (uint64_t)h * kD;
+      va = ld4f(src + 4 * l);
+      vb = ld4f(src + kHalf + 4 * l);
+    }
+    norm_and_turn<kD>(va, vb, a.query_gain, a.turns, l, p, a.epsilon);
+    if (!active) return;
+    float* dst = a.roped + (uint64_t)row * a.roped_stride + (uint64_t)h * kD;
+    *reinterpret_cast<float4*>(dst + 4 * l) = va;
+    *reinterpret_cast<float4*>(dst + kHalf + 4 * l) = vb;
+    return;
+  }
+  const uint32_t part = blockIdx.y - query_groups;
+  const bool is_value = part >= a.cache.kv_heads;
+  const uint32_t kv = is_value ? part - a.cache.kv_heads : part;
+
+  // The step's rows of the block: the workgroup is that of the first of them. The
+  // row before, mostly of the same block in a prompt, spares the others the rest.
+  const uint32_t sequence = a.sequences ? a.sequences[row] : row;
+  const uint32_t block = p / kScaleSlots;
+  if (a.sequences && row > 0 && a.sequences[row - 1] == sequence) {
+    const uint32_t before = a.positions[row - 1];
+    if (before != kNone && before / kScaleSlots == block) return;
+  }
+  const uint32_t index = p / a.cache.page_slots;
+  const uint32_t page = page_at(a.cache.table, a.cache.sequences, a.cache.width, a.cache.pages,
+                                sequence, index);
+  if (page == kNone) return;
+  if (t < kScaleSlots) member[t] = 0;
+  __syncthreads();
+  bool later = false;
+  if (a.sequences) {
+    for (uint32_t r = t; r < a.rows; r += kThreads) {
+      const uint32_t at = a.positions[r];
+      if (at != kNone && at / kScaleSlots == block && a.sequences[r] == sequence) {
+        // Of rows at one position the last.
+        atomicMax(&member[at % kScaleSlots], r + 1);
+        later = later || r < row;
+      }
+    }
+  } else if (t == 0) {  // each row is its own request
+    member[p % kScaleSlots] = row + 1;
+  }
+  if (__syncthreads_or(later)) return;
+
+  const uint32_t first_slot = block * kScaleSlots - index * a.cache.page_slots;
+  uint8_t* codes = static_cast<uint8_t*>(is_value ? a.cache.values : a.cache.keys) +
+                   page * a.cache.page_stride +
+                   ((uint64_t)first_slot * a.cache.kv_heads + kv) * kD;
+  float* scale_at = (is_value ? a.cache.value_scales : a.cache.key_scales) +
+                    page * a.cache.scale_stride +
+                    (uint64_t)(first_slot / kScaleSlots) * a.cache.kv_heads + kv;
+  float scale = *scale_at;
+  if (member[0] || !(scale > 0.0f) || scale == __builtin_inff()) scale = 0.0f;
+
+  uint32_t from[kTurns];
+  float4 va[kTurns], vb[kTurns];
+  uint32_t ca[kTurns], cb[kTurns];  // what the block holds
+#pragma unroll
+  for (uint32_t i = 0; i < kTurns; ++i) {
+    const uint32_t slot = i * kGroups + group;
+    from[i] = slot < kScaleSlots ? member[slot] : 0;
+    va[i] = vb[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    ca[i] = cb[i] = 0;
+    if (from[i]) {
+      const float* src = (is_value ? a.value : a.key) + (uint64_t)(from[i] - 1) * a.kv_stride +
+                         (uint64_t)kv * kD;
+      va[i] = ld4f(src + 4 * l);
+      vb[i] = ld4f(src + kHalf + 4 * l);
+    } else if (slot < kScaleSlots) {
+      const uint8_t* src = codes + (uint64_t)slot * a.cache.kv_heads * kD;
+      ca[i] = *reinterpret_cast<const uint32_t*>(src + 4 * l);
+      cb[i] = *reinterpret_cast<const uint32_t*>(src + kHalf + 4 * l);
+    }
+  }
+  float most = 0.0f;
+#pragma unroll
+  for (uint32_t i = 0; i < kTurns; ++i) {
+    const uint32_t slot = i * kGroups + group;
+    if (!is_value)
+      norm_and_turn<kD>(va[i], vb[i], a.key_gain, a.turns, l, block * kScaleSlots + slot,
+                        a.epsilon);
+    if (from[i]) most = __builtin_fmaxf(most, __builtin_fmaxf(most_of(va[i]), most_of(vb[i])));
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) most = __builtin_fmaxf(most, __shfl_xor(most, o));
+  if (t % 64 == 0) wave_most[t / 64] = most;
+  __syncthreads();
+#pragma unroll
+  for (uint32_t w = 0; w < kThreads / 64; ++w) most = __builtin_fmaxf(most, wave_most[w]);
+  const float need = bits_to_float(block_scale_bits(float_to_bits(most)));
+  const float after = __builtin_fmaxf(scale, need);
+  const float ratio = after > 0.0f ? scale / after : 0.0f;
+  const float by = after > 0.0f ? after : 1.0f;  // all zeros: any
+#pragma unroll
+  for (uint32_t i = 0; i < kTurns; ++i) {
+    const uint32_t slot = i * kGroups + group;
+    if (slot >= kScaleSlots || (!from[i] && ratio == 1.0f)) continue;
+    uint8_t* dst = codes + (uint64_t)slot * a.cache.kv_heads * kD;
+    *reinterpret_cast<uint32_t*>(dst + 4 * l) =
+        from[i] ? codes_of(va[i], by) : rescaled(ca[i], ratio);
+    *reinterpret_cast<uint32_t*>(dst + kHalf + 4 * l) =
+        from[i] ? codes_of(vb[i], by) : rescaled(cb[i], ratio);
+  }
+  if (t == 0) *scale_at = after;
+}
+
+template <int kD>
+void launch_rope(hipStream_t s, const PagedRopeArgs& a) {
+  constexpr uint32_t kGroups = kThreads / (kD / 8);
+  const uint32_t groups = (a.query_heads + kGroups - 1) / kGroups;
+  hipLaunchKernelGGL(paged_rope_i8_kernel<kD>, dim3(a.rows, groups + 2 * a.cache.kv_heads),
+                     dim3(kThreads), 0, s, a, groups);
+}
+
+// ---- reading back --------------------------------------------------------------
+
+constexpr int kPiece = 16;  // values that a thread takes
+
+// A piece of a cache row in F32.
+template <CacheFormat kFrom>
+struct Piece {
+  uint4 raw[kFrom == kCacheI8 ? 1 : 2];
+  float scale;
+  __device__ __forceinline__ void load(const void* pool, uint64_t at, const float* scale_at) {
+    const uint4* src;
+    if constexpr (kFrom == kCacheI8) {
+      src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pool) + at);
+      scale = *scale_at;
+    } else {
+      src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(pool) + at);
+      raw[1] = src[1];
+    }
+    raw[0] = src[0];
+  }
+  __device__ __forceinline__ float get(int i) const {
+    const uint4 r = raw[kFrom == kCacheI8 ? 0 : i / 8];
+    const uint32_t words[4] = {r.x, r.y, r.z, r.w};
+    if constexpr (kFrom == kCacheI8)
+      return (float)(int8_t)(words[i / 4] >> 8 * (i % 4)) * scale;
+    const uint16_t half = (uint16_t)(words[i % 8 / 2] >> 16 * (i % 2));
+    if constexpr (kFrom == kCacheBf16) return bits_to_float((uint32_t)half << 16);
+    return (float)__builtin_bit_cast(_Float16, half);
+  }
+};
+
+template <int kTo>
+__device__ __forceinline__ uint16_t half_of(float x) {
+  if constexpr (kTo == 1) return f16_pack_device(x);
+  return __builtin_bit_cast(uint16_t, (__bf16)x);
+}
+
+template <CacheFormat kFrom, int kTo>
+__device__ __forceinline__ void store(void* to, uint64_t at, const Piece<kFrom>& piece, bool there) {
+  if constexpr (kTo == 0) {
+    float4* dst = reinterpret_cast<float4*>(static_cast<float*>(to) + at);
+#pragma unroll
+    for (int i = 0; i < kPiece / 4; ++i)
+      dst[i] = there ? make_float4(piece.get(4 * i), piece.get(4 * i + 1), piece.get(4 * i + 2),
+                                   piece.get(4 * i + 3))
+                     : make_float4(0.f, 0.f, 0.f, 0.f);
+  } else {
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(to) + at);
+#pragma unroll
+    for (int i = 0; i < kPiece / 8; ++i) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        w[j] = there ? half_of<kTo>(piece.get(8 * i + 2 * j)) |
+                           (uint32_t)half_of<kTo>(piece.get(8 * i + 2 * j + 1)) << 16
+                     : 0u;
+      dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
+template <CacheFormat kFrom, int kTo>
+__global__ __launch_bounds__(kThreads) void paged_read_kernel(PagedReadArgs a, uint32_t row_pieces,
+                                                              uint32_t rows_each) {
+  const uint32_t first = blockIdx.x * rows_each;
+  const uint32_t rows = min(rows_each, a.rows - first);
+  for (uint32_t i = blockIdx.y * kThreads + threadIdx.x; i < rows * row_pieces;
+       i += gridDim.y * kThreads) {
+    const uint32_t row = first + i / row_pieces, piece = i % row_pieces;
+    const uint32_t p = a.positions[row];
+    if (p == kNone) continue;
+    const uint32_t sequence = a.sequences ? a.sequences[row] : row;
+    const uint32_t index = p / a.cache.page_slots, slot = p - index * a.cache.page_slots;
+    const uint32_t page = page_at(a.cache.table, a.cache.sequences, a.cache.width, a.cache.pages,
+                                  sequence, index);
+    const bool there = page != kNone;
+    Piece<kFrom> key, value;
+    if (there) {
+      const uint64_t at = page * a.cache.page_stride +
+                          (uint64_t)slot * a.cache.kv_heads * a.cache.head_dim +
+                          (uint64_t)piece * kPiece;
+      const uint64_t scale = page * a.cache.scale_stride +
+                             (uint64_t)(slot / kScaleSlots) * a.cache.kv_heads +
+                             piece * kPiece / a.cache.head_dim;
+      key.load(a.cache.keys, at, a.cache.key_scales + scale);
+      value.load(a.cache.values, at, a.cache.value_scales + scale);
+    }
+    const uint64_t to = (uint64_t)row * a.stride + (uint64_t)piece * kPiece;
+    store<kFrom, kTo>(a.keys, to, key, there);
+    store<kFrom, kTo>(a.values, to, value, there);
+  }
+}
+
+template <CacheFormat kFrom, int kTo>
+void launch_read(hipStream_t s, const PagedReadArgs& a) {
+  // Whole rows of a workgroup, a piece a thread.
+  const uint32_t pieces = a.cache.kv_heads * a.cache.head_dim / kPiece;
+  const uint32_t rows = pieces < kThreads ? kThreads / pieces : 1;
+  const uint32_t split = (pieces + kThreads - 1) / kThreads;
+  hipLaunchKernelGGL((paged_read_kernel<kFrom, kTo>),
+                     dim3((a.rows + rows - 1) / rows, split), dim3(kThreads), 0, s, a, pieces, rows);
+}
+template <CacheFormat kFrom>
+hipError_t launch_read_to(hipStream_t s, const PagedReadArgs& a) {
+  switch (a.format) {
+    case 0: launch_read<kFrom, 0>(s, a); break;
+    case 1: launch_read<kFrom, 1>(s, a); break;
+    case 30: launch_read<kFrom, 30>(s, a); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_paged_rope_i8(hipStream_t s, const PagedRopeArgs& a) {
+  switch (a.cache.head_dim) {
+    case 64: launch_rope<64>(s, a); break;
+    case 128: launch_rope<128>(s, a); break;
+    case 256: launch_rope<256>(s, a); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_paged_read(hipStream_t s, const PagedReadArgs& a) {
+  if (a.rows == 0) return hipErrorInvalidValue;
+  switch (a.cache.format) {
+    case kCacheF16: return launch_read_to<kCacheF16>(s, a);
+    case kCacheBf16: return launch_read_to<kCacheBf16>(s, a);
+    case kCacheI8: return launch_read_to<kCacheI8>(s, a);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace frz

@@ -106,10 +106,11 @@ __global__ __launch_bounds__(256) void paged_rope_kernel(PagedRopeArgs a) {
     *reinterpret_cast<float4*>(dst + 4 * l) = va;
     *reinterpret_cast<float4*>(dst + kHalf + 4 * l) = vb;
   } else if (kept) {
-    uint16_t* dst = (is_value ? a.cache.values : a.cache.keys) + at + (uint64_t)kv * kD;
-    *reinterpret_cast<ushort4*>(dst + 4 * l) = a.cache.bf16 ? pack4_bf16(va) : pack4_f16(va);
-    *reinterpret_cast<ushort4*>(dst + kHalf + 4 * l) =
-        a.cache.bf16 ? pack4_bf16(vb) : pack4_f16(vb);
+    const bool bf16 = a.cache.format == kCacheBf16;
+    uint16_t* dst = static_cast<uint16_t*>(is_value ? a.cache.values : a.cache.keys) + at +
+                    (uint64_t)kv * kD;
+    *reinterpret_cast<ushort4*>(dst + 4 * l) = bf16 ? pack4_bf16(va) : pack4_f16(va);
+    *reinterpret_cast<ushort4*>(dst + kHalf + 4 * l) = bf16 ? pack4_bf16(vb) : pack4_f16(vb);
   }
 }
 
@@ -125,6 +126,7 @@ void launch_heads(hipStream_t s, const PagedRopeArgs& a) {
 
 hipError_t launch_paged_rope(hipStream_t s, const PagedRopeArgs& a) {
   if (a.rows == 0 || a.rows > kMostRows) return hipErrorInvalidValue;
+  if (a.cache.format == kCacheI8) return launch_paged_rope_i8(s, a);
   switch (a.cache.head_dim) {
     case 64: launch_heads<64>(s, a); break;
     case 128: launch_heads<128>(s, a); break;

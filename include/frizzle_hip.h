@@ -238,12 +238,16 @@ int frz_op_draw(frz_device* dev, const uint32_t* candidates_dev,
  * its steps on the stream), and with any device current. Pointers to floats
  * or 16-bit values must be multiples of 16 bytes and strides of 4 floats. */
 #define FRZ_FORMAT_F16 1
+#define FRZ_FORMAT_I8 24
 #define FRZ_FORMAT_BF16 30
 #define FRZ_NO_POSITION 0xFFFFFFFFu
 #define FRZ_NO_PAGE 0xFFFFFFFFu
 #define FRZ_NO_ADAPTER 0xFFFFFFFFu
 /* Caches in pages. Page p's slot s holds head h's key at keys + p *
- * page_stride + (s * kv_heads + h) * head_dim, its value likewise; a
+ * page_stride + (s * kv_heads + h) * head_dim, its value likewise, 16 bits each
+ * or 8: whole numbers of -127 to 127, times the scale at key_scales (or
+ * value_scales) + p * scale_stride + (s / 16) * kv_heads + h, which the block's
+ * 16 slots share. A
  * request's key at position j is in slot j % page_slots of the page that
  * table[request * width + j / page_slots] names. Requests may share pages
  * that they only read. An entry that names no page of the pool (FRZ_NO_PAGE,
@@ -252,16 +256,20 @@ int frz_op_draw(frz_device* dev, const uint32_t* candidates_dev,
 typedef struct frz_pages {
   void* keys;             /* dev */
   void* values;           /* dev */
-  int format;             /* FRZ_FORMAT_F16 or FRZ_FORMAT_BF16 */
+  int format;             /* FRZ_FORMAT_F16, FRZ_FORMAT_BF16 or FRZ_FORMAT_I8 */
   int kv_heads;           /* 1 to 1,024 */
   int head_dim;           /* 64, 128 or 256 */
   uint32_t page_slots;    /* a multiple of 16 */
   uint32_t pages;         /* pages in the pool */
-  uint64_t page_stride;   /* values from a page to the next, a multiple of 8;
-                           * pages * page_stride at most 2^48 */
+  uint64_t page_stride;   /* values from a page to the next, a multiple of 16
+                           * bytes; pages * page_stride at most 2^48 */
   const uint32_t* table;  /* dev: sequences rows of width entries */
   uint32_t sequences;
   uint32_t width;         /* width * page_slots at most 2^24 */
+  /* FRZ_FORMAT_I8 alone; not read otherwise. */
+  float* key_scales;      /* dev */
+  float* value_scales;    /* dev */
+  uint64_t scale_stride;  /* scales from a page to the next, as page_stride */
 } frz_pages;
 /* Each row's QK-norm and rope, its key and value appended to its request's
  * pages: frz_op_rope's arithmetic, bit for bit, at positions of the rows'
@@ -272,7 +280,16 @@ typedef struct frz_pages {
  * Keys and values round to the cache's format, to nearest even (F16
  * saturates at 65,504). Of rows at one request's position the last one's
  * stay; two requests must not append to a page that they share, nor one through
- * two entries of its row that name one page. */
+ * two entries of its row that name one page.
+ * Into 8 bits, a block (16 slots of a head's keys, or values) gets the least
+ * power of two, from 2^-126 to 2^121, by which none of its rows' values is past
+ * 127, or keeps its scale where that is larger: where the scale grows, what the
+ * block held goes by it as well. All numbers are rounded to nearest even; a
+ * number that came in earlier is off by less than the block's scale in all, one
+ * of this step by half of it. A block whose first slot is written is begun anew,
+ * and so is one whose scale is not above 0 and finite: nothing of what it held
+ * is left, slots not written are 0. Infinities count as the largest number, NaN
+ * as 0. */
 int frz_op_rope_paged(frz_device* dev, const frz_pages* cache, const uint32_t* sequences,
                       const uint32_t* positions, const float* turns, const float* query_gain,
                       const float* key_gain, const float* query, const float* key,
@@ -288,13 +305,34 @@ int frz_op_rope_paged(frz_device* dev, const frz_pages* cache, const uint32_t* s
  * or to 2^-23 of itself, or 2^-51 of its head's largest (F16): a score is off by
  * some 2^-22 of the sum of its products' sizes, and an output by twice as much of
  * the largest value that is read as its scores are off, and by 1e-6 of it.
- * A row with no key gets zeros. Cached values must be
+ * A row with no key gets zeros. Cached values, and scales, must be
  * finite where a row reads them, and may be anything elsewhere. out's rows are
- * out_stride floats apart; out must not overlap query. */
+ * out_stride floats apart; out must not overlap query.
+ * Over 8 bits keys and values are their numbers times any scales, and a query is
+ * held to 2^-30 of its head's largest value, or to 2^-139. */
 int frz_op_attention_paged(frz_device* dev, const frz_pages* cache, const uint32_t* sequences,
                            const uint32_t* positions, const float* query, int q_stride,
                            float* out, int out_stride, int query_heads, uint32_t window,
                            float scale, uint32_t rows);
+/* The same over the request's first `sinks` keys too, which stay visible however
+ * far the window has gone: a row reads those at [0, sinks) and at (position -
+ * window, position], each once. The pages between may be gone (FRZ_NO_PAGE in the
+ * table, or other requests'). */
+int frz_op_attention_paged_sinks(frz_device* dev, const frz_pages* cache,
+                                 const uint32_t* sequences, const uint32_t* positions,
+                                 const float* query, int q_stride, float* out, int out_stride,
+                                 int query_heads, uint32_t window, uint32_t sinks, float scale,
+                                 uint32_t rows);
+/* Reads a cache back: row r's key and value, at positions[r] of the request
+ * sequences[r] (null: request r), all heads, as kv_heads * head_dim values of
+ * `format` (F32, F16 or BF16) at keys and values + r * stride, for up to 2^24
+ * rows. Numbers of 8 bits are multiplied by their scales, in F32; all round to
+ * the format to nearest even (F16 saturates at 65,504). A key that is not there
+ * is zeros, a row at FRZ_NO_POSITION is left as it is. stride is a multiple of 8;
+ * keys, values and the cache must not overlap. */
+int frz_op_read_paged(frz_device* dev, const frz_pages* cache, const uint32_t* sequences,
+                      const uint32_t* positions, int format, void* keys, void* values,
+                      uint64_t stride, uint32_t rows);
 /* Low-rank adapters of a projection, in one pool: adapter a's down matrix is
  * rank rows of cols weights at down + a * rank * cols, its up matrix rows
  * rows of rank at up + a * rows * rank. Its own rank may be lower: only the
