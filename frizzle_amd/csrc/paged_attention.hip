@@ -136,7 +136,7 @@ struct Shape {
 
 // Workgroups a compute unit runs at once, by the registers that a shape takes.
 template <int kD, CacheFormat kF, int kW>
-constexpr int kWorkgroups = kD == 256   ? (kF == kCacheI8 && kW < 16 ? 2 : 1)
+constexpr int kWorkgroups = kD == 256   ? (1)
                             : kD == 128 ? (Shape<kD, kF, kW>::kTiles == 1 ? 3 : 2)
                                         : (Shape<kD, kF, kW>::kTiles <= 2 ? 4 : 3);
 template <int kD, CacheFormat kF, int kW>
@@ -187,6 +187,16 @@ template <int kShift>
 __device__ __forceinline__ float row_rotated(float x) {
   return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x),
                                                                0x120 + kShift, 0xF, 0xF, true));
+}
+
+// All 64 lanes' x, into each of them: by lanes 32, 16, 8 .. 1 away in turn.
+template <typename Op>
+__device__ __forceinline__ float across_wave(float x, Op op) {
+  x = across_groups(x, op);
+  x = op(x, row_rotated<8>(x));
+  x = op(x, row_rotated<4>(x));
+  x = op(x, row_rotated<2>(x));
+  return op(x, row_rotated<1>(x));
 }
 
 // A head's columns summed, into each of them.
@@ -412,7 +422,7 @@ void paged_attention_kernel(PagedAttentionArgs a) {
   struct Block {
     uint64_t at[2];
     int lo[2], hi[2];
-    float key_scale[2], value_scale[2];  // of 8 bits
+    uint32_t turn;  // of those whose pages are known
   };
   auto locate = [&](uint32_t counted, uint32_t turn, Block* k) {
     const BlockKeys b = block_keys(keys, counted);
@@ -426,11 +436,8 @@ void paged_attention_kernel(PagedAttentionArgs a) {
       const bool some = k->lo[h] < k->hi[h];
       k->at[h] = some ? page + (uint64_t)k->lo[h] * row_values : 0;
       k->hi[h] = some ? k->hi[h] : k->lo[h];
-      if constexpr (S::kI8) {
-        k->key_scale[h] = bits_to_float(lane_of(float_to_bits(key_scales), 2 * turn + h));
-        k->value_scale[h] = bits_to_float(lane_of(float_to_bits(value_scales), 2 * turn + h));
-      }
     }
+    k->turn = turn;
     return k->lo[0] < k->hi[0] || k->lo[1] < k->hi[1];
   };
   // Rows come through a buffer of just those that are read: a lane whose row is
@@ -439,12 +446,15 @@ void paged_attention_kernel(PagedAttentionArgs a) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(pool + S::kBytes * k.at[h]), 0,
                                              (k.hi[h] - k.lo[h]) * (int)row_bytes, kBufferWord3);
   };
+  // Where a lane's first row would begin, were it the first that is read.
+  const int key_at = n * (int)row_bytes + 16 * g;
+  const int value_at = 4 * g * (int)row_bytes + S::kBytes * S::kVec * n;
   uint4 key_rows[2][S::kChunks];
   auto load_keys = [&](const Block& k) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const __amdgpu_buffer_rsrc_t rows = rows_of(key_pool, k, h);
-      const int at = (n - k.lo[h]) * (int)row_bytes + 16 * g;
+      const int at = key_at - k.lo[h] * (int)row_bytes;
 #pragma unroll
       for (int c = 0; c < S::kChunks; ++c)
         key_rows[h][c] = __builtin_bit_cast(
@@ -458,7 +468,7 @@ void paged_attention_kernel(PagedAttentionArgs a) {
       const __amdgpu_buffer_rsrc_t rows = rows_of(value_pool, k, h);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int at = (4 * g + e - k.lo[h]) * (int)row_bytes + S::kBytes * S::kVec * n;
+        const int at = value_at + (e - k.lo[h]) * (int)row_bytes;
 #pragma unroll
         for (int s = 0; s < S::kSpans; ++s) {
           if constexpr (S::kWords == 4) {
@@ -501,8 +511,6 @@ void paged_attention_kernel(PagedAttentionArgs a) {
     }
     k->at[0] = k->at[1] = 0;
     k->lo[0] = k->lo[1] = k->hi[0] = k->hi[1] = 0;  // no row
-    if constexpr (S::kI8)
-      k->key_scale[0] = k->key_scale[1] = k->value_scale[0] = k->value_scale[1] = 0.0f;
     return false;
   };
   if (seek(&now)) {
@@ -516,23 +524,18 @@ void paged_attention_kernel(PagedAttentionArgs a) {
       // The query as whole numbers below 2^30, four digits of -128 to 127 each:
       // adding 128 of every digit makes them a word's bytes, 128 too large each,
       // which flipping the bytes' top bits takes off again.
-      float most = 0.0f, bad = 0.0f;  // not 0 but NaN past F32's numbers
+      float most = 0.0f;  // NaN where one is
 #pragma unroll
       for (int c = 0; c < S::kChunks; ++c)
 #pragma unroll
-        for (int i = 0; i < S::kPiece; ++i) {
-          most = __builtin_fmaxf(most, __builtin_fabsf(x[c][i]));
-          bad = fmaf_(x[c][i], 0.0f, bad);
-        }
-      most = across_groups(most, [](float p, float r) { return __builtin_fmaxf(p, r); });
-      bad = across_groups(bad, [](float p, float r) { return p + r; });
+        for (int i = 0; i < S::kPiece; ++i)
+          most = __builtin_elementwise_maximum(most, __builtin_fabsf(x[c][i]));
+      most = across_groups(most, [](float p, float r) { return __builtin_elementwise_maximum(p, r); });
       int up = 127 + T::kQueryTop - (int)(float_to_bits(most) >> 23);
       up = up > T::kMostUp ? T::kMostUp : up;
-      const int far = up > 100 ? up - 100 : 0;  // in two steps, as 2^138 is past F32
-      const float factor = bits_to_float((uint32_t)(127 + up - far) << 23);
-      const float again = bits_to_float((uint32_t)(127 + far) << 23);
       // 2^12 here and 2^-12 in the digits' scales keep both ordinary numbers.
-      key_back = a.scale_log2e * bits_to_float((uint32_t)(127 + 12 - up) << 23) + bad;
+      key_back = a.scale_log2e * __builtin_ldexpf(1.0f, 12 - up);
+      if (!(most <= kLargest)) key_back = __builtin_nanf("");
 #pragma unroll
       for (int t = 0; t < S::kQueryTiles; ++t) {
         const uint32_t digit = t * S::kPerTile + n / kW;
@@ -546,12 +549,10 @@ void paged_attention_kernel(PagedAttentionArgs a) {
           for (int i = 0; i < 4; ++i) {
             uint32_t z[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int whole = (int)rint_(x[c][4 * i + j] * factor * again);
-              z[j] = ((uint32_t)whole + 0x80808080u) ^ 0x80808080u;
-            }
-            w[i] = __builtin_amdgcn_perm(z[1], z[0], pick) |
-                   __builtin_amdgcn_perm(z[3], z[2], pick) << 16;
+            for (int j = 0; j < 4; ++j)
+              z[j] = (uint32_t)(int)rint_(__builtin_ldexpf(x[c][4 * i + j], up)) + 0x80808080u;
+            w[i] = (__builtin_amdgcn_perm(z[1], z[0], pick) |
+                    __builtin_amdgcn_perm(z[3], z[2], pick) << 16) ^ 0x80808080u;
           }
           q[t][c] = make_uint4(w[0], w[1], w[2], w[3]);
         }
@@ -601,6 +602,16 @@ void paged_attention_kernel(PagedAttentionArgs a) {
           }
       }
       hold();
+      // The block's scales, before the lanes may take those of further ones; not with
+      // its rows' places, which would make the first rows wait for them.
+      float key_scale[2], value_scale[2];
+      if constexpr (S::kI8) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          key_scale[h] = bits_to_float(lane_of(float_to_bits(key_scales), 2 * now.turn + h));
+          value_scale[h] = bits_to_float(lane_of(float_to_bits(value_scales), 2 * now.turn + h));
+        }
+      }
       // After the last block, of no rows: a branch around the loads would make
       // each wait one for all that are under way.
       block += kWaves;
@@ -612,19 +623,23 @@ void paged_attention_kernel(PagedAttentionArgs a) {
       float most = kMinusInf, weight[8];  // scores first
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float back = 0.0f;
-        if constexpr (S::kI8) {
-          // A product past F32 of a query and numbers that are all 0 is 0.
-          back = key_back * now.key_scale[h];
-          back = __builtin_fminf(__builtin_fmaxf(back, -kLargest), kLargest) + (key_back - key_back);
+        float back[S::kScales];
+#pragma unroll
+        for (int i = 0; i < S::kScales; ++i) {
+          back[i] = scale[i];
+          if constexpr (S::kI8) {
+            // A query past F32 by numbers that are all 0 is 0; NaN stays.
+            back[i] *= key_back * key_scale[h];
+            back[i] = __builtin_elementwise_minimum(
+                __builtin_elementwise_maximum(back[i], -kLargest), kLargest);
+          }
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float s = (float)scores[h][0][e] * scale[0];
+          float s = (float)scores[h][0][e] * back[0];
 #pragma unroll
-          for (int i = 1; i < S::kScales; ++i) s = fmaf_((float)scores[h][i][e], scale[i], s);
+          for (int i = 1; i < S::kScales; ++i) s = fmaf_((float)scores[h][i][e], back[i], s);
           s = across_columns<kW>(s);
-          if constexpr (S::kI8) s *= back;
           const bool live = 4 * g + e >= now.lo[h] && 4 * g + e < now.hi[h];
           weight[4 * h + e] = live ? s : kMinusInf;
           most = __builtin_fmaxf(most, weight[4 * h + e]);
@@ -650,8 +665,8 @@ void paged_attention_kernel(PagedAttentionArgs a) {
       }
       if constexpr (S::kI8) {
         // A value's weight has its block's scale in it, over the largest so far.
-        const float here = __builtin_fmaxf(__builtin_fabsf(now.value_scale[0]),
-                                           __builtin_fabsf(now.value_scale[1]));
+        const float here = __builtin_fmaxf(__builtin_fabsf(value_scale[0]),
+                                           __builtin_fabsf(value_scale[1]));
         if (__ballot(here > top_scale)) {
           const float old = top_scale / here;
 #pragma unroll
@@ -662,7 +677,7 @@ void paged_attention_kernel(PagedAttentionArgs a) {
           each_top = 1.0f / here;
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) weight[i] *= now.value_scale[i / 4] * each_top;
+        for (int i = 0; i < 8; ++i) weight[i] *= value_scale[i / 4] * each_top;
       }
       uint4 w[S::kTiles];
 #pragma unroll
@@ -787,52 +802,76 @@ void paged_attention_kernel(PagedAttentionArgs a) {
 // launch, but read all of a row's states, 640 KB for 157 parts of four heads,
 // through one compute unit: 16 us.)
 constexpr uint32_t kJoinWaves = 4, kThreads = 64 * kJoinWaves, kJoinGroups = kThreads / 16;
+// States that a group asks for with the statistics: of up to 64 parts, and of more
+// (few parts take 0.5 us longer where all ask for ten, 157 1.5 where all for four).
+constexpr uint32_t kEarly = 10, kFew = 4;
 template <int kD, bool kI8>
 __global__ __launch_bounds__(kThreads) void paged_attention_join_kernel(PagedAttentionArgs a) {
   __shared__ float wave_top[kJoinWaves], wave_sum[kJoinWaves];
   __shared__ float factors[kMostJoinedParts];
   __shared__ float4 sums[kJoinGroups][16];
+  const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6, group = t / 16;
+  // What is read comes in two steps: the records (any first one, were there none),
+  // then the statistics with the first states.
   const uint32_t count = *a.record_count;
-  const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  uint4 record = a.records[blockIdx.x];
   for (uint32_t i = blockIdx.x; i < count; i += gridDim.x) {
-    const uint4 record = a.records[i];
+    if (i != blockIdx.x) record = a.records[i];
     const uint32_t h = blockIdx.y / (kD / 64), d = blockIdx.y % (kD / 64) * 64 + t % 16 * 4;
     const uint32_t parts = record.z;
     if (h >= record.y >> 16) continue;
     const uint64_t first = (uint64_t)record.w * kHeadBlock + h;
-    float top = kMinusInf;
-    for (uint32_t p = t; p < parts; p += kThreads)
-      top = __builtin_fmaxf(top, a.stats[2 * (first + (uint64_t)p * kHeadBlock)]);
-    for (int o = 32; o > 0; o >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, o));
+    auto stats_of = [&](uint32_t p) {
+      return *reinterpret_cast<const float2*>(a.stats + 2 * (first + (uint64_t)p * kHeadBlock));
+    };
+    auto state_of = [&](uint32_t p) {
+      return *reinterpret_cast<const float4*>(a.states + (first + (uint64_t)p * kHeadBlock) * kD + d);
+    };
+    const float2 mine = stats_of(t < parts ? t : 0);
+    float4 early[kEarly];
+    auto ask = [&](uint32_t k) {
+      const uint32_t p = group + k * kJoinGroups;
+      early[k] = state_of(p < parts ? p : 0);
+    };
+#pragma unroll
+    for (uint32_t k = 0; k < kFew; ++k) ask(k);
+    if (parts > kFew * kJoinGroups) {
+#pragma unroll
+      for (uint32_t k = kFew; k < kEarly; ++k) ask(k);
+    }
+    float top = t < parts ? mine.x : kMinusInf;
+    for (uint32_t p = t + kThreads; p < parts; p += kThreads)
+      top = __builtin_fmaxf(top, stats_of(p).x);
+    top = across_wave(top, [](float p, float r) { return __builtin_fmaxf(p, r); });
     __syncthreads();  // the last record's reads are done
     if (lane == 0) wave_top[wave] = top;
     __syncthreads();
     for (uint32_t w = 0; w < kJoinWaves; ++w) top = __builtin_fmaxf(top, wave_top[w]);
     float weights = 0.0f;
     for (uint32_t p = t; p < parts; p += kThreads) {
-      const float2 s =
-          *reinterpret_cast<const float2*>(a.stats + 2 * (first + (uint64_t)p * kHeadBlock));
+      const float2 s = p == t ? mine : stats_of(p);
       const float f = top == kMinusInf ? 0.0f : __builtin_amdgcn_exp2f(s.x - top);
       factors[p] = kI8 ? f * s.y : f;  // of 8 bits a part's outputs are over its weights
       weights = fmaf_(s.y, f, weights);
     }
-    for (int o = 32; o > 0; o >>= 1) weights += __shfl_xor(weights, o);
+    weights = across_wave(weights, [](float p, float r) { return p + r; });
     if (lane == 0) wave_sum[wave] = weights;
     __syncthreads();
-    const uint32_t group = t / 16;
     const float l = wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3];
     const float each = kI8 && l != 0.0f ? 1.0f / l : 1.0f;  // so that no sum is past the outputs
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-    for (uint32_t p = group; p < parts; p += kJoinGroups) {
-      const float f = factors[p] * each;
-      const float4 o = *reinterpret_cast<const float4*>(
-          a.states + (first + (uint64_t)p * kHeadBlock) * kD + d);
+    auto add = [&](uint32_t p, const float4& o) {
+      const float f = kI8 ? factors[p] * each : factors[p];
       sum.x = fmaf_(o.x, f, sum.x);
       sum.y = fmaf_(o.y, f, sum.y);
       sum.z = fmaf_(o.z, f, sum.z);
       sum.w = fmaf_(o.w, f, sum.w);
-    }
+    };
+#pragma unroll
+    for (uint32_t k = 0; k < kEarly; ++k)
+      if (group + k * kJoinGroups < parts) add(group + k * kJoinGroups, early[k]);
+#pragma unroll 8
+    for (uint32_t p = group + kEarly * kJoinGroups; p < parts; p += kJoinGroups) add(p, state_of(p));
     sums[group][t % 16] = sum;
     __syncthreads();
     if (t < 64) {
