@@ -24,7 +24,8 @@ namespace {
 
 using namespace rules;
 
-constexpr uint32_t kThreads = 256;
+constexpr uint32_t kRopeThreads = 512, kRopeAtOnce = 1024;
+static_assert(kRopeThreads >= kMostRows, "a thread looks at a row");
 
 // A number of the block's scale, rounded to nearest even; NaN is 0.
 __device__ __forceinline__ int code_of(float x) {
@@ -32,8 +33,14 @@ __device__ __forceinline__ int code_of(float x) {
   return x == x ? (int)rint_(__builtin_fminf(__builtin_fmaxf(x, -top), top)) : 0;
 }
 __device__ __forceinline__ uint32_t codes_of(float4 v, float scale) {
-  return (uint32_t)(code_of(v.x / scale) & 0xFF) | (uint32_t)(code_of(v.y / scale) & 0xFF) << 8 |
-         (uint32_t)(code_of(v.z / scale) & 0xFF) << 16 | (uint32_t)code_of(v.w / scale) << 24;
+  if ((float_to_bits(scale) & 0x7FFFFFu) == 0) {  // a power of two, mostly: its product is the quotient
+    const float each = 1.0f / scale;
+    v = make_float4(v.x * each, v.y * each, v.z * each, v.w * each);
+  } else {
+    v = make_float4(v.x / scale, v.y / scale, v.z / scale, v.w / scale);
+  }
+  return (uint32_t)(code_of(v.x) & 0xFF) | (uint32_t)(code_of(v.y) & 0xFF) << 8 |
+         (uint32_t)(code_of(v.z) & 0xFF) << 16 | (uint32_t)code_of(v.w) << 24;
 }
 // Four numbers by a scale `ratio` times as large (at most 1).
 __device__ __forceinline__ uint32_t rescaled(uint32_t codes, float ratio) {
@@ -71,22 +78,25 @@ __device__ __forceinline__ void norm_and_turn(float4& va, float4& vb, const floa
   rope_rotate(va, vb, 0, cosine, sine);
 }
 
-// blockIdx.y: the groups of query heads, then each head's keys, then its values.
-template <int kD>
-__global__ __launch_bounds__(kThreads) void paged_rope_i8_kernel(PagedRopeArgs a,
-                                                                 uint32_t query_groups) {
+// The last workgroups turn queries. The others take a tile of rows and one
+// key-value head, whose keys are half of a workgroup's threads and whose values the
+// other half, and of those rows the blocks that they are the first in the step to be
+// in, one after another: mostly one or none of a prompt's.
+template <int kD, uint32_t kTileRows>
+__global__ __launch_bounds__(kRopeThreads) void paged_rope_i8_kernel(PagedRopeArgs a,
+                                                                     uint32_t query_groups,
+                                                                     uint32_t tiles) {
   constexpr uint32_t kLanes = kD / 8, kHalf = kD / 2;
-  constexpr uint32_t kGroups = kThreads / kLanes;  // heads, or rows of a block, at once
+  constexpr uint32_t kHeads = kRopeThreads / kLanes;  // of queries, at once
+  constexpr uint32_t kGroups = kHeads / 2;            // rows of a block, at once
   constexpr uint32_t kTurns = kGroups < kScaleSlots ? kScaleSlots / kGroups : 1;
-  __shared__ uint32_t member[kScaleSlots];  // the row that writes a slot, and 1
-  __shared__ float wave_most[kThreads / 64];
-  const uint32_t row = blockIdx.x, t = threadIdx.x;
-  const uint32_t group = t / kLanes, l = t % kLanes;
-  const uint32_t p = a.positions[row];
-  if (p == kNone) return;
-
-  if (blockIdx.y < query_groups) {
-    const uint32_t h = blockIdx.y * kGroups + group;
+  const uint32_t t = threadIdx.x, l = t % kLanes;
+  const uint32_t appends = tiles * a.cache.kv_heads;
+  if (blockIdx.x >= appends) {
+    const uint32_t row = (blockIdx.x - appends) / query_groups;
+    const uint32_t h = (blockIdx.x - appends) % query_groups * kHeads + t / kLanes;
+    const uint32_t p = a.positions[row];
+    if (p == kNone) return;
     const bool active = h < a.query_heads;
     float4 va = make_float4(0.f, 0.f, 0.f, 0.f), vb = va;
     if (active) {
@@ -101,111 +111,145 @@ __global__ __launch_bounds__(kThreads) void paged_rope_i8_kernel(PagedRopeArgs a
     *reinterpret_cast<float4*>(dst + kHalf + 4 * l) = vb;
     return;
   }
-  const uint32_t part = blockIdx.y - query_groups;
-  const bool is_value = part >= a.cache.kv_heads;
-  const uint32_t kv = is_value ? part - a.cache.kv_heads : part;
-
-  // The step's rows of the block: the workgroup is that of the first of them. The
-  // row before, mostly of the same block in a prompt, spares the others the rest.
-  const uint32_t sequence = a.sequences ? a.sequences[row] : row;
-  const uint32_t block = p / kScaleSlots;
-  if (a.sequences && row > 0 && a.sequences[row - 1] == sequence) {
-    const uint32_t before = a.positions[row - 1];
-    if (before != kNone && before / kScaleSlots == block) return;
+  __shared__ uint32_t members[kTileRows][kScaleSlots];  // the row that writes a slot, and 1
+  __shared__ uint32_t taken;  // rows of the tile that are not the first of their block
+  __shared__ float wave_most[kRopeThreads / 64];
+  const uint32_t kv = blockIdx.x % a.cache.kv_heads;
+  const uint32_t tile = blockIdx.x / a.cache.kv_heads;
+  const uint32_t rows = (a.rows - tile + tiles - 1) / tiles;
+  // Each thread holds its row of the step against the tile's.
+  auto sequence_of = [&](uint32_t r) { return a.sequences ? a.sequences[r] : r; };
+  const uint32_t mine = min(t, a.rows - 1);
+  const uint32_t p_mine = t < a.rows ? a.positions[mine] : kNone;
+  const uint32_t sequence_mine = sequence_of(mine);
+  uint32_t p_tile[kTileRows], sequence_tile[kTileRows];
+#pragma unroll
+  for (uint32_t k = 0; k < kTileRows; ++k) {
+    const uint32_t r = tile + min(k, rows - 1) * tiles;
+    p_tile[k] = a.positions[r];
+    sequence_tile[k] = sequence_of(r);
   }
-  const uint32_t index = p / a.cache.page_slots;
-  const uint32_t page = page_at(a.cache.table, a.cache.sequences, a.cache.width, a.cache.pages,
-                                sequence, index);
-  if (page == kNone) return;
-  if (t < kScaleSlots) member[t] = 0;
+  if (t < kTileRows * kScaleSlots) members[t / kScaleSlots][t % kScaleSlots] = 0;
+  if (t == 0) taken = 0;
   __syncthreads();
-  bool later = false;
-  if (a.sequences) {
-    for (uint32_t r = t; r < a.rows; r += kThreads) {
-      const uint32_t at = a.positions[r];
-      if (at != kNone && at / kScaleSlots == block && a.sequences[r] == sequence) {
-        // Of rows at one position the last.
-        atomicMax(&member[at % kScaleSlots], r + 1);
-        later = later || r < row;
+#pragma unroll
+  for (uint32_t k = 0; k < kTileRows; ++k) {
+    if ((k == 0 || k < rows) && p_mine != kNone && p_tile[k] != kNone && sequence_mine == sequence_tile[k] &&
+        p_mine / kScaleSlots == p_tile[k] / kScaleSlots) {
+      atomicMax(&members[k][p_mine % kScaleSlots], t + 1);  // of rows at one position the last
+      if (t < tile + k * tiles) atomicOr(&taken, 1u << k);
+    }
+  }
+  __syncthreads();
+  const uint32_t others = taken;
+#pragma unroll 1
+  for (uint32_t k = 0; k < rows; ++k) {
+    if (others >> k & 1) continue;
+    uint32_t p = kNone, sequence = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kTileRows; ++i) {
+      p = i == k ? p_tile[i] : p;
+      sequence = i == k ? sequence_tile[i] : sequence;
+    }
+    if (p == kNone) continue;
+    const uint32_t block = p / kScaleSlots;
+    const uint32_t index = p / a.cache.page_slots;
+    const uint32_t page = page_at(a.cache.table, a.cache.sequences, a.cache.width, a.cache.pages,
+                                  sequence, index);
+    if (page == kNone) continue;
+    const uint32_t* member = members[k];
+
+    const bool is_value = t >= kRopeThreads / 2;
+    const uint32_t group = t % (kRopeThreads / 2) / kLanes;
+    const uint32_t first_slot = block * kScaleSlots - index * a.cache.page_slots;
+    uint8_t* codes = static_cast<uint8_t*>(is_value ? a.cache.values : a.cache.keys) +
+                     page * a.cache.page_stride +
+                     ((uint64_t)first_slot * a.cache.kv_heads + kv) * kD;
+    float* scale_at = (is_value ? a.cache.value_scales : a.cache.key_scales) +
+                      page * a.cache.scale_stride +
+                      (uint64_t)(first_slot / kScaleSlots) * a.cache.kv_heads + kv;
+    float scale = *scale_at;
+    if (member[0] || !(scale > 0.0f) || scale == __builtin_inff()) scale = 0.0f;
+
+    uint32_t from[kTurns];
+    float4 va[kTurns], vb[kTurns];
+    uint32_t ca[kTurns], cb[kTurns];  // what the block holds
+#pragma unroll
+    for (uint32_t i = 0; i < kTurns; ++i) {
+      const uint32_t slot = i * kGroups + group;
+      from[i] = slot < kScaleSlots ? member[slot] : 0;
+      va[i] = vb[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      ca[i] = cb[i] = 0;
+      if (from[i]) {
+        const float* src = (is_value ? a.value : a.key) + (uint64_t)(from[i] - 1) * a.kv_stride +
+                           (uint64_t)kv * kD;
+        va[i] = ld4f(src + 4 * l);
+        vb[i] = ld4f(src + kHalf + 4 * l);
+      } else if (slot < kScaleSlots) {
+        const uint8_t* src = codes + (uint64_t)slot * a.cache.kv_heads * kD;
+        ca[i] = *reinterpret_cast<const uint32_t*>(src + 4 * l);
+        cb[i] = *reinterpret_cast<const uint32_t*>(src + kHalf + 4 * l);
       }
     }
-  } else if (t == 0) {  // each row is its own request
-    member[p % kScaleSlots] = row + 1;
-  }
-  if (__syncthreads_or(later)) return;
-
-  const uint32_t first_slot = block * kScaleSlots - index * a.cache.page_slots;
-  uint8_t* codes = static_cast<uint8_t*>(is_value ? a.cache.values : a.cache.keys) +
-                   page * a.cache.page_stride +
-                   ((uint64_t)first_slot * a.cache.kv_heads + kv) * kD;
-  float* scale_at = (is_value ? a.cache.value_scales : a.cache.key_scales) +
-                    page * a.cache.scale_stride +
-                    (uint64_t)(first_slot / kScaleSlots) * a.cache.kv_heads + kv;
-  float scale = *scale_at;
-  if (member[0] || !(scale > 0.0f) || scale == __builtin_inff()) scale = 0.0f;
-
-  uint32_t from[kTurns];
-  float4 va[kTurns], vb[kTurns];
-  uint32_t ca[kTurns], cb[kTurns];  // what the block holds
+    float most = 0.0f;
 #pragma unroll
-  for (uint32_t i = 0; i < kTurns; ++i) {
-    const uint32_t slot = i * kGroups + group;
-    from[i] = slot < kScaleSlots ? member[slot] : 0;
-    va[i] = vb[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    ca[i] = cb[i] = 0;
-    if (from[i]) {
-      const float* src = (is_value ? a.value : a.key) + (uint64_t)(from[i] - 1) * a.kv_stride +
-                         (uint64_t)kv * kD;
-      va[i] = ld4f(src + 4 * l);
-      vb[i] = ld4f(src + kHalf + 4 * l);
-    } else if (slot < kScaleSlots) {
-      const uint8_t* src = codes + (uint64_t)slot * a.cache.kv_heads * kD;
-      ca[i] = *reinterpret_cast<const uint32_t*>(src + 4 * l);
-      cb[i] = *reinterpret_cast<const uint32_t*>(src + kHalf + 4 * l);
+    for (uint32_t i = 0; i < kTurns; ++i) {
+      const uint32_t slot = i * kGroups + group;
+      if (!is_value && __ballot(from[i] != 0))
+        norm_and_turn<kD>(va[i], vb[i], a.key_gain, a.turns, l, block * kScaleSlots + slot,
+                          a.epsilon);
+      if (from[i]) most = __builtin_fmaxf(most, __builtin_fmaxf(most_of(va[i]), most_of(vb[i])));
     }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) most = __builtin_fmaxf(most, __shfl_xor(most, o));
+    if (t % 64 == 0) wave_most[t / 64] = most;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t w = 0; w < kRopeThreads / 128; ++w)
+      most = __builtin_fmaxf(most, wave_most[is_value * (kRopeThreads / 128) + w]);
+    const float need = bits_to_float(block_scale_bits(float_to_bits(most)));
+    const float after = __builtin_fmaxf(scale, need);
+    const float ratio = after > 0.0f ? scale / after : 0.0f;
+    const float by = after > 0.0f ? after : 1.0f;  // all zeros: any
+#pragma unroll
+    for (uint32_t i = 0; i < kTurns; ++i) {
+      const uint32_t slot = i * kGroups + group;
+      if (slot >= kScaleSlots || (!from[i] && ratio == 1.0f)) continue;
+      uint8_t* dst = codes + (uint64_t)slot * a.cache.kv_heads * kD;
+      *reinterpret_cast<uint32_t*>(dst + 4 * l) =
+          from[i] ? codes_of(va[i], by) : rescaled(ca[i], ratio);
+      *reinterpret_cast<uint32_t*>(dst + kHalf + 4 * l) =
+          from[i] ? codes_of(vb[i], by) : rescaled(cb[i], ratio);
+    }
+    if (t % (kRopeThreads / 2) == 0) *scale_at = after;
+    __syncthreads();  // what is shared is read
   }
-  float most = 0.0f;
-#pragma unroll
-  for (uint32_t i = 0; i < kTurns; ++i) {
-    const uint32_t slot = i * kGroups + group;
-    if (!is_value)
-      norm_and_turn<kD>(va[i], vb[i], a.key_gain, a.turns, l, block * kScaleSlots + slot,
-                        a.epsilon);
-    if (from[i]) most = __builtin_fmaxf(most, __builtin_fmaxf(most_of(va[i]), most_of(vb[i])));
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) most = __builtin_fmaxf(most, __shfl_xor(most, o));
-  if (t % 64 == 0) wave_most[t / 64] = most;
-  __syncthreads();
-#pragma unroll
-  for (uint32_t w = 0; w < kThreads / 64; ++w) most = __builtin_fmaxf(most, wave_most[w]);
-  const float need = bits_to_float(block_scale_bits(float_to_bits(most)));
-  const float after = __builtin_fmaxf(scale, need);
-  const float ratio = after > 0.0f ? scale / after : 0.0f;
-  const float by = after > 0.0f ? after : 1.0f;  // all zeros: any
-#pragma unroll
-  for (uint32_t i = 0; i < kTurns; ++i) {
-    const uint32_t slot = i * kGroups + group;
-    if (slot >= kScaleSlots || (!from[i] && ratio == 1.0f)) continue;
-    uint8_t* dst = codes + (uint64_t)slot * a.cache.kv_heads * kD;
-    *reinterpret_cast<uint32_t*>(dst + 4 * l) =
-        from[i] ? codes_of(va[i], by) : rescaled(ca[i], ratio);
-    *reinterpret_cast<uint32_t*>(dst + kHalf + 4 * l) =
-        from[i] ? codes_of(vb[i], by) : rescaled(cb[i], ratio);
-  }
-  if (t == 0) *scale_at = after;
 }
 
 template <int kD>
 void launch_rope(hipStream_t s, const PagedRopeArgs& a) {
-  constexpr uint32_t kGroups = kThreads / (kD / 8);
-  const uint32_t groups = (a.query_heads + kGroups - 1) / kGroups;
-  hipLaunchKernelGGL(paged_rope_i8_kernel<kD>, dim3(a.rows, groups + 2 * a.cache.kv_heads),
-                     dim3(kThreads), 0, s, a, groups);
+  constexpr uint32_t kHeads = kRopeThreads / (kD / 8);
+  const uint32_t groups = (a.query_heads + kHeads - 1) / kHeads;
+  // A tile of one row, or of up to four where workgroups of one would be more than run
+  // at once, four a compute unit. A tile's rows are an odd number apart, so that neither
+  // the first rows of a step nor every sixteenth, which are the first of their blocks
+  // where rows lie in any order and in theirs, fall into few tiles. (507 rows in any
+  // order, 8 key-value heads: tiles of rows side by side 17 us, these 11.6, of eight
+  // such rows 12.5, of one 16.5.)
+  const uint32_t even = (a.rows * a.cache.kv_heads + kRopeAtOnce - 1) / kRopeAtOnce;
+  const uint32_t tile = even < 4 ? even : 4;
+  uint32_t tiles = (a.rows + tile - 1) / tile;
+  if (tile > 1 && tiles % 2 == 0) ++tiles;
+  const dim3 grid(tiles * a.cache.kv_heads + a.rows * groups), threads(kRopeThreads);
+  if (tile == 1)
+    hipLaunchKernelGGL((paged_rope_i8_kernel<kD, 1>), grid, threads, 0, s, a, groups, tiles);
+  else
+    hipLaunchKernelGGL((paged_rope_i8_kernel<kD, 4>), grid, threads, 0, s, a, groups, tiles);
 }
 
 // ---- reading back --------------------------------------------------------------
 
+constexpr uint32_t kThreads = 256;
 constexpr int kPiece = 16;  // values that a thread takes
 
 // A piece of a cache row in F32.
