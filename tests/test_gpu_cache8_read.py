@@ -82,6 +82,28 @@ def test_many_rows(device, rows, kv, dim):
         assert np.array_equal(g, w[positions])
 
 
+@pytest.mark.parametrize("cache,fmt,kv,dim,rows", [
+    (I8, BF16, 2, 128, 40001), (I8, F32, 1, 256, 20003), (F16, F16, 3, 64, 50001),
+    (I8, F16, 1024, 64, 150)])
+def test_more_than_the_caches_hold(device, cache, fmt, kv, dim, rows):
+    # Over 32 MB of outputs, rows of no position and keys of no page among them.
+    rng = np.random.default_rng(rows)
+    paged = any_pool(device, rng, [90, 300], kv, dim, 16, cache)
+    paged.table[1, 2] = NONE
+    paged.upload()
+    requests = rng.integers(0, 2, rows)
+    positions = np.where(requests == 0, rng.integers(0, 90, rows), rng.integers(0, 300, rows))
+    positions[rng.random(rows) < 0.1] = NONE
+    got = read(device, paged, requests, positions, fmt, stride=kv * dim + 8)
+    every = [expected(paged, np.full(n, r), np.arange(n), fmt, kv * dim + 8)
+             for r, n in enumerate((90, 300))]
+    for which, g in enumerate(got):
+        w = np.concatenate([every[0][which], every[1][which], to_format(np.full(
+            (1, kv * dim + 8), 7.0), fmt)])
+        w = w[np.where(positions == NONE, 390, positions + 90 * requests)]
+        assert np.array_equal(g, w, equal_nan=g.dtype == np.float32)
+
+
 def test_the_ends_of_the_range(device):
     rng = np.random.default_rng(4)
     paged = Paged8(device, rng, [48], 1, 64, 16)
