@@ -502,7 +502,7 @@ struct PagedAttentionArgs {
   float* stats;
   uint4* records;
   uint32_t* record_count;
-  uint32_t units = 0, at_once = 0;  // set by the launcher
+  uint32_t units = 0, at_once = 0, shared_units = 1;  // set by the launcher
 };
 constexpr int kMostComputeUnits = 256;  // gfx950's
 constexpr int kAttentionWorkgroups = 4;  // a compute unit's at once, at most

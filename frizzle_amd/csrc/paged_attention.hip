@@ -70,6 +70,7 @@ constexpr float kLargest = 0x1.fffffep127f;
 // launch_shape.
 constexpr uint64_t kWaveBlocks = 32, kFewValues = 2048, kManyValues = 8192;
 constexpr int kBufferWord3 = 0x00020000;  // raw 32-bit data
+constexpr uint32_t kDies = 8;  // workgroups go to them in turn
 constexpr float kLeastTop = 0x1p-126f;
 constexpr float kCodeUnit = 1024.0f;  // what a value's number of 8 bits is the 2^-10 of
 
@@ -291,13 +292,14 @@ __device__ __forceinline__ bool find_part(const PagedAttentionArgs& a, uint32_t 
   if (owners == 0) return false;
   const int leader = __builtin_ctzll(owners);  // the first lane whose parts reach past `want`
   uint32_t rest = want - (to - total) * a.units, joined_before = joined_to - joined;
-  uint32_t row = 0, position_ = 0, sequence_ = 0, parts_ = 0;
+  uint32_t row = 0, position_ = 0, sequence_ = 0, blocks_ = 0, parts_ = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const bool here = parts_ == 0 && rest < parts[i] * a.units;
     row = here ? lane * kPer + i : row;
     position_ = here ? position[i] : position_;
     sequence_ = here ? sequence[i] : sequence_;
+    blocks_ = here ? blocks[i] : blocks_;
     parts_ = here ? parts[i] : parts_;
     const bool past = parts_ == 0;
     rest -= past ? parts[i] * a.units : 0;
@@ -309,7 +311,7 @@ __device__ __forceinline__ bool find_part(const PagedAttentionArgs& a, uint32_t 
   out->parts = lane_of(parts_, leader);
   rest = lane_of(rest, leader);
   joined_before = lane_of(joined_before, leader);
-  out->chunk = chunk;
+  out->chunk = row_chunk(lane_of(blocks_, leader), out->parts, chunk);
   // Neighbouring workgroups take the head blocks of the same keys, whose
   // rows lie side by side.
   out->unit = rest % a.units;
@@ -332,10 +334,18 @@ void paged_attention_kernel(PagedAttentionArgs a) {
   const uint32_t wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int n = lane & 15, g = lane >> 4;
 
+  // Head blocks that read the same lines go to one die, whose cache then has each once.
+  uint32_t want = blockIdx.x;
+  if (a.shared_units > 1) {
+    const uint32_t in_die = blockIdx.x / kDies;
+    want = (in_die / a.shared_units * kDies + blockIdx.x % kDies) * a.shared_units +
+           in_die % a.shared_units;
+  }
   Part part;
   if constexpr (kWhole) {
-    part.row = blockIdx.x / a.units;
-    part.unit = blockIdx.x % a.units;
+    if (want >= a.rows * a.units) return;
+    part.row = want / a.units;
+    part.unit = want % a.units;
     part.position = a.positions[part.row];
     if (part.position == kNone) return;
     part.sequence = a.sequences ? a.sequences[part.row] : part.row;
@@ -343,8 +353,8 @@ void paged_attention_kernel(PagedAttentionArgs a) {
     part.parts = 1;
     part.chunk = kMostKeys / kBlockKeys;
   } else {
-    const bool found = a.rows <= 64 ? find_part<1>(a, blockIdx.x, lane, &part)
-                                    : find_part<kMostRows / 64>(a, blockIdx.x, lane, &part);
+    const bool found = a.rows <= 64 ? find_part<1>(a, want, lane, &part)
+                                    : find_part<kMostRows / 64>(a, want, lane, &part);
     if (blockIdx.x == 0 && threadIdx.x == 0) *a.record_count = part.records;
     if (!found) return;
   }
@@ -887,9 +897,21 @@ __global__ __launch_bounds__(kThreads) void paged_attention_join_kernel(PagedAtt
 
 template <int kD, CacheFormat kF, int kW>
 hipError_t launch_shape(hipStream_t s, PagedAttentionArgs a, uint32_t heads, int compute_units) {
+  typedef Shape<kD, kF, kW> S;
   static_assert(kFits<kD, kF, kW>, "the workspace holds their parts");
   const uint32_t units = a.rows * a.units;
   a.at_once = kWorkgroups<kD, kF, kW> * (uint32_t)compute_units;
+  // Units side by side that read the same lines: a key-value head's head blocks, and two
+  // heads of 64 bytes (four rows of 100,000 keys, 16 heads of 64 in 8 bits, 270 -> 215
+  // us). Not all of a row's heads, which cost 256-wide ones 4%, and not where a die's
+  // compute units do not take them whole, as one would have a workgroup more to do.
+  a.shared_units = a.units / a.cache.kv_heads;
+  if (kD * S::kBytes < 128 && a.cache.kv_heads % 2 == 0) a.shared_units *= 2;
+  if (a.at_once % (kDies * a.shared_units) != 0) a.shared_units = 1;
+  auto grid = [&](uint64_t n) {
+    const uint32_t even = a.shared_units > 1 ? kDies * a.shared_units : 1;
+    return dim3((uint32_t)((n + even - 1) / even * even));
+  };
   // The most blocks that a row can have. Where they are few, each unit is one
   // workgroup's (kWhole), which then need not find its part, nor leave a state
   // to a second launch: always to kFewValues (64 requests of up to 250 keys, 256
@@ -905,13 +927,13 @@ hipError_t launch_shape(hipStream_t s, PagedAttentionArgs a, uint32_t heads, int
   const uint64_t blocks =
       most_row_blocks((uint64_t)a.cache.width * a.cache.page_slots, a.window, a.sinks);
   if (units >= a.at_once && blocks <= kWaveBlocks) {
-    hipLaunchKernelGGL((paged_attention_kernel<kD, kF, kW, 1, true>), dim3(units), dim3(64), 0,
+    hipLaunchKernelGGL((paged_attention_kernel<kD, kF, kW, 1, true>), grid(units), dim3(64), 0,
                        s, a);
     return hipGetLastError();
   }
   const bool few = 8 * units < 3 * (uint32_t)compute_units;
   if (blocks * kD <= (few ? kFewValues : kManyValues)) {
-    hipLaunchKernelGGL((paged_attention_kernel<kD, kF, kW, kPartWaves, true>), dim3(units),
+    hipLaunchKernelGGL((paged_attention_kernel<kD, kF, kW, kPartWaves, true>), grid(units),
                        dim3(64 * kPartWaves), 0, s, a);
     return hipGetLastError();
   }
@@ -919,7 +941,7 @@ hipError_t launch_shape(hipStream_t s, PagedAttentionArgs a, uint32_t heads, int
   const uint64_t fill = units * blocks;
   const uint64_t bound = most_parts(units, a.at_once);
   hipLaunchKernelGGL((paged_attention_kernel<kD, kF, kW, kPartWaves, false>),
-                     dim3((uint32_t)(fill < bound ? fill : bound)), dim3(64 * kPartWaves), 0, s, a);
+                     grid(fill < bound ? fill : bound), dim3(64 * kPartWaves), 0, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const uint32_t joins = most_joined_parts(units, a.at_once) / 2;

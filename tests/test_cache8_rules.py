@@ -44,7 +44,22 @@ static int wrong(uint32_t window, uint32_t sinks, uint32_t capacity, uint32_t to
   return off;
 }
 
+// Rows whose parts, cut as evenly as fours leave them, are not as many as the chunk's,
+// none empty and none longer.
+static int uneven(uint32_t chunk, uint32_t to) {
+  int off = 0;
+  for (uint32_t n = 1; n < to; ++n) {
+    const uint32_t parts = row_parts(n, chunk, 1.0f / chunk), each = row_chunk(n, parts, chunk);
+    off += each > chunk || parts * each < n || (parts - 1) * each >= n;
+  }
+  return off;
+}
+
 int main(int argc, char** argv) {
+  if (argc == 3) {
+    std::printf("%d\n", uneven(strtoul(argv[1], 0, 10), strtoul(argv[2], 0, 10)));
+    return 0;
+  }
   if (argc == 5)
     std::printf("%d\n", wrong(strtoul(argv[1], 0, 10), strtoul(argv[2], 0, 10),
                               strtoul(argv[3], 0, 10), strtoul(argv[4], 0, 10)));
@@ -74,6 +89,11 @@ def test_every_key_in_one_block(rules, sinks, window, capacity):
     assert rules(window, sinks, capacity, 450) == [0]
 
 
+@pytest.mark.parametrize("chunk", [1, 2, 4, 8, 12, 16, 44, 84, 132, 1000, 4096])
+def test_parts_of_a_row_are_even(rules, chunk):
+    assert rules(chunk, 20000) == [0]
+
+
 def bits(x):
     return struct.unpack("<I", struct.pack("<f", x))[0]
 
@@ -97,4 +117,5 @@ def test_scales_are_the_least_powers_of_two(rules):
 
 
 def test_scales_past_the_range_are_the_last(rules):
-    assert [number(b) for b in rules(bits(math.inf), bits(3.4e38))] == [2.0 ** 121] * 2
+    assert [number(b) for b in rules(bits(math.inf), bits(3.4e38), bits(math.inf))] == [
+        2.0 ** 121] * 3
