@@ -23,7 +23,7 @@ constexpr size_t kAdapterBytes =
 constexpr size_t kScratchBytes = kAttentionBytes > kAdapterBytes ? kAttentionBytes : kAdapterBytes;
 
 constexpr int kMostHeads = 1024;
-constexpr uint32_t kMostReadRows = 1u << 24;
+constexpr uint32_t kMostReadRows = 1u << 23;  // a launch counts 2^32 threads at most
 constexpr float kMostScale = 4096.0f;  // 2^13 in log2 units, as the kernel takes
 
 bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -75,7 +75,7 @@ const char* refuse_pages(const frz_pages* c, int query_heads, uint32_t rows, uin
       return "scale_stride (at least a page's scales, a pool of at most 2^48)";
   }
   if (rows < 1 || rows > most_rows)
-    return most_rows == rules::kMostRows ? "rows (1 to 512)" : "rows (1 to 2^24)";
+    return most_rows == rules::kMostRows ? "rows (1 to 512)" : "rows (1 to 2^23)";
   return nullptr;
 }
 

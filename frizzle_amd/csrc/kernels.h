@@ -509,7 +509,7 @@ constexpr int kAttentionWorkgroups = 4;  // a compute unit's at once, at most
 constexpr int kMostJoinedParts = 3 * kAttentionWorkgroups * kMostComputeUnits;
 // Values of one head in all of their states: workgroups of a compute unit take
 // kAttentionWidth of them together, at most.
-constexpr int kAttentionWidth = 512;
+constexpr int kAttentionWidth = 384;
 constexpr int kMostStateValues = 3 * kAttentionWidth * kMostComputeUnits;
 hipError_t launch_paged_attention(hipStream_t s, const PagedAttentionArgs& a, int compute_units);
 

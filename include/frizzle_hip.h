@@ -325,7 +325,7 @@ int frz_op_attention_paged_sinks(frz_device* dev, const frz_pages* cache,
                                  uint32_t rows);
 /* Reads a cache back: row r's key and value, at positions[r] of the request
  * sequences[r] (null: request r), all heads, as kv_heads * head_dim values of
- * `format` (F32, F16 or BF16) at keys and values + r * stride, for up to 2^24
+ * `format` (F32, F16 or BF16) at keys and values + r * stride, for up to 2^23
  * rows. Numbers of 8 bits are multiplied by their scales, in F32; all round to
  * the format to nearest even (F16 saturates at 65,504). A key that is not there
  * is zeros, a row at FRZ_NO_POSITION is left as it is. stride is a multiple of 8;

@@ -84,7 +84,7 @@ def test_sinks_refused(more, text):
     (dict(positions=P + 2), "16 bytes"), (dict(sequences=P + 1), "16 bytes"),
     (dict(stride=504), "stride"), (dict(stride=516), "stride"), (dict(stride=0), "stride"),
     (dict(stride=1 << 62), "stride"), (dict(stride=1 << 47), "stride"), (dict(rows=0), "rows"),
-    (dict(rows=(1 << 24) + 1), "rows"), (dict(rows=NONE), "rows"), (dict(values=2 * P), "each other"),
+    (dict(rows=(1 << 23) + 1), "rows"), (dict(rows=NONE), "rows"), (dict(values=2 * P), "each other"),
     (dict(keys=P), "cache"), (dict(values=P), "cache"),
 ])
 def test_reads_refused(more, text):
