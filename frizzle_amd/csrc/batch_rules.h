@@ -166,7 +166,7 @@ FRZ_RULE uint32_t row_parts(uint32_t blocks, uint32_t chunk, float each) {
 
 // Blocks of each part of a row cut into several, the last perhaps fewer: as even as
 // fours leave them, not the chunk's and a rest (64 rows of 6,250 keys, 4 key-value
-// heads, 256 wide, of 8 bits, one workgroup's each or two's: 186 us by rests, 170 so).
+// heads, 256 wide, of 8 bits, a part or two each: 187 us by rests, 155 so).
 FRZ_RULE uint32_t row_chunk(uint32_t blocks, uint32_t parts, uint32_t chunk) {
   if (parts < 2 || chunk < kPartWaves) return chunk;
   const uint32_t each = (blocks + parts - 1) / parts;

@@ -19,6 +19,8 @@
 //                 no move; A = V: the lane's 8 keys' rows at dimensions 8n ..,
 //                 paired up two keys a register by v_perm. O^T leaves each
 //                 lane one head, so m and l stay a lane's own.
+// A row's first keys, where it has them apart from its window's, are blocks of
+// their own before the window's, each looked at for its own keys alone.
 //
 // The matrix cores take 16-bit operands, the cache's type; the query and the
 // weights are F32. Each is split into parts that add up to it, hi + lo of F16
@@ -38,14 +40,30 @@
 // on F32 does not hold the maximum 24 above). All scales are exact, products are
 // exact in F32, sums F32.
 //
+// A cache of 8 bits is whole numbers c, -127 to 127, and a scale s of each 16 slots
+// of a head, which is half a block, so that both scales are the wave's own numbers:
+//   S = (q . c) s_k     on the matrix cores' whole numbers, 64 a turn: keys go in as
+//                       they lie in memory, the query as four digits of 8 bits,
+//                       columns n, n + W, n + 2W .. of a head, or further tiles. It
+//                       is held to 2^-30 of its head's largest; sums are exact.
+//   O = (p s_v / t) . c t  on those of F16: a byte and a constant make each c exact,
+//                       p s_v / t is split as above. t is the largest s_v so far, the
+//                       outputs' unit, kept as m is: weights stay below 2^14, and a
+//                       part leaves its outputs over its weights, so that no sum is
+//                       past F32 where no value is.
+// Values' bytes as F16 are half of a block's 330 vector instructions (256 wide); the
+// query's digits spare the keys' as many.
+//
 // Keys outside the row's range or in no page are never read: their rows are
 // zeros, and their scores -inf.
 //
 // Whole calls, 256 wide, F16 but where said: three requests of 98,001 to
 // 131,072 keys over 4 key-value heads (1.4 GB) 235 us, 6.0 TB/s; 61 of 40 to
-// 8,192 keys (99 MB) 24.8 us, 4.0 TB/s; 32 of 1 to 4,001 keys, 8 BF16 key-value
-// heads of 128 (70 MB), 20.6 us, 3.4 TB/s; one of 5,004 keys (5 MB) 11.0 us,
-// two launches of dependent loads.
+// 8,192 keys (99 MB) 24.5 us, 4.0 TB/s; 32 of 1 to 4,001 keys, 8 BF16 key-value
+// heads of 128 (70 MB), 20.0 us, 3.5 TB/s; one of 5,004 keys (5 MB) 10.1 us,
+// two launches of dependent loads. The same of 8 bits: 130 us (702 MB, 5.4 TB/s),
+// 17.9, 16.1 and 11.0. 29 requests' first 130 and last 4,000 keys, 8 BF16 heads of
+// 128 (491 MB), 99 us, 5.0 TB/s.
 
 #include <type_traits>
 
@@ -135,7 +153,9 @@ struct Shape {
   static constexpr int kWords = (kVec * kBytes + 3) / 4;
 };
 
-// Workgroups a compute unit runs at once, by the registers that a shape takes.
+// Workgroups a compute unit runs at once, by the registers that a shape takes; 256 wide
+// of 8 bits one, though two would fit (61 requests 17.9 us, 20.6 by two; long ones 130
+// and 136).
 template <int kD, CacheFormat kF, int kW>
 constexpr int kWorkgroups = kD == 256   ? (1)
                             : kD == 128 ? (Shape<kD, kF, kW>::kTiles == 1 ? 3 : 2)
@@ -807,7 +827,7 @@ void paged_attention_kernel(PagedAttentionArgs a) {
 
 // The parts of the rows that have several, joined in order: a workgroup a
 // (record, head, 64 dimensions), 16 lanes of it the dimensions, four each,
-// and its 16 groups every sixteenth part. Some 2 us, a launch and five loads one
+// and its 16 groups every sixteenth part. Some 2 us, a launch and three loads one
 // after another. (The last part's workgroup joining them itself would save the
 // launch, but read all of a row's states, 640 KB for 157 parts of four heads,
 // through one compute unit: 16 us.)

@@ -12,6 +12,10 @@
 // values are D / 8 lanes, as in paged_rope.hip, and its rows the workgroup's
 // groups of lanes. Queries are turned by workgroups of their own.
 //
+// What bounds it is a chain of loads: the step's positions, the table, the block's
+// scale and rows, between launch and store. A token's kernel takes 4.2 us (2 of it a
+// launch's), 61 requests' 5.4, 507 rows of three prompts (32 + 16 heads of 128) 11.5.
+//
 // Read. A thread takes eight values of a row's keys and of its values, both loads under
 // way together; what bounds it is memory: 95,001 rows of 8 x 128 as BF16 (585 MB) take
 // 110 us, 5.3 TB/s, where a copy of 2 GiB reaches 4.9.
