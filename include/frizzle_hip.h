@@ -236,7 +236,8 @@ int frz_op_draw(frz_device* dev, const uint32_t* candidates_dev,
  * frz_sync waits. They may be made from several threads at once, though not
  * while one of the device's models is made or runs in another (it captures
  * its steps on the stream), and with any device current. Pointers to floats
- * or 16-bit values must be multiples of 16 bytes and strides of 4 floats. */
+ * and to values of 16 or 8 bits must be multiples of 16 bytes (to scales of 4) and
+ * strides of 4 floats. */
 #define FRZ_FORMAT_F16 1
 #define FRZ_FORMAT_I8 24
 #define FRZ_FORMAT_BF16 30
