@@ -122,9 +122,9 @@ struct Types<kCacheBf16> {
 };
 
 // Numbers of 8 bits are F16 to their weights.
+constexpr int kDigits = 4;  // of a query
 template <>
 struct Types<kCacheI8> : Types<kCacheF16> {
-  static constexpr int kDigits = 4;    // of a query
   static constexpr int kQueryTop = 29;
   static constexpr int kMostUp = 138;  // the query is at most 2^138 times itself
   static __device__ __forceinline__ i32x4 mfma_digits(uint4 a, uint4 b, i32x4 c) {
@@ -141,7 +141,7 @@ struct Shape {
   static constexpr int kParts = Types<kF>::kParts;
   static constexpr int kPerTile = 16 / kW;                              // parts a column tile holds
   static constexpr int kTiles = (kParts + kPerTile - 1) / kPerTile;     // column tiles
-  static constexpr int kQueryTiles = kI8 ? 4 / kPerTile : kTiles;
+  static constexpr int kQueryTiles = kI8 ? kDigits / kPerTile : kTiles;
   // Tiles whose query is not scaled alike, and so whose sums are apart.
   static constexpr int kScales = kF == kCacheBf16 ? 1 : kQueryTiles;
   static constexpr bool kSpare = kTiles * kPerTile > kParts;            // columns of no part
@@ -157,7 +157,7 @@ struct Shape {
 // of 8 bits one, though two would fit (61 requests 17.9 us, 20.6 by two; long ones 130
 // and 136).
 template <int kD, CacheFormat kF, int kW>
-constexpr int kWorkgroups = kD == 256   ? (1)
+constexpr int kWorkgroups = kD == 256   ? 1
                             : kD == 128 ? (Shape<kD, kF, kW>::kTiles == 1 ? 3 : 2)
                                         : (Shape<kD, kF, kW>::kTiles <= 2 ? 4 : 3);
 template <int kD, CacheFormat kF, int kW>
@@ -350,6 +350,11 @@ void paged_attention_kernel(PagedAttentionArgs a) {
   constexpr int kPitch = kD + 8;  // floats a head's outputs take in LDS
   __shared__ __attribute__((aligned(16))) float joined_out[kWaves][kW * kPitch];
   __shared__ float joined_m[kWaves][kW], joined_l[kWaves][kW], joined_top[kWaves];
+  // Of 8 bits the waves share the query's digits, a wave every fourth piece of them.
+  constexpr int kOwn = S::kI8 ? (S::kChunks + kWaves - 1) / kWaves : S::kChunks;
+  constexpr bool kShared = S::kI8 && kWaves > 1;
+  __shared__ uint4 digits[kShared ? S::kQueryTiles * S::kChunks : 1][64];
+  __shared__ float largest[kShared ? kWaves : 1][16];
   const int lane = threadIdx.x & 63;
   const uint32_t wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int n = lane & 15, g = lane >> 4;
@@ -427,15 +432,17 @@ void paged_attention_kernel(PagedAttentionArgs a) {
   Column<kF> columns[S::kTiles];
 #pragma unroll
   for (int t = 0; t < S::kTiles; ++t) columns[t] = Column<kF>(t * S::kPerTile + n / kW);
-  float x[S::kChunks][S::kPiece];
+  float x[kOwn][S::kPiece];
   {
     const float* src =
         a.query + (uint64_t)part.row * a.q_stride + (uint64_t)(head0 + (head < heads ? head : 0)) * kD;
 #pragma unroll
-    for (int c = 0; c < S::kChunks; ++c)
+    for (int c = 0; c < kOwn; ++c)
 #pragma unroll
       for (int i = 0; i < S::kPiece; i += 4) {
-        const float4 v = *reinterpret_cast<const float4*>(src + S::kPiece * (4 * c + g) + i);
+        // (A wave past the last piece takes that again.)
+        const int at = kShared ? min(c * kWaves + (int)wave, S::kChunks - 1) : c;
+        const float4 v = *reinterpret_cast<const float4*>(src + S::kPiece * (4 * at + g) + i);
         x[c][i] = v.x;
         x[c][i + 1] = v.y;
         x[c][i + 2] = v.z;
@@ -543,7 +550,8 @@ void paged_attention_kernel(PagedAttentionArgs a) {
     k->lo[0] = k->lo[1] = k->hi[0] = k->hi[1] = 0;  // no row
     return false;
   };
-  if (seek(&now)) {
+  const bool some = seek(&now);
+  if (S::kI8 || some) {
     load_keys(now);
     load_values(now);
     hold();
@@ -556,11 +564,18 @@ void paged_attention_kernel(PagedAttentionArgs a) {
       // which flipping the bytes' top bits takes off again.
       float most = 0.0f;  // NaN where one is
 #pragma unroll
-      for (int c = 0; c < S::kChunks; ++c)
+      for (int c = 0; c < kOwn; ++c)
 #pragma unroll
         for (int i = 0; i < S::kPiece; ++i)
           most = __builtin_elementwise_maximum(most, __builtin_fabsf(x[c][i]));
       most = across_groups(most, [](float p, float r) { return __builtin_elementwise_maximum(p, r); });
+      if constexpr (kShared) {
+        if (g == 0) largest[wave][n] = most;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w)
+          most = __builtin_elementwise_maximum(most, largest[w][n]);
+      }
       int up = 127 + T::kQueryTop - (int)(float_to_bits(most) >> 23);
       up = up > T::kMostUp ? T::kMostUp : up;
       // 2^12 here and 2^-12 in the digits' scales keep both ordinary numbers.
@@ -573,7 +588,7 @@ void paged_attention_kernel(PagedAttentionArgs a) {
         // Byte `digit` of two words, next to each other.
         const uint32_t pick = digit | (4 + digit) << 8 | 0x0C0C0000u;
 #pragma unroll
-        for (int c = 0; c < S::kChunks; ++c) {
+        for (int c = 0; c < kOwn; ++c) {
           uint32_t w[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -584,8 +599,21 @@ void paged_attention_kernel(PagedAttentionArgs a) {
             w[i] = (__builtin_amdgcn_perm(z[1], z[0], pick) |
                     __builtin_amdgcn_perm(z[3], z[2], pick) << 16) ^ 0x80808080u;
           }
-          q[t][c] = make_uint4(w[0], w[1], w[2], w[3]);
+          const uint4 piece = make_uint4(w[0], w[1], w[2], w[3]);
+          if constexpr (kShared) {
+            const int at = c * kWaves + (int)wave;
+            if (at < S::kChunks) digits[t * S::kChunks + at][lane] = piece;
+          } else {
+            q[t][c] = piece;
+          }
         }
+      }
+      if constexpr (kShared) {
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < S::kQueryTiles; ++t)
+#pragma unroll
+          for (int c = 0; c < S::kChunks; ++c) q[t][c] = digits[t * S::kChunks + c][lane];
       }
     } else {
       float most = 0.0f;
@@ -615,7 +643,7 @@ void paged_attention_kernel(PagedAttentionArgs a) {
         }
       }
     }
-    for (bool more = true; more;) {
+    for (bool more = some; more;) {
       typedef typename std::conditional<S::kI8, i32x4, f32x4>::type Sums;
       Sums scores[2][S::kScales];
 #pragma unroll
