@@ -62,7 +62,7 @@
 // 8,192 keys (99 MB) 24.5 us, 4.0 TB/s; 32 of 1 to 4,001 keys, 8 BF16 key-value
 // heads of 128 (70 MB), 20.0 us, 3.5 TB/s; one of 5,004 keys (5 MB) 10.1 us,
 // two launches of dependent loads. The same of 8 bits: 130 us (702 MB, 5.4 TB/s),
-// 17.9, 16.1 and 11.0. 29 requests' first 130 and last 4,000 keys, 8 BF16 heads of
+// 16.4, 15.8 and 10.8. 29 requests' first 130 and last 4,000 keys, 8 BF16 heads of
 // 128 (491 MB), 99 us, 5.0 TB/s.
 
 #include <type_traits>
@@ -154,8 +154,8 @@ struct Shape {
 };
 
 // Workgroups a compute unit runs at once, by the registers that a shape takes; 256 wide
-// of 8 bits one, though two would fit (61 requests 17.9 us, 20.6 by two; long ones 130
-// and 136).
+// of 8 bits one, though two would fit (61 requests 16.4 us, 18.7 by two; long ones 130
+// and 134).
 template <int kD, CacheFormat kF, int kW>
 constexpr int kWorkgroups = kD == 256   ? 1
                             : kD == 128 ? (Shape<kD, kF, kW>::kTiles == 1 ? 3 : 2)
@@ -350,7 +350,10 @@ void paged_attention_kernel(PagedAttentionArgs a) {
   constexpr int kPitch = kD + 8;  // floats a head's outputs take in LDS
   __shared__ __attribute__((aligned(16))) float joined_out[kWaves][kW * kPitch];
   __shared__ float joined_m[kWaves][kW], joined_l[kWaves][kW], joined_top[kWaves];
-  // Of 8 bits the waves share the query's digits, a wave every fourth piece of them.
+  // Of 8 bits the waves share the query's digits, a wave every fourth piece of them (61
+  // requests 16.4 us, 17.9 by waves of all their own). Of 16 bits, whose parts take
+  // fewer instructions, a row of few keys waits longer for it than it spares (one of
+  // 5,004 10.1 -> 10.4 us, though 61 24.5 -> 23.8).
   constexpr int kOwn = S::kI8 ? (S::kChunks + kWaves - 1) / kWaves : S::kChunks;
   constexpr bool kShared = S::kI8 && kWaves > 1;
   __shared__ uint4 digits[kShared ? S::kQueryTiles * S::kChunks : 1][64];
