@@ -5,7 +5,7 @@ import math
 import numpy as np
 
 import frizzle_amd as fz
-from _batch import BF16, F16, F32, NONE, Paged, of_format, ptr
+from _batch import F16, NONE, Paged, of_format, ptr, to_format
 from frizzle_amd import _lib
 
 I8 = 24
@@ -153,7 +153,6 @@ def read(device, paged, requests, positions, fmt, stride=None, start=7.0):
     """The op's keys and values, [row][stride] bits of `fmt`; rows start at 7."""
     rows, size = len(positions), paged.kv * paged.dim
     stride = stride or size
-    from _batch import to_format
     out = [device.array(np.broadcast_to(to_format(np.array([start]), fmt), (rows, stride)).copy())
            for _ in range(2)]
     dp = device.array(np.asarray(positions, np.uint32))
@@ -248,7 +247,7 @@ def check(device, paged, positions, query, heads, window, scale, requests=None, 
     return got
 
 
-def any_pool(device, rng, lengths, kv, dim, slots, fmt, wide=0):
+def any_pool(device, rng, lengths, kv, dim, slots, fmt=F16, wide=0):
     if fmt == I8:
         return Paged8(device, rng, lengths, kv, dim, slots, wide=wide)
     return Paged(device, rng, lengths, kv, dim, slots, fmt, wide=wide)

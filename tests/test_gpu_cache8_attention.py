@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 import frizzle_amd as fz
-from _batch import NONE, F32
+from _batch import NONE
 from _cache8 import BLOCK, Paged8, attention, check, exact
 
 pytestmark = pytest.mark.gpu
@@ -203,3 +203,39 @@ def test_the_most_rows_and_heads(device):
     check(device, paged, positions, query, 4, 64, 0.125)
     paged, query, positions = batch(device, 7, [33, 0, 150], 1024, 512, 64, 16)
     check(device, paged, positions, query, 1024, NONE, 0.125)
+
+
+def test_a_pool_past_32_bits(device):
+    # Pages 2^31 numbers and 2^29 scales apart: the last begin at 2^32 and 2^32 bytes.
+    from frizzle_amd import _lib
+    rng = np.random.default_rng(22)
+    dim, slots, pages, stride, scale_stride = 256, 16, 3, 1 << 31, 1 << 29
+    lib = fz.load()
+    big = fz.runtime.DeviceArray(device, stride * (pages - 1) + 2 * slots * dim, np.uint8, (1,))
+    far = fz.runtime.DeviceArray(device, 4 * (scale_stride * (pages - 1) + 2), np.uint8, (1,))
+    codes = rng.integers(-127, 128, (pages, 2, slots, dim)).astype(np.int8)
+    scales = np.exp2(rng.integers(-7, -4, (pages, 2))).astype(np.float32)
+    for p in range(pages):
+        _lib.check(lib.frz_write(device.handle, big.ptr + stride * p,
+                                 np.ascontiguousarray(codes[p]).ctypes.data, codes[p].nbytes))
+        _lib.check(lib.frz_write(device.handle, far.ptr + 4 * scale_stride * p,
+                                 np.ascontiguousarray(scales[p]).ctypes.data, scales[p].nbytes))
+    table = device.array(np.array([[2, 0, 1]], np.uint32))
+    positions = device.array(np.array([44], np.uint32))
+    query = rng.normal(0, 1.5, (1, 1024)).astype(np.float32)
+    dq, do = device.array(query), device.empty((1, 1024), np.float32)
+    c = fz.Pages(big.ptr, big.ptr + slots * dim, 24, 1, dim, slots, pages, stride, table.ptr, 1, 3,
+                 far.ptr, far.ptr + 4, scale_stride)
+    _lib.check(lib.frz_op_attention_paged(device.handle, c, None, positions.ptr, dq.ptr, 1024,
+                                          do.ptr, 1024, 4, NONE, 1 / 16, 1))
+    device.sync()
+    got = do.numpy()[0].reshape(4, dim)
+    big.free()
+    far.free()
+    order = [2, 0, 1]
+    k, v = ((codes[order, i].astype(np.float64) * scales[order, i][:, None, None])
+            .reshape(-1, dim)[:45] for i in (0, 1))
+    s = query.astype(np.float64).reshape(4, dim) @ k.T / 16
+    w = np.exp(s - s.max(1, keepdims=True))
+    want = w / w.sum(1, keepdims=True) @ v
+    assert np.linalg.norm(got - want) <= 5e-6 * np.linalg.norm(want)

@@ -1,10 +1,10 @@
 """Attention over a request's first keys and a window, over caches of every format,
-against 64 bits; and a step of appends, attention and reads together."""
+against 64 bits."""
 import numpy as np
 import pytest
 
-from _batch import BF16, F16, F32, NONE, attention as plain
-from _cache8 import I8, any_pool, attention, check, read
+from _batch import BF16, F16, NONE, attention as plain
+from _cache8 import I8, any_pool, attention, check
 
 pytestmark = pytest.mark.gpu
 
