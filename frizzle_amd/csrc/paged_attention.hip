@@ -977,7 +977,18 @@ hipError_t launch_shape(hipStream_t s, PagedAttentionArgs a, uint32_t heads, int
   // are cut (those 483 take the 127).
   const uint64_t blocks =
       most_row_blocks((uint64_t)a.cache.width * a.cache.page_slots, a.window, a.sinks);
-  if (units >= a.at_once && blocks <= kWaveBlocks) {
+  // Of 8 bits a workgroup's waves are through a row sooner, so that only rows of few
+  // blocks go a wave each, the fewer the less there is for all waves to do: one where
+  // workgroups run at once, 13 where a quarter of the waves still do, any where all have a
+  // unit each (128 requests of 10 to 500 keys, 8 heads of 128, 21.2 us by waves, 15.1 by
+  // workgroups; 200 of 1 to 64 8.0 and 10.9).
+  uint64_t most = kWaveBlocks;
+  if (S::kI8) {
+    const uint32_t held = a.at_once * (kD == 256 && kW < 16 ? 2 : 1);  // two fit, though
+    if (units < kPartWaves * held)
+      most = units > held ? 1 + (uint64_t)kPartWaves * (units - held) / held : 1;
+  }
+  if (units >= a.at_once && blocks <= most) {
     hipLaunchKernelGGL((paged_attention_kernel<kD, kF, kW, 1, true>), grid(units), dim3(64), 0,
                        s, a);
     return hipGetLastError();

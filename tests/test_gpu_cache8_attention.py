@@ -61,6 +61,17 @@ def test_many_short_rows(device, dim, group, window):
     check(device, paged, positions, query, 4 * group, window, dim ** -0.5)
 
 
+# As many units as waves run at once, and fewer of fewer blocks: a wave each.
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows,group,kv,most", [(512, 1, 8, 90), (500, 6, 8, 40), (512, 12, 8, 33),
+                                                (300, 3, 4, 31), (400, 2, 1, 32)])
+def test_rows_of_a_wave_each(device, dim, rows, group, kv, most):
+    rng = np.random.default_rng(dim + rows)
+    lengths = [int(n) for n in rng.integers(0, most + 1, rows)]
+    paged, query, positions = batch(device, group, lengths, kv * group, kv, dim, 16)
+    check(device, paged, positions, query, kv * group, NONE, dim ** -0.5)
+
+
 @TABLES
 def test_rows_of_a_request_in_any_order_and_requests_that_are_not_there(device, keys):
     rng = np.random.default_rng(9)
