@@ -975,13 +975,13 @@ hipError_t launch_shape(hipStream_t s, PagedAttentionArgs a, uint32_t heads, int
   // heads 128 wide: 214 by workgroups, 257 by waves). The host knows the table's
   // width and the window, not the rows: short rows in a wide table without a window
   // are cut (those 483 take the 127).
-  const uint64_t blocks =
-      most_row_blocks((uint64_t)a.cache.width * a.cache.page_slots, a.window, a.sinks);
-  // Of 8 bits a workgroup's waves are through a row sooner, so that only rows of few
-  // blocks go a wave each, the fewer the less there is for all waves to do: one where
-  // workgroups run at once, 13 where a quarter of the waves still do, any where all have a
-  // unit each (128 requests of 10 to 500 keys, 8 heads of 128, 21.2 us by waves, 15.1 by
-  // workgroups; 200 of 1 to 64 8.0 and 10.9).
+  const uint64_t capacity = (uint64_t)a.cache.width * a.cache.page_slots;
+  const uint64_t blocks = most_row_blocks(capacity, a.window, a.sinks);
+  // Of 8 bits a workgroup's waves are through a row sooner, so that rows go a wave each
+  // only if they have few blocks: one where all units' workgroups run at once, up to 12
+  // where nearly every wave that does has a unit, any number from there on (128 requests
+  // of 10 to 500 keys, 8 heads of 128, 21.2 us by waves, 15.1 by workgroups; 200 of 1 to
+  // 64 8.0 and 10.9).
   uint64_t most = kWaveBlocks;
   if (S::kI8) {
     const uint32_t held = a.at_once * (kD == 256 && kW < 16 ? 2 : 1);  // two fit, though
@@ -994,7 +994,13 @@ hipError_t launch_shape(hipStream_t s, PagedAttentionArgs a, uint32_t heads, int
     return hipGetLastError();
   }
   const bool few = 8 * units < 3 * (uint32_t)compute_units;
-  if (blocks * kD <= (few ? kFewValues : kManyValues)) {
+  // Twice as many where it is the window that leaves rows short, which makes them alike
+  // (rows of a table this wide may be one long one among short): of 8 bits (100 of a
+  // window of 1,024, 256 wide, 21.0 us cut, 17.1 whole; 32 of 300 10.4 and 9.1), and of
+  // 16 where units are half of what runs at once (200 of 1,024 47 and 41, 100 of 2,000
+  // with 4 heads of 128 108 and 84; but 100 of 1,024 30 and 32).
+  const bool alike = blocks * kBlockKeys < capacity && (S::kI8 || 2 * units >= a.at_once);
+  if (blocks * kD <= (alike ? 2 : 1) * (few ? kFewValues : kManyValues)) {
     hipLaunchKernelGGL((paged_attention_kernel<kD, kF, kW, kPartWaves, true>), grid(units),
                        dim3(64 * kPartWaves), 0, s, a);
     return hipGetLastError();

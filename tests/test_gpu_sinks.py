@@ -52,6 +52,18 @@ def test_many_rows(device, fmt):
     check(device, paged, positions, query, 4, 60, 0.125, sinks=18)
 
 
+# Rows of a wide table that a window leaves short: a workgroup each.
+@FORMATS
+@pytest.mark.parametrize("rows,heads,kv,dim,window,sinks", [
+    (150, 4, 1, 256, 900, 10), (33, 4, 1, 256, 300, 4), (100, 8, 4, 128, 1900, 33),
+    (70, 40, 2, 64, 2500, 1)])
+def test_many_rows_of_a_window(device, fmt, rows, heads, kv, dim, window, sinks):
+    rng = np.random.default_rng(rows)
+    lengths = [int(n) for n in rng.integers(0, 2 * window, rows)]
+    paged, query, positions = batch(device, rows, lengths, heads, kv, dim, 32, fmt, wide=200)
+    check(device, paged, positions, query, heads, window, dim ** -0.5, sinks=sinks)
+
+
 @FORMATS
 def test_pages_between_that_are_gone_or_hold_anything(device, fmt):
     # What lies between first keys and window is other requests', or nothing: also the
