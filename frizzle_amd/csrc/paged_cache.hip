@@ -255,34 +255,39 @@ void launch_rope(hipStream_t s, const PagedRopeArgs& a) {
 // ---- reading back --------------------------------------------------------------
 
 constexpr uint32_t kThreads = 256;
-constexpr int kPiece = 8;  // values that a thread takes at once, 16 bytes of output or 32
+// Values that a thread takes at once: 16 bytes of output, so that each of a wave's stores
+// fills whole lines. 40,000 rows of 8 x 128 bytes as F32 by 8 values and two stores:
+// 153 us; so 60 (6.8 TB/s).
+template <int kTo>
+constexpr int kPieceOf = kTo == 0 ? 4 : 8;
 // Outputs past what the L2 caches hold (8 of 4 MB) go past them too, and a thread then
 // takes two pieces, all loads first. 40,000 rows of 8 x 128 as BF16 (160 MB): 54 us by
 // one piece, 52 by two, 37 past the caches; 95,001 rows 126, 118 and 110. A window's 512
-// of 256, as F16: 3.0 by one piece, 4.0 by two.
+// of 256, as F16: 3.0 by one piece, 4.0 by two. 10,000 rows as F32: 24.2 us in the caches,
+// 16.4 past them.
 constexpr uint64_t kCachedBytes = 32u << 20;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // A piece of a cache row.
-template <CacheFormat kFrom>
+template <CacheFormat kFrom, int kPiece>
 struct Piece {
-  static constexpr int kWords = kFrom == kCacheI8 ? 2 : 4;
+  static constexpr int kWords = kFrom == kCacheI8 ? kPiece / 4 : kPiece / 2;
+  typedef uint32_t Words __attribute__((ext_vector_type(kWords)));
   uint32_t words[kWords];
   float scale;
   __device__ __forceinline__ void load(const void* pool, uint64_t at, const float* scales,
                                        uint64_t scale_at) {
     if constexpr (kFrom == kCacheI8) {
-      const uint2 r = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(pool) + at);
-      words[0] = r.x;
-      words[1] = r.y;
+      take(static_cast<const uint8_t*>(pool) + at);
       scale = scales[scale_at];
     } else {
-      const uint4 r = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(pool) + at);
-      words[0] = r.x;
-      words[1] = r.y;
-      words[2] = r.z;
-      words[3] = r.w;
+      take(static_cast<const uint16_t*>(pool) + at);
     }
+  }
+  __device__ __forceinline__ void take(const void* from) {
+    const Words w = *static_cast<const Words*>(from);
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) words[i] = w[i];
   }
   __device__ __forceinline__ float get(int i) const {
     if constexpr (kFrom == kCacheI8)
@@ -306,15 +311,13 @@ __device__ __forceinline__ void put(void* dst, u32x4 v) {
 }
 
 template <CacheFormat kFrom, int kTo, bool kPast>
-__device__ __forceinline__ void store(void* to, uint64_t at, const Piece<kFrom>& piece, bool there) {
+__device__ __forceinline__ void store(void* to, uint64_t at,
+                                      const Piece<kFrom, kPieceOf<kTo>>& piece, bool there) {
   if constexpr (kTo == 0) {
+    u32x4 w;
 #pragma unroll
-    for (int i = 0; i < kPiece; i += 4) {
-      u32x4 w = {0, 0, 0, 0};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = there ? float_to_bits(piece.get(i + j)) : 0u;
-      put<kPast>(static_cast<float*>(to) + at + i, w);
-    }
+    for (int j = 0; j < 4; ++j) w[j] = there ? float_to_bits(piece.get(j)) : 0u;
+    put<kPast>(static_cast<float*>(to) + at, w);
   } else {
     u32x4 w;
 #pragma unroll
@@ -333,7 +336,8 @@ __global__ __launch_bounds__(kThreads) void paged_read_kernel(PagedReadArgs a, u
   const uint32_t first = blockIdx.x * rows_each;
   const uint32_t count = min(rows_each, a.rows - first) * row_pieces;
   const uint32_t from = blockIdx.y * kPieces * kThreads + threadIdx.x;
-  Piece<kFrom> key[kPieces], value[kPieces];
+  constexpr int kPiece = kPieceOf<kTo>;
+  Piece<kFrom, kPiece> key[kPieces], value[kPieces];
   bool there[kPieces], live[kPieces];
   uint32_t row[kPieces], piece[kPieces], p[kPieces], sequence[kPieces];
 #pragma unroll
@@ -374,7 +378,7 @@ __global__ __launch_bounds__(kThreads) void paged_read_kernel(PagedReadArgs a, u
 template <CacheFormat kFrom, int kTo, uint32_t kPieces>
 void launch_pieces(hipStream_t s, const PagedReadArgs& a) {
   constexpr uint32_t kMost = kPieces * kThreads;
-  const uint32_t pieces = a.cache.kv_heads * a.cache.head_dim / kPiece;
+  const uint32_t pieces = a.cache.kv_heads * a.cache.head_dim / kPieceOf<kTo>;
   const uint32_t rows = pieces < kMost ? kMost / pieces : 1;
   hipLaunchKernelGGL((paged_read_kernel<kFrom, kTo, kPieces>),
                      dim3((a.rows + rows - 1) / rows, (pieces + kMost - 1) / kMost),

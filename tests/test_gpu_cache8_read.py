@@ -104,6 +104,11 @@ def test_more_than_the_caches_hold(device, cache, fmt, kv, dim, rows):
         assert np.array_equal(g, w, equal_nan=g.dtype == np.float32)
 
 
+@pytest.mark.parametrize("cache", [I8, BF16])
+def test_wide_rows_as_f32_past_the_caches(device, cache):
+    test_more_than_the_caches_hold(device, cache, F32, 1024, 64, 75)
+
+
 def test_the_ends_of_the_range(device):
     rng = np.random.default_rng(4)
     paged = Paged8(device, rng, [48], 1, 64, 16)
