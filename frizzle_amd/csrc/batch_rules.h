@@ -103,6 +103,28 @@ FRZ_RULE uint64_t most_row_blocks(uint64_t capacity, uint32_t window, uint32_t s
   return most ? most : 1;
 }
 
+// Whether no row is cut, for their most blocks: up to kFewValues (blocks times head_dim)
+// always (64 requests of up to 250 keys, 256 wide, 12.6 us cut, 10.8 whole), to
+// kManyValues where the units keep the compute units at work (100 of a window of 512:
+// 22.6 and 17.2; but 16: 11.9 and 16.0). No further, though a window leaves rows alike
+// that have outgrown it: of those that have not, the longest is still at it when the
+// others are done (130 rows of 100 to 2,000 keys, window 2,000, F16, 256 wide, 37 us cut,
+// 51 whole; 300 74 and 84), and one more unit than runs at once is a second round.
+// A row of 8 bits takes 6 us and 0.3 a block, whatever its width but for the narrowest's
+// 0.2, and is then as short as cut ones' two launches (256 wide, whole and cut, of rows
+// past the window, of 100 to 2,000 keys, of one of those among some of 100): 32 rows,
+// window 400, 10.5 and 10.7, 10.4 and 10.6, 10.0 and 10.3; but window 600 12.0 and 11.3,
+// 11.9 and 11.1, 11.2 and 10.3; 100 rows, window 1,000, 17.1 and 19.6, 17.1 and 17.2,
+// 15.5 and 14.3; but window 1,400 21.3 and 23.1, 20.9 and 18.8, 19.9 and 14.2.
+constexpr uint64_t kFewValues = 2048, kManyValues = 8192;
+constexpr uint64_t kFewBlocksI8 = 16, kManyBlocksI8 = 36;
+FRZ_RULE bool uncut(uint64_t blocks, uint32_t head_dim, bool i8, uint32_t units,
+                    uint32_t compute_units) {
+  const bool few = 8ull * units < 3ull * compute_units;
+  if (blocks * head_dim <= (few ? kFewValues : kManyValues)) return true;
+  return i8 && blocks <= (few ? kFewBlocksI8 : kManyBlocksI8);
+}
+
 // ---- caches of 8 bits ----------------------------------------------------------
 
 constexpr uint32_t kScaleSlots = 16;  // tokens that share a scale

@@ -84,9 +84,7 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 
 constexpr float kMinusInf = -__builtin_inff();
 constexpr float kLargest = 0x1.fffffep127f;
-// Rows of no more blocks than these, or blocks times head_dim, are not cut: see
-// launch_shape.
-constexpr uint64_t kWaveBlocks = 32, kFewValues = 2048, kManyValues = 8192;
+constexpr uint64_t kWaveBlocks = 32;  // of rows that go a wave each: see launch_shape
 constexpr int kBufferWord3 = 0x00020000;  // raw 32-bit data
 constexpr uint32_t kDies = 8;  // workgroups go to them in turn
 constexpr float kLeastTop = 0x1p-126f;
@@ -963,18 +961,14 @@ hipError_t launch_shape(hipStream_t s, PagedAttentionArgs a, uint32_t heads, int
     const uint32_t even = a.shared_units > 1 ? kDies * a.shared_units : 1;
     return dim3((uint32_t)((n + even - 1) / even * even));
   };
-  // The most blocks that a row can have. Where they are few, each unit is one
-  // workgroup's (kWhole), which then need not find its part, nor leave a state
-  // to a second launch: always to kFewValues (64 requests of up to 250 keys, 256
-  // wide, 12.6 us cut, 10.8 whole), and to kManyValues where enough units are
-  // there to keep the compute units at work (100 of a window of 512: 22.6 and
-  // 17.2; but 16: 11.9 and 16.0). Where more units are there than workgroups run
-  // at once, a unit is a wave's: four waves would each have had a block or two
-  // of a short row (483 rows of 16 to 31 keys, 8 key-value heads, 256 wide, 127
-  // us and 35; 512 of a window of 512 67 and 52; not of 63 blocks, 400 rows of 8
-  // heads 128 wide: 214 by workgroups, 257 by waves). The host knows the table's
-  // width and the window, not the rows: short rows in a wide table without a window
-  // are cut (those 483 take the 127).
+  // The most blocks that a row can have. Where they are few (uncut), each unit is one
+  // workgroup's (kWhole), which then need not find its part, nor leave a state to a
+  // second launch. Where more units are there than workgroups run at once, a unit is a
+  // wave's: four waves would each have had a block or two of a short row (483 rows of 16
+  // to 31 keys, 8 key-value heads, 256 wide, 127 us and 35; 512 of a window of 512 67 and
+  // 52; not of 63 blocks, 400 rows of 8 heads 128 wide: 214 by workgroups, 257 by waves).
+  // The host knows the table's width and the window, not the rows: short rows in a wide
+  // table without a window are cut (those 483 take the 127).
   const uint64_t capacity = (uint64_t)a.cache.width * a.cache.page_slots;
   const uint64_t blocks = most_row_blocks(capacity, a.window, a.sinks);
   // Of 8 bits a workgroup's waves are through a row sooner, so that rows go a wave each
@@ -993,14 +987,7 @@ hipError_t launch_shape(hipStream_t s, PagedAttentionArgs a, uint32_t heads, int
                        s, a);
     return hipGetLastError();
   }
-  const bool few = 8 * units < 3 * (uint32_t)compute_units;
-  // Twice as many where it is the window that leaves rows short, which makes them alike
-  // (rows of a table this wide may be one long one among short): of 8 bits (100 of a
-  // window of 1,024, 256 wide, 21.0 us cut, 17.1 whole; 32 of 300 10.4 and 9.1), and of
-  // 16 where units are half of what runs at once (200 of 1,024 47 and 41, 100 of 2,000
-  // with 4 heads of 128 108 and 84; but 100 of 1,024 30 and 32).
-  const bool alike = blocks * kBlockKeys < capacity && (S::kI8 || 2 * units >= a.at_once);
-  if (blocks * kD <= (alike ? 2 : 1) * (few ? kFewValues : kManyValues)) {
+  if (uncut(blocks, kD, S::kI8, units, (uint32_t)compute_units)) {
     hipLaunchKernelGGL((paged_attention_kernel<kD, kF, kW, kPartWaves, true>), grid(units),
                        dim3(64 * kPartWaves), 0, s, a);
     return hipGetLastError();
