@@ -579,13 +579,17 @@ void paged_attention_kernel(PagedAttentionArgs a) {
       }
       int up = 127 + T::kQueryTop - (int)(float_to_bits(most) >> 23);
       up = up > T::kMostUp ? T::kMostUp : up;
-      // 2^12 here and 2^-12 in the digits' scales keep both ordinary numbers.
-      key_back = a.scale_log2e * __builtin_ldexpf(1.0f, 12 - up);
+      // Of a power below 2^-100 the rest lies in the digits' scales, so that what meets
+      // the blocks' scales, which may make up for it, has all of its bits; one of the
+      // digits' is 0 only where its part of a score is below 2^-90.
+      const int power = __builtin_amdgcn_frexp_expf(a.scale_log2e) - up;
+      const int here = power < -100 ? -100 : power;
+      key_back = __builtin_ldexpf(__builtin_amdgcn_frexp_mantf(a.scale_log2e), here);
       if (!(most <= kLargest)) key_back = __builtin_nanf("");
 #pragma unroll
       for (int t = 0; t < S::kQueryTiles; ++t) {
         const uint32_t digit = t * S::kPerTile + n / kW;
-        scale[t] = bits_to_float((127 - 12 + 8 * digit) << 23);
+        scale[t] = __builtin_ldexpf(1.0f, 8 * (int)digit + power - here);
         // Byte `digit` of two words, next to each other.
         const uint32_t pick = digit | (4 + digit) << 8 | 0x0C0C0000u;
 #pragma unroll
