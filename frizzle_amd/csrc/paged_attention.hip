@@ -47,10 +47,11 @@
 //                       columns n, n + W, n + 2W .. of a head, or further tiles. It
 //                       is held to 2^-30 of its head's largest; sums are exact.
 //   O = (p s_v / t) . c t  on those of F16: a byte and a constant make each c exact,
-//                       p s_v / t is split as above. t is the largest s_v so far, the
-//                       outputs' unit, kept as m is: weights stay below 2^14, and a
-//                       part leaves its outputs over its weights, so that no sum is
-//                       past F32 where no value is.
+//                       p s_v / t is split as above. t is the largest s_v so far
+//                       (of numbers that are not all 0), the outputs' unit, kept as m
+//                       is: weights stay below 2^14, and a part leaves its outputs
+//                       over its weights, so that no sum is past F32 where no value
+//                       is.
 // Values' bytes as F16 are half of a block's 330 vector instructions (256 wide); the
 // query's digits spare the keys' as many.
 //
@@ -727,10 +728,27 @@ void paged_attention_kernel(PagedAttentionArgs a) {
         l += weight[i];
       }
       if constexpr (S::kI8) {
-        // A value's weight has its block's scale in it, over the largest so far.
-        const float here = __builtin_fmaxf(__builtin_fabsf(value_scale[0]),
-                                           __builtin_fabsf(value_scale[1]));
-        if (__ballot(here > top_scale)) {
+        // A value's weight has its block's scale in it, over the largest so far of a
+        // block that is not all zeros to the row: beside the scale of one that is,
+        // whose large values are outside the window or gone, the others' would vanish.
+        auto widest = [&] {
+          return __builtin_fmaxf(__builtin_fabsf(value_scale[0]),
+                                 __builtin_fabsf(value_scale[1]));
+        };
+        if (__ballot(widest() > top_scale)) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t any = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+              for (int s = 0; s < S::kSpans; ++s) {
+                const uint4& r = value_rows[h][e][s];
+                any |= r.x | r.y | r.z | r.w;
+              }
+            if (!__ballot(any != 0)) value_scale[h] = 0.0f;
+          }
+          const float here = __builtin_fmaxf(widest(), top_scale);
           const float old = top_scale / here;
 #pragma unroll
           for (int s = 0; s < S::kSpans; ++s)

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from _batch import NONE
-from _cache8 import Paged8, check
+from _cache8 import BLOCK, Paged8, check
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +35,54 @@ def test_numbers_that_balance(device, dim, heads, kv, keys, query_size, key_powe
     paged.upload()
     query = (query * np.float32(query_size)).astype(np.float32)
     check(device, paged, positions, query, heads, NONE, float(np.float32(scale)))
+
+
+# A block whose numbers are all 0 holds no value, however large its scale, and so does one
+# of whose keys those that are not 0 lie outside the window: the others' outputs keep
+# check()'s bound, of the largest value that is read.
+@pytest.mark.parametrize("dim,heads,kv", [(256, 4, 1), (128, 8, 1), (128, 6, 2), (64, 12, 1)])
+@pytest.mark.parametrize("keys", [0, 16384])
+@pytest.mark.parametrize("power", [18, 30, 60, 121, 127])
+def test_scales_of_blocks_of_zeros(device, dim, heads, kv, keys, power):
+    lengths = [150, 33, 700, 16, 4000]
+    paged, query, positions = batch(device, 32, lengths, heads, kv, dim, 16, wide=keys // 16)
+    codes, scales = paged.codes()[1], paged.scales()[1]
+    rng = np.random.default_rng(33)
+    for r, n in enumerate(lengths):
+        for j in range(0, n, BLOCK):
+            if r == 3 or rng.random() < 0.4:
+                page, head = paged.page(r, j), rng.integers(0, kv)
+                codes[page, :, head] = 0
+                scales[page, 0, head] = 2.0 ** power
+    paged.upload()
+    for window, sinks in ((NONE, 0), (100, 0), (70, 20)):
+        check(device, paged, positions, query, heads, window, dim ** -0.5, sinks=sinks)
+
+
+@pytest.mark.parametrize("dim,heads,kv", [(256, 4, 1), (128, 8, 1), (64, 12, 1)])
+@pytest.mark.parametrize("keys", [0, 16384])
+def test_scales_of_keys_outside_the_window(device, dim, heads, kv, keys):
+    # The window's first key is the second of its block; what gave the block its scale was
+    # the first, as an append writes it: the others are 0 beside it.
+    lengths = [57 + BLOCK, 200, 713]
+    paged, query, positions = batch(device, 34, lengths, heads, kv, dim, 16, wide=keys // 16)
+    window = 40
+    for r, n in enumerate(lengths):
+        first = n - window
+        page = paged.page(r, first)
+        codes, scales = paged.codes()[1], paged.scales()[1]
+        codes[page, :first % BLOCK + 1] = 127
+        codes[page, first % BLOCK:] = 0
+        scales[page] = 2.0 ** 40
+    paged.upload()
+    check(device, paged, positions, query, heads, window, dim ** -0.5)
+    check(device, paged, positions, query, heads, window, dim ** -0.5, sinks=3)
+
+
+def test_values_of_zeros_alone(device):
+    paged, query, positions = batch(device, 35, [150, 700], 4, 1, 256, 16)
+    paged.codes()[1][:] = 0
+    paged.scales()[1][:] = 2.0 ** 100
+    paged.upload()
+    got = check(device, paged, positions, query, 4, NONE, 1 / 16)
+    assert (got == 0.0).all()
