@@ -199,7 +199,9 @@ int frz_op_rope_paged(frz_device* dev, const frz_pages* cache, const uint32_t* s
   a.query_heads = (uint32_t)query_heads;
   a.epsilon = epsilon;
   a.rows = rows;
-  return enqueue(dev, what, [&] { return launch_paged_rope(dev->stream, a); });
+  return enqueue(dev, what, [&] {
+    return launch_paged_rope(dev->stream, a, dev->props.multiProcessorCount);
+  });
 }
 
 int frz_op_attention_paged(frz_device* dev, const frz_pages* cache, const uint32_t* sequences,

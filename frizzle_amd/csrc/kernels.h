@@ -466,9 +466,9 @@ struct PagedRopeArgs {
   float epsilon;
   uint32_t rows;
 };
-hipError_t launch_paged_rope(hipStream_t s, const PagedRopeArgs& a);
+hipError_t launch_paged_rope(hipStream_t s, const PagedRopeArgs& a, int compute_units);
 // The same into a cache of 8 bits (launch_paged_rope calls it).
-hipError_t launch_paged_rope_i8(hipStream_t s, const PagedRopeArgs& a);
+hipError_t launch_paged_rope_i8(hipStream_t s, const PagedRopeArgs& a, int compute_units);
 
 struct PagedReadArgs {
   PagedCache cache;

@@ -29,7 +29,8 @@ namespace {
 
 using namespace rules;
 
-constexpr uint32_t kRopeThreads = 512, kRopeAtOnce = 1024;
+constexpr uint32_t kRopeThreads = 512;
+constexpr uint32_t kRopeWorkgroups = 4;  // that a compute unit runs at once
 static_assert(kRopeThreads >= kMostRows, "a thread looks at a row");
 
 // A number of the block's scale, rounded to nearest even; NaN is 0.
@@ -232,16 +233,17 @@ __global__ __launch_bounds__(kRopeThreads) void paged_rope_i8_kernel(PagedRopeAr
 }
 
 template <int kD>
-void launch_rope(hipStream_t s, const PagedRopeArgs& a) {
+void launch_rope(hipStream_t s, const PagedRopeArgs& a, int compute_units) {
   constexpr uint32_t kHeads = kRopeThreads / (kD / 8);
   const uint32_t groups = (a.query_heads + kHeads - 1) / kHeads;
   // A tile of one row, or of up to four where workgroups of one would be more than run
-  // at once, four a compute unit. A tile's rows are an odd number apart, so that neither
+  // at once. A tile's rows are an odd number apart, so that neither
   // the first rows of a step nor every sixteenth, which are the first of their blocks
   // where rows lie in any order and in theirs, fall into few tiles. (507 rows in any
   // order, 8 key-value heads: tiles of rows side by side 17 us, these 11.6, of eight
   // such rows 12.5, of one 16.5.)
-  const uint32_t even = (a.rows * a.cache.kv_heads + kRopeAtOnce - 1) / kRopeAtOnce;
+  const uint32_t at_once = kRopeWorkgroups * (uint32_t)compute_units;
+  const uint32_t even = (a.rows * a.cache.kv_heads + at_once - 1) / at_once;
   const uint32_t tile = even < 4 ? even : 4;
   uint32_t tiles = (a.rows + tile - 1) / tile;
   if (tile > 1 && tiles % 2 == 0) ++tiles;
@@ -403,11 +405,12 @@ hipError_t launch_read_to(hipStream_t s, const PagedReadArgs& a) {
 
 }  // namespace
 
-hipError_t launch_paged_rope_i8(hipStream_t s, const PagedRopeArgs& a) {
+hipError_t launch_paged_rope_i8(hipStream_t s, const PagedRopeArgs& a, int compute_units) {
+  if (compute_units <= 0) return hipErrorInvalidValue;
   switch (a.cache.head_dim) {
-    case 64: launch_rope<64>(s, a); break;
-    case 128: launch_rope<128>(s, a); break;
-    case 256: launch_rope<256>(s, a); break;
+    case 64: launch_rope<64>(s, a, compute_units); break;
+    case 128: launch_rope<128>(s, a, compute_units); break;
+    case 256: launch_rope<256>(s, a, compute_units); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();

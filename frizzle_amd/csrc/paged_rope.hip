@@ -124,9 +124,9 @@ void launch_heads(hipStream_t s, const PagedRopeArgs& a) {
 
 }  // namespace
 
-hipError_t launch_paged_rope(hipStream_t s, const PagedRopeArgs& a) {
+hipError_t launch_paged_rope(hipStream_t s, const PagedRopeArgs& a, int compute_units) {
   if (a.rows == 0 || a.rows > kMostRows) return hipErrorInvalidValue;
-  if (a.cache.format == kCacheI8) return launch_paged_rope_i8(s, a);
+  if (a.cache.format == kCacheI8) return launch_paged_rope_i8(s, a, compute_units);
   switch (a.cache.head_dim) {
     case 64: launch_heads<64>(s, a); break;
     case 128: launch_heads<128>(s, a); break;
