@@ -881,7 +881,8 @@ void paged_attention_kernel(PagedAttentionArgs a) {
 // and its 16 groups every sixteenth part. Some 2 us, a launch and three loads one
 // after another. (The last part's workgroup joining them itself would save the
 // launch, but read all of a row's states, 640 KB for 157 parts of four heads,
-// through one compute unit: 16 us.)
+// through one compute unit: 16 us. Rows of few parts so, which have 16 KB in four,
+// were not tried.)
 constexpr uint32_t kJoinWaves = 4, kThreads = 64 * kJoinWaves, kJoinGroups = kThreads / 16;
 // States that a group asks for with the statistics: of up to 64 parts, and of more
 // (few parts take 0.5 us longer where all ask for ten, 157 1.5 where all for four).
@@ -995,7 +996,7 @@ hipError_t launch_shape(hipStream_t s, PagedAttentionArgs a, uint32_t heads, int
   const uint64_t blocks = most_row_blocks(capacity, a.window, a.sinks);
   // Of 8 bits a workgroup's waves are through a row sooner, so that rows go a wave each
   // only if they have few blocks: one where all units' workgroups run at once, up to 12
-  // where nearly every wave that does has a unit, any number from there on (128 requests
+  // where nearly every wave that does has a unit, kWaveBlocks from there on (128 requests
   // of 10 to 500 keys, 8 heads of 128, 21.2 us by waves, 15.1 by workgroups; 200 of 1 to
   // 64 8.0 and 10.9).
   uint64_t most = kWaveBlocks;

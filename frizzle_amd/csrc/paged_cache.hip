@@ -15,10 +15,13 @@
 // What bounds it is a chain of loads: the step's positions, the table, the block's
 // scale and rows, between launch and store. A token's kernel takes 4.2 us (2 of it a
 // launch's), 61 requests' 5.4, 507 rows of three prompts (32 + 16 heads of 128) 11.5.
+// A token of each of 128 requests of 8 key-value heads takes 8.9, of 512 29, where a
+// workgroup has four blocks, and so four such chains, one after another.
 //
-// Read. A thread takes eight values of a row's keys and of its values, both loads under
-// way together; what bounds it is memory: 95,001 rows of 8 x 128 as BF16 (585 MB) take
-// 110 us, 5.3 TB/s, where a copy of 2 GiB reaches 4.9.
+// Read. A thread takes one or two pieces of a row's keys and of its values, 16 bytes of
+// output each, all loads under way together; what bounds it is memory: 95,001 rows of
+// 8 x 128 as BF16 (585 MB) take 110 us, 5.3 TB/s, where a copy of 2 GiB reaches 4.9; of
+// caches of 16 bits (778 MB) 135, 5.7.
 
 #include "batch_rules.h"
 #include "kernels.h"
@@ -87,7 +90,7 @@ __device__ __forceinline__ void norm_and_turn(float4& va, float4& vb, const floa
 // The last workgroups turn queries. The others take a tile of rows and one
 // key-value head, whose keys are half of a workgroup's threads and whose values the
 // other half, and of those rows the blocks that they are the first in the step to be
-// in, one after another: mostly one or none of a prompt's.
+// in, one after another: mostly one or none of a prompt's, of single tokens all.
 template <int kD, uint32_t kTileRows>
 __global__ __launch_bounds__(kRopeThreads) void paged_rope_i8_kernel(PagedRopeArgs a,
                                                                      uint32_t query_groups,

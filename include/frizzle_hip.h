@@ -290,7 +290,8 @@ typedef struct frz_pages {
  * of this step by half of it. A block whose first slot is written is begun anew,
  * and so is one whose scale is not above 0 and finite: nothing of what it held
  * is left, slots not written are 0: a request's positions come in order, one call
- * after another. Infinities count as the largest number, NaN as 0. */
+ * after another. Numbers past 127 * 2^121 (3.376e38), infinities among them, count as
+ * that, NaN as 0. */
 int frz_op_rope_paged(frz_device* dev, const frz_pages* cache, const uint32_t* sequences,
                       const uint32_t* positions, const float* turns, const float* query_gain,
                       const float* key_gain, const float* query, const float* key,
