@@ -558,7 +558,7 @@ void paged_attention_kernel(PagedAttentionArgs a) {
     load_values(now);
     hold();
     float scale[S::kQueryTiles];  // what turns the scaled query's products into log2 units
-    float key_back = 0.0f;        // of 8 bits: the key's scale aside
+    float key_back = 0.0f, key_rest = 1.0f;  // of 8 bits: the key's scale aside
     uint4 q[S::kQueryTiles][S::kChunks];
     if constexpr (S::kI8) {
       // The query as whole numbers below 2^30, four digits of -128 to 127 each:
@@ -580,17 +580,18 @@ void paged_attention_kernel(PagedAttentionArgs a) {
       }
       int up = 127 + T::kQueryTop - (int)(float_to_bits(most) >> 23);
       up = up > T::kMostUp ? T::kMostUp : up;
-      // Of a power below 2^-100 the rest lies in the digits' scales, so that what meets
-      // the blocks' scales, which may make up for it, has all of its bits; one of the
-      // digits' is 0 only where its part of a score is below 2^-90.
+      // Of a power below 2^-100 the rest is a factor of its own, so that what meets the
+      // blocks' scales, which may make up for it, has all of its bits; it is 0 only
+      // where scores are below 2^-70.
       const int power = __builtin_amdgcn_frexp_expf(a.scale_log2e) - up;
       const int here = power < -100 ? -100 : power;
       key_back = __builtin_ldexpf(__builtin_amdgcn_frexp_mantf(a.scale_log2e), here);
+      key_rest = __builtin_ldexpf(1.0f, power - here);
       if (!(most <= kLargest)) key_back = __builtin_nanf("");
 #pragma unroll
       for (int t = 0; t < S::kQueryTiles; ++t) {
         const uint32_t digit = t * S::kPerTile + n / kW;
-        scale[t] = __builtin_ldexpf(1.0f, 8 * (int)digit + power - here);
+        scale[t] = bits_to_float((127 + 8 * digit) << 23);
         // Byte `digit` of two words, next to each other.
         const uint32_t pick = digit | (4 + digit) << 8 | 0x0C0C0000u;
 #pragma unroll
@@ -693,7 +694,7 @@ void paged_attention_kernel(PagedAttentionArgs a) {
           back[i] = scale[i];
           if constexpr (S::kI8) {
             // A query past F32 by numbers that are all 0 is 0; NaN stays.
-            back[i] *= key_back * key_scale[h];
+            back[i] *= key_back * key_scale[h] * key_rest;
             back[i] = __builtin_elementwise_minimum(
                 __builtin_elementwise_maximum(back[i], -kLargest), kLargest);
           }
@@ -748,7 +749,9 @@ void paged_attention_kernel(PagedAttentionArgs a) {
               }
             if (!__ballot(any != 0)) value_scale[h] = 0.0f;
           }
-          const float here = __builtin_fmaxf(widest(), top_scale);
+        }
+        const float here = widest();
+        if (__ballot(here > top_scale)) {
           const float old = top_scale / here;
 #pragma unroll
           for (int s = 0; s < S::kSpans; ++s)
