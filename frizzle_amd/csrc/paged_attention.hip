@@ -63,7 +63,7 @@
 // 8,192 keys (99 MB) 24.5 us, 4.0 TB/s; 32 of 1 to 4,001 keys, 8 BF16 key-value
 // heads of 128 (70 MB), 20.0 us, 3.5 TB/s; one of 5,004 keys (5 MB) 10.1 us,
 // two launches of dependent loads. The same of 8 bits: 130 us (702 MB, 5.4 TB/s),
-// 16.4, 15.8 and 10.8. 29 requests' first 130 and last 4,000 keys, 8 BF16 heads of
+// 16.6, 16.0 and 10.9. 29 requests' first 130 and last 4,000 keys, 8 BF16 heads of
 // 128 (491 MB), 99 us, 5.0 TB/s.
 
 #include <type_traits>
@@ -732,6 +732,8 @@ void paged_attention_kernel(PagedAttentionArgs a) {
         // A value's weight has its block's scale in it, over the largest so far of a
         // block that is not all zeros to the row: beside the scale of one that is,
         // whose large values are outside the window or gone, the others' would vanish.
+        // (0.1 to 0.3 us a call; to look at the first block only once one far below it
+        // is there takes as long, and more registers.)
         auto widest = [&] {
           return __builtin_fmaxf(__builtin_fabsf(value_scale[0]),
                                  __builtin_fabsf(value_scale[1]));
